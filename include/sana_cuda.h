@@ -468,6 +468,131 @@ int sana_cuda_prompt_pairs_device(sana_cuda_ctx *ctx, int pairs, const float *ne
                                   const float *positive, int positive_rows, const int *positive_real, int hidden,
                                   int L, float *enc, float *bias);
 
+/* --- operators of the text encoder's blocks (device pointers) -------------------------------
+ * The denoiser reads the hidden states of a decoder-only text encoder (Gemma-2 in the
+ * reference, gemma_encoder.cpp:188-244, which runs it through llama.cpp). These are the
+ * operators of such an encoder's blocks around the dense products that sana_op_gemm_device
+ * offers, in the forms a server of prompts needs: prompts of different lengths as the rows of
+ * one batch, keys and values in a paged cache whose instruction prefix is computed once and
+ * shared, and single tokens for prompt rewriting. No reference counterpart (llama.cpp's).
+ *
+ * All take device pointers of the handle's device (whatever device is current), queue their
+ * work on the handle's stream, allocate nothing, never wait for the device and may be captured
+ * into a CUDA graph. Argument errors that the host can see are SANA_ERR_INVALID and launch
+ * nothing. What only the device sees (a page number outside the pool, a sequence longer than
+ * the table, more new tokens than `max_new` or than `rows`, an offset beyond the rows) is
+ * checked there: the kernels access nothing out of range, leave out the keys or rows
+ * concerned, and record it; the next sana_cuda_synchronize (or host-buffer call) of the handle
+ * returns SANA_ERR_INVALID once and clears the record. */
+enum { SANA_DTYPE_F32 = 0, SANA_DTYPE_BF16 = 1, SANA_DTYPE_E4M3 = 2 };
+
+/* Residual addition and root-mean-square norm of rows x [rows, C] in one pass:
+ *   h = x + residual, rounded to the residual's type (the stream is held in it);
+ *   y = h / sqrt(mean(h^2) + eps) * (weight + weight_offset)       (mean and root in fp32)
+ * x F32 or BF16, row stride ldx elements. residual F32 or BF16 [rows, C], row stride ldr, or
+ * NULL (h = x, residual_dtype ignored). sum receives h in the residual's type with row stride
+ * ldr; it may be residual itself (in place), must not overlap it otherwise, and may be NULL.
+ * weight [C] fp32 or NULL (ones; weight_offset is then ignored). out [rows, C], row stride
+ * ldo, F32, BF16, or E4M3 with scale: fp32 [rows, ceil(C / group)] (contiguous), one scale per
+ * `group` channels of a row, the last group possibly shorter; group 0 is the whole row:
+ *   scale = max(max|y| / 448, 2^-100),  out = y / scale rounded to nearest even.
+ * A NaN among a group's y makes its scale and values NaN. out may be x where the types agree.
+ * 1 <= C <= 16384. */
+int sana_op_add_rms_norm_device(sana_cuda_ctx *ctx, const void *x, int x_dtype, long long ldx, const void *residual,
+                                int residual_dtype, long long ldr, void *sum, const float *weight,
+                                float weight_offset, float eps, long long rows, int C, void *out, int out_dtype,
+                                long long ldo, float *scale, int group);
+
+/* The frequencies of rotary positions: freq[i] (radians per position, 64 bits) of the
+ * rotated/2 pairs, host only. base^(-2i / rotated), then by `scaling`:
+ *   SANA_ROPE_PLAIN    as they are;
+ *   SANA_ROPE_LINEAR   all divided by `stretch` (positions interpolated);
+ *   SANA_ROPE_BASE     base replaced by base * stretch^(rotated / (rotated - 2));
+ *   SANA_ROPE_PARTS    pairs with at most `slow` turns over `context` positions divided by
+ *                      stretch, those with at least `fast` turns left, linear in the number
+ *                      of turns between them.
+ * stretch >= 1. context, slow < fast are read by SANA_ROPE_PARTS alone. */
+enum { SANA_ROPE_PLAIN = 0, SANA_ROPE_LINEAR = 1, SANA_ROPE_BASE = 2, SANA_ROPE_PARTS = 3 };
+int sana_rotary_frequencies(int rotated, double base, int scaling, double stretch, double context, double slow,
+                            double fast, double *freq);
+
+/* How heads are turned: the first `rotated` channels of each head (even, <= head_dim; the
+ * rest stays), as pairs (i, i + rotated/2), or (2i, 2i+1) with interleaved != 0:
+ *   y_a = m (x_a cos t - x_b sin t), y_b = m (x_b cos t + x_a sin t),  t = position * freq[i]
+ * with the product and its reduction in 64 bits. freq: device, rotated/2 doubles; magnitude
+ * m scales the turned channels (1 for none). */
+typedef struct sana_rotary {
+    const double *freq;
+    int rotated;
+    int interleaved;
+    float magnitude;
+} sana_rotary;
+
+/* Rotary positions of `rows` rows of q [rows, q_heads, head_dim] and k [rows, kv_heads,
+ * head_dim] (heads contiguous, row strides ldq / ldk elements; k NULL or kv_heads 0 for none)
+ * at the int32 positions [rows] (device; negative ones turn backwards, which undoes a turn).
+ * dtype F32 or BF16. q_out / k_out have the same strides and may be q / k (in place). */
+int sana_op_rotary_device(sana_cuda_ctx *ctx, const sana_rotary *rotary, int dtype, long long rows, int head_dim,
+                          const int *positions, const void *q, long long ldq, int q_heads, void *q_out,
+                          const void *k, long long ldk, int kv_heads, void *k_out);
+
+/* A pool of pages of keys and values: token `t` of page `p`, head `h`, starts at element
+ * p * page_stride + t * token_stride + h * head_stride of k and of v (64-bit offsets), its
+ * head_dim channels are contiguous. A plain contiguous cache is a pool with one page per
+ * sequence. page_size is any positive number. */
+typedef struct sana_paged_cache {
+    void *k, *v;
+    int dtype; /* F32 or BF16 */
+    int pages, page_size, kv_heads, head_dim;
+    long long page_stride, token_stride, head_stride;
+} sana_paged_cache;
+
+/* A batch of sequences, each with new tokens as the rows row_start[s] .. row_start[s+1]-1 of
+ * q (and k, v) and kv_len[s] tokens in the cache, the new ones included (they are its last):
+ * new token j of sequence s has the position kv_len[s] - (row_start[s+1] - row_start[s]) + j.
+ * Position t lives on page page_table[s * table_stride + t / page_size]. row_start
+ * [sequences + 1] ascending, kv_len [sequences], page_table [sequences, table_width]: int32,
+ * device; entries behind a sequence's last page are not read, and neither are entries that no
+ * new token sees. max_new and max_kv are upper bounds of the new and of the cached tokens of
+ * any sequence (they size the launch; a larger kv_len is taken as max_kv's violation and
+ * recorded). Rows behind the last sequence are left as they were. A sequence may have no new
+ * token. */
+typedef struct sana_paged_batch {
+    int sequences, rows, max_new, max_kv;
+    const int *row_start;
+    const int *kv_len;
+    const int *page_table;
+    long long table_stride;
+    int table_width;
+} sana_paged_batch;
+
+/* Rotary positions of a batch's new rows, and their append to the cache, in one launch: q
+ * turned into q_out (which may be q), k turned and v copied into their tokens' places.
+ * rotary NULL appends without turning (q, q_out unused). q [rows, q_heads, head_dim], k and v
+ * [rows, kv_heads, head_dim] of the cache's dtype, row strides ldq (q and q_out), ldk, ldv. */
+int sana_op_rotary_append_device(sana_cuda_ctx *ctx, const sana_rotary *rotary, const sana_paged_batch *batch,
+                                 const sana_paged_cache *cache, const void *q, long long ldq, int q_heads,
+                                 void *q_out, const void *k, long long ldk, const void *v, long long ldv);
+
+/* Causal attention of a batch's new tokens over the paged cache (which already holds their own
+ * keys and values): the token at position p sees the positions j <= p and, with window > 0,
+ * of those only j > p - window or j < sinks:
+ *   out = softmax_j(s_j) v_j,  s_j = scale q.k_j, or softcap * tanh(scale q.k_j / softcap)
+ * with softcap > 0. Query head h reads cache head h / (q_heads / kv_heads). q and out
+ * [rows, q_heads, head_dim] of the cache's dtype, row strides ldq, ldo (out must not overlap
+ * q); scores, softmax statistics and sums are fp32. What a token does not see does not reach
+ * its output, be it NaN or infinite; a token that sees nothing gets zeros. head_dim <= 256.
+ * BF16 with head_dim a multiple of 8 and 16-byte aligned pointers and strides runs on the
+ * tensor cores, the rest on the CUDA cores. workspace: device, 16-byte aligned,
+ * sana_op_paged_attention_workspace() bytes of the same batch, cache, heads, window and sinks
+ * (0 bytes: may be NULL); its contents need no preparation and nothing is kept in it, but two
+ * calls that may overlap (two streams, two graphs in flight) need one each. */
+int sana_op_paged_attention_device(sana_cuda_ctx *ctx, const sana_paged_batch *batch, const sana_paged_cache *cache,
+                                   const void *q, long long ldq, int q_heads, float scale, int window, int sinks,
+                                   float softcap, void *out, long long ldo, void *workspace, size_t workspace_bytes);
+size_t sana_op_paged_attention_workspace(sana_cuda_ctx *ctx, const sana_paged_batch *batch,
+                                         const sana_paged_cache *cache, int q_heads, int window, int sinks);
+
 /* --- the VAE decoder (vae.h:11-92, vae.cpp:243-325, vae_ops.cpp) ---------------------------- */
 
 /* The decoder's structure, mirroring SanaVaeWeights (vae.h:43-73): up block i has `channels`

@@ -14,6 +14,7 @@
 
 #include <cuda.h>
 
+#include "encoder.h"
 #include "engine.h"
 #include "gguf.h"
 #include "sana_cuda.h"
@@ -1630,6 +1631,276 @@ int sana_cuda_prompt_pairs_device(sana_cuda_ctx* ctx, int pairs, const float* ne
         sana::Engine& eng = engine(ctx);
         sana::prompt_pairs(negative, positive, pairs, positive_rows, hidden, L, counts, enc, bias, eng.stream());
     });
+}
+
+/* --- operators of the text encoder's blocks ----------------------------------------------- */
+
+namespace {
+
+bool act_dtype(int t) { return t == SANA_DTYPE_F32 || t == SANA_DTYPE_BF16; }
+
+// `rows` rows of `width` elements with stride ld
+void check_rows(const char* what, const void* ptr, long long rows, long long ld, long long width) {
+    if (rows > 0 && !ptr) throw sana::InvalidArg(std::string(what) + " must not be NULL");
+    if (ld < width) throw sana::InvalidArg(std::string(what) + ": the row stride is below the row's width");
+}
+
+sana::PagedBatch paged_batch_of(const sana_paged_batch* b) {
+    SANA_REQUIRE(b != nullptr, "batch must not be NULL");
+    SANA_REQUIRE(b->sequences >= 0 && b->rows >= 0 && b->max_new >= 0 && b->max_kv >= 0 && b->table_width >= 0,
+                 "negative batch sizes");
+    SANA_REQUIRE(b->sequences == 0 || (b->row_start && b->kv_len && (b->page_table || b->table_width == 0)),
+                 "row_start, kv_len and page_table must not be NULL");
+    SANA_REQUIRE(b->table_stride >= b->table_width, "table_stride is below table_width");
+    sana::PagedBatch o;
+    o.S = b->sequences;
+    o.rows = b->rows;
+    o.max_new = b->max_new;
+    o.max_kv = b->max_kv;
+    o.row_start = b->row_start;
+    o.kv_len = b->kv_len;
+    o.table = b->page_table;
+    o.table_stride = b->table_stride;
+    o.table_width = b->table_width;
+    return o;
+}
+
+sana::PagedCache paged_cache_of(const sana_paged_cache* c) {
+    SANA_REQUIRE(c != nullptr, "cache must not be NULL");
+    SANA_REQUIRE(act_dtype(c->dtype), "the cache's dtype must be F32 or BF16");
+    SANA_REQUIRE(c->pages >= 0 && c->page_size >= 1 && c->kv_heads >= 1 && c->head_dim >= 1, "invalid cache sizes");
+    SANA_REQUIRE(c->pages == 0 || (c->k && c->v), "k and v of the cache must not be NULL");
+    SANA_REQUIRE(c->page_stride >= 0 && c->token_stride >= 0 && c->head_stride >= 0, "negative cache strides");
+    sana::PagedCache o;
+    o.k = c->k;
+    o.v = c->v;
+    o.dtype = c->dtype;
+    o.pages = c->pages;
+    o.page_size = c->page_size;
+    o.kv_heads = c->kv_heads;
+    o.D = c->head_dim;
+    o.page_stride = c->page_stride;
+    o.token_stride = c->token_stride;
+    o.head_stride = c->head_stride;
+    return o;
+}
+
+sana::Rotary rotary_of(const sana_rotary* r, int head_dim) {
+    SANA_REQUIRE(r != nullptr, "rotary must not be NULL");
+    SANA_REQUIRE(r->rotated >= 0 && r->rotated % 2 == 0 && r->rotated <= head_dim && r->rotated <= 512,
+                 "rotated must be even, at most head_dim and at most 512");
+    SANA_REQUIRE(r->rotated == 0 || r->freq, "freq must not be NULL");
+    sana::Rotary o;
+    o.freq = r->freq;
+    o.rotated = r->rotated;
+    o.interleaved = r->interleaved != 0;
+    o.magnitude = r->magnitude;
+    return o;
+}
+
+sana::PagedAttention paged_attention_of(const sana_paged_batch* batch, const sana_paged_cache* cache, int q_heads,
+                                        int window, int sinks) {
+    sana::PagedAttention p{};
+    p.batch = paged_batch_of(batch);
+    p.cache = paged_cache_of(cache);
+    SANA_REQUIRE(p.cache.D <= 256, "head_dim must be at most 256");
+    SANA_REQUIRE(p.cache.kv_heads <= 65535, "too many cache heads");
+    SANA_REQUIRE(q_heads >= 1 && q_heads % p.cache.kv_heads == 0, "q_heads must be a multiple of kv_heads");
+    SANA_REQUIRE(window >= 0 && sinks >= 0, "window and sinks must not be negative");
+    SANA_REQUIRE(static_cast<long long>(p.batch.max_new) * (q_heads / p.cache.kv_heads) <= 0x3fffffffLL &&
+                     p.batch.max_kv <= 0x3fffffff,
+                 "max_new or max_kv too large");
+    p.q_heads = q_heads;
+    p.window = window;
+    p.sinks = sinks;
+    return p;
+}
+
+}  // namespace
+
+int sana_op_add_rms_norm_device(sana_cuda_ctx* ctx, const void* x, int x_dtype, long long ldx, const void* residual,
+                                int residual_dtype, long long ldr, void* sum, const float* weight,
+                                float weight_offset, float eps, long long rows, int C, void* out, int out_dtype,
+                                long long ldo, float* scale, int group) {
+    return guard(ctx, [&] {
+        SANA_REQUIRE(rows >= 0 && rows <= 0x7fffffffLL, "rows must be in [0, 2^31)");
+        SANA_REQUIRE(C >= 1 && C <= sana::kNormMaxChannels, "C must be in [1, 16384]");
+        SANA_REQUIRE(act_dtype(x_dtype) && (!residual || act_dtype(residual_dtype)), "x and residual must be F32 or BF16");
+        SANA_REQUIRE(act_dtype(out_dtype) || out_dtype == SANA_DTYPE_E4M3, "out must be F32, BF16 or E4M3");
+        SANA_REQUIRE(eps >= 0.f, "eps must not be negative");
+        SANA_REQUIRE(group >= 0, "group must not be negative");
+        SANA_REQUIRE(out_dtype == SANA_DTYPE_E4M3 || group == 0, "a group size goes with an E4M3 output only");
+        SANA_REQUIRE(out_dtype != SANA_DTYPE_E4M3 || scale || rows == 0, "an E4M3 output needs scale");
+        SANA_REQUIRE(residual || !sum, "sum needs a residual");
+        check_rows("x", x, rows, ldx, C);
+        check_rows("out", out, rows, ldo, C);
+        if (residual) check_rows("residual", residual, rows, ldr, C);
+        sana::AddRmsNorm p;
+        p.x = x;
+        p.residual = residual;
+        p.sum = sum;
+        p.weight = weight;
+        p.out = out;
+        p.scale = scale;
+        p.ldx = ldx;
+        p.ldr = ldr;
+        p.ldo = ldo;
+        p.rows = rows;
+        p.x_dtype = x_dtype;
+        p.r_dtype = residual_dtype;
+        p.out_dtype = out_dtype;
+        p.C = C;
+        p.group = group;
+        p.offset = weight_offset;
+        p.eps = eps;
+        sana::Engine& eng = engine(ctx);
+        CurrentDevice on(eng.device());
+        sana::add_rms_norm(p, eng.num_sms(), eng.stream());
+    });
+}
+
+int sana_rotary_frequencies(int rotated, double base, int scaling, double stretch, double context, double slow,
+                            double fast, double* freq) {
+    if (!freq || rotated < 2 || rotated % 2 != 0 || !(base > 0.0) || !(stretch >= 1.0) || !std::isfinite(base * stretch))
+        return SANA_ERR_INVALID;
+    if (scaling < SANA_ROPE_PLAIN || scaling > SANA_ROPE_PARTS) return SANA_ERR_INVALID;
+    if (scaling == SANA_ROPE_BASE && rotated == 2) return SANA_ERR_INVALID;
+    if (scaling == SANA_ROPE_PARTS && !(context > 0.0 && slow >= 0.0 && fast > slow)) return SANA_ERR_INVALID;
+    if (scaling == SANA_ROPE_BASE) base *= std::pow(stretch, static_cast<double>(rotated) / (rotated - 2));
+    for (int i = 0; i < rotated / 2; ++i) {
+        double f = std::pow(base, -2.0 * i / rotated);
+        if (scaling == SANA_ROPE_LINEAR) {
+            f /= stretch;
+        } else if (scaling == SANA_ROPE_PARTS) {
+            constexpr double kTwoPi = 6.283185307179586;
+            const double turns = context * f / kTwoPi;
+            const double keep = std::min(1.0, std::max(0.0, (turns - slow) / (fast - slow)));
+            f = f * keep + f / stretch * (1.0 - keep);
+        }
+        freq[i] = f;
+    }
+    return SANA_OK;
+}
+
+int sana_op_rotary_device(sana_cuda_ctx* ctx, const sana_rotary* rotary, int dtype, long long rows, int head_dim,
+                          const int* positions, const void* q, long long ldq, int q_heads, void* q_out, const void* k,
+                          long long ldk, int kv_heads, void* k_out) {
+    return guard(ctx, [&] {
+        SANA_REQUIRE(act_dtype(dtype), "dtype must be F32 or BF16");
+        SANA_REQUIRE(rows >= 0 && rows <= 0x7fffffffLL && head_dim >= 1 && q_heads >= 0 && kv_heads >= 0,
+                     "invalid rotary sizes");
+        SANA_REQUIRE(static_cast<long long>(head_dim) * (static_cast<long long>(q_heads) + kv_heads) <= 0x3fffffffLL,
+                     "a row is too wide");
+        SANA_REQUIRE(positions || rows == 0, "positions must not be NULL");
+        if (!k) kv_heads = 0;
+        if (q_heads) {
+            check_rows("q", q, rows, ldq, static_cast<long long>(q_heads) * head_dim);
+            check_rows("q_out", q_out, rows, ldq, static_cast<long long>(q_heads) * head_dim);
+        }
+        if (kv_heads) {
+            check_rows("k", k, rows, ldk, static_cast<long long>(kv_heads) * head_dim);
+            check_rows("k_out", k_out, rows, ldk, static_cast<long long>(kv_heads) * head_dim);
+        }
+        sana::RotaryRows p{};
+        p.rot = rotary_of(rotary, head_dim);
+        p.dtype = dtype;
+        p.D = head_dim;
+        p.q_heads = q_heads;
+        p.kv_heads = kv_heads;
+        p.rows = rows;
+        p.ldq = ldq;
+        p.ldk = ldk;
+        p.q = q;
+        p.q_out = q_out;
+        p.k = k;
+        p.k_out = k_out;
+        p.positions = positions;
+        sana::Engine& eng = engine(ctx);
+        CurrentDevice on(eng.device());
+        p.bad = eng.bad();
+        sana::rotary_rows(p, false, eng.stream());
+    });
+}
+
+int sana_op_rotary_append_device(sana_cuda_ctx* ctx, const sana_rotary* rotary, const sana_paged_batch* batch,
+                                 const sana_paged_cache* cache, const void* q, long long ldq, int q_heads, void* q_out,
+                                 const void* k, long long ldk, const void* v, long long ldv) {
+    return guard(ctx, [&] {
+        sana::RotaryRows p{};
+        p.batch = paged_batch_of(batch);
+        p.cache = paged_cache_of(cache);
+        SANA_REQUIRE(q_heads >= 0, "q_heads must not be negative");
+        SANA_REQUIRE(static_cast<long long>(p.cache.D) * (static_cast<long long>(q_heads) + 2LL * p.cache.kv_heads) <=
+                         0x3fffffffLL,
+                     "a row is too wide");
+        if (rotary) {
+            p.rot = rotary_of(rotary, p.cache.D);
+        } else {
+            p.rot = sana::Rotary{nullptr, 0, 0, 1.f};
+            q_heads = 0;
+        }
+        const long long width = static_cast<long long>(p.cache.kv_heads) * p.cache.D;
+        check_rows("k", k, p.batch.rows, ldk, width);
+        check_rows("v", v, p.batch.rows, ldv, width);
+        if (q_heads) {
+            check_rows("q", q, p.batch.rows, ldq, static_cast<long long>(q_heads) * p.cache.D);
+            check_rows("q_out", q_out, p.batch.rows, ldq, static_cast<long long>(q_heads) * p.cache.D);
+        }
+        p.dtype = p.cache.dtype;
+        p.D = p.cache.D;
+        p.q_heads = q_heads;
+        p.kv_heads = p.cache.kv_heads;
+        p.rows = p.batch.rows;
+        p.ldq = ldq;
+        p.ldk = ldk;
+        p.ldv = ldv;
+        p.q = q;
+        p.q_out = q_out;
+        p.k = k;
+        p.v = v;
+        sana::Engine& eng = engine(ctx);
+        CurrentDevice on(eng.device());
+        p.bad = eng.bad();
+        if (p.batch.S > 0) sana::rotary_rows(p, true, eng.stream());
+    });
+}
+
+int sana_op_paged_attention_device(sana_cuda_ctx* ctx, const sana_paged_batch* batch, const sana_paged_cache* cache,
+                                   const void* q, long long ldq, int q_heads, float scale, int window, int sinks,
+                                   float softcap, void* out, long long ldo, void* workspace, size_t workspace_bytes) {
+    return guard(ctx, [&] {
+        sana::PagedAttention p = paged_attention_of(batch, cache, q_heads, window, sinks);
+        const long long width = static_cast<long long>(q_heads) * p.cache.D;
+        check_rows("q", q, p.batch.rows, ldq, width);
+        check_rows("out", out, p.batch.rows, ldo, width);
+        SANA_REQUIRE(std::isfinite(scale), "scale must be finite");
+        SANA_REQUIRE(softcap >= 0.f && std::isfinite(softcap), "softcap must be finite and not negative");
+        sana::Engine& eng = engine(ctx);
+        const size_t need = sana::paged_attention_workspace(p, eng.num_sms());
+        SANA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
+                     "the workspace is smaller than sana_op_paged_attention_workspace() says");
+        SANA_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "the workspace must be 16-byte aligned");
+        CurrentDevice on(eng.device());
+        p.q = q;
+        p.out = out;
+        p.ldq = ldq;
+        p.ldo = ldo;
+        p.scale = scale;
+        p.softcap = softcap;
+        p.workspace = workspace;
+        p.bad = eng.bad();
+        p.err = eng.err();
+        sana::paged_attention(p, eng.num_sms(), eng.stream());
+    });
+}
+
+size_t sana_op_paged_attention_workspace(sana_cuda_ctx* ctx, const sana_paged_batch* batch,
+                                         const sana_paged_cache* cache, int q_heads, int window, int sinks) {
+    size_t n = 0;
+    const int rc = guard(ctx, [&] {
+        n = sana::paged_attention_workspace(paged_attention_of(batch, cache, q_heads, window, sinks), engine(ctx).num_sms());
+    });
+    return rc == SANA_OK ? n : 0;
 }
 
 /* --- the VAE decoder (vae.h, vae.cpp:243-325) ------------------------------------------- */

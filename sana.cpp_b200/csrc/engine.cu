@@ -2,6 +2,8 @@
 // CUDA-graph capture of the whole denoising loop. See engine.h.
 #include "engine.h"
 
+#include "encoder.h"
+
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -283,14 +285,16 @@ void Engine::denoise_loop_pair_device(const float* lat, int B, int H, int W, con
 }
 
 void Engine::check_device_error() {
-    int h = 0;
-    SANA_CUDA(cudaMemcpyAsync(&h, err_.get(), sizeof(int), cudaMemcpyDeviceToHost, st_));
+    int h[2] = {0, 0};  // the error code, and beside it what kernels found in device data (encoder.h)
+    SANA_CUDA(cudaMemcpyAsync(h, err_.get(), sizeof(h), cudaMemcpyDeviceToHost, st_));
     SANA_CUDA(cudaStreamSynchronize(st_));
-    if (h != 0) {
-        SANA_CUDA(cudaMemsetAsync(err_.get(), 0, sizeof(int), st_));
+    if (h[0] != 0 || h[1] != 0) {
+        SANA_CUDA(cudaMemsetAsync(err_.get(), 0, sizeof(h), st_));
         SANA_CUDA(cudaStreamSynchronize(st_));
-        throw TimeoutError("a device-side wait exceeded its time limit (code " + std::to_string(h) + ")");
     }
+    if (h[0] != 0)
+        throw TimeoutError("a device-side wait exceeded its time limit (code " + std::to_string(h[0]) + ")");
+    if (h[1] != 0) throw InvalidArg(bad_input_message(h[1]));
 }
 
 void Engine::gemm_act(const void* A, long long lda, const void* Bw, long long ldb, int M, int N, int K,

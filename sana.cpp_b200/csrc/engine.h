@@ -156,6 +156,8 @@ class Engine {
     // Device-side error word (timeouts); checked and cleared after every host API call.
     void check_device_error();
     int* err() const { return err_.as<int>(); }
+    // What kernels found wrong in device data (BadInput, encoder.h); reported like err.
+    int* bad() const { return err_.as<int>() + 1; }
     // Optional RMSNorm of the cross-attention q and k projections over each token's C channels,
     // not part of the reference's block (off by default). q_w / k_w: n_blocks pointers to [C]
     // weights (NULL array or entries = ones).

@@ -1,0 +1,629 @@
+// Attention of a chunk of new tokens over a paged cache:
+//   out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  s_j = scale q.k_j or cap tanh(scale q.k_j / cap),
+// in one pass over the keys with the running maximum m and sum; scores, statistics and sums fp32.
+// Two kernels here: a tensor-core one for bf16 (mma.sync; single tokens and short chunks, which
+// read much and compute little) and a CUDA-core one for fp32 and for what the first does not take.
+// pattn.cuh has the packing of rows, the key ranges and the splits.
+#include <algorithm>
+#include <cmath>
+
+#include "pattn.cuh"
+
+namespace sana {
+namespace pattn {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNegInf = -INFINITY;
+
+// --- CUDA cores -------------------------------------------------------------------------------
+// 32 packed rows x 32 keys per step, four threads per row: thread c of a row takes keys c + 4 i of
+// the scores and channels 4 c + 16 i of the output. q, k and v sit in shared memory as fp32 rows
+// padded by four words, so that the eight rows (or four keys) a warp reads at once lie in
+// different banks.
+constexpr int kSRows = 32, kSKeys = 32, kSThreads = 128;
+
+template <class T>
+__global__ void __launch_bounds__(kSThreads) paged_simt_kernel(const __grid_constant__ Args a) {
+    extern __shared__ float sm[];
+    __shared__ long long offs[kSKeys];
+    const PagedAttention& p = a.p;
+    const int tid = threadIdx.x, D = p.cache.D, D4 = (D + 3) & ~3, ld = D4 + 4;
+    float* Qs = sm;
+    float* Ks = Qs + kSRows * ld;
+    float* Vs = Ks + kSKeys * ld;
+    const int tile = a.row_tiles - 1 - static_cast<int>(blockIdx.x % a.row_tiles);
+    const int rest = blockIdx.x / a.row_tiles, split = rest % a.splits, s = rest / a.splits, kvh = blockIdx.y;
+    const Sequence sq = sequence(p, s, blockIdx.x % (a.row_tiles * a.splits) == 0 && kvh == 0 && tid == 0);
+    const int rr0 = tile * kSRows;
+    if (!sq.ok || rr0 >= sq.n_new * a.G) return;
+    const KeyTiles kt = key_tiles(sq.past, sq.n_new, a.G, rr0, rr0 + kSRows, p.window, p.sinks, kSKeys);
+    const int t0 = split * a.split_tiles, t1 = min(kt.n, t0 + a.split_tiles);
+    if (t0 >= t1) return;
+    const bool partial = kt.n > a.split_tiles;
+
+    const T* q = static_cast<const T*>(p.q);
+    for (int i = tid; i < kSRows * D4; i += kSThreads) {
+        const int r = i / D4, d = i - r * D4, rr = rr0 + r;
+        float v = 0.f;
+        if (rr < sq.n_new * a.G && d < D)
+            v = to_f(q[(sq.row0 + rr / a.G) * p.ldq + static_cast<long long>(kvh * a.G + rr % a.G) * D + d]);
+        Qs[r * ld + d] = v;
+    }
+    const int r = tid >> 2, c = tid & 3, rr = rr0 + r;
+    const bool live = rr < sq.n_new * a.G;
+    const int pos = live ? sq.past + rr / a.G : -1;
+    float4 o[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    float m = kNegInf, l = 0.f;
+    const T* kc = static_cast<const T*>(p.cache.k) + kvh * p.cache.head_stride;
+    const T* vc = static_cast<const T*>(p.cache.v) + kvh * p.cache.head_stride;
+
+    for (int t = t0; t < t1; ++t) {
+        int start, end;
+        key_range(kt, t, kSKeys, start, end);
+        __syncthreads();  // the previous step's readers are done
+        if (tid < kSKeys) offs[tid] = start + tid < end ? key_offset(p, s, start + tid) : -1;
+        __syncthreads();
+        for (int i = tid; i < kSKeys * D4; i += kSThreads) {
+            const int key = i / D4, d = i - key * D4;
+            const long long off = offs[key];
+            const bool in = off >= 0 && d < D;
+            Ks[key * ld + d] = in ? to_f(kc[off + d]) : 0.f;
+            Vs[key * ld + d] = in ? to_f(vc[off + d]) : 0.f;
+        }
+        __syncthreads();
+        float sc[8] = {};
+        const float4* qv = reinterpret_cast<const float4*>(Qs + r * ld);
+        for (int d = 0; d < D4 / 4; ++d) {
+            const float4 x = qv[d];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float4 y = *reinterpret_cast<const float4*>(Ks + (c + 4 * i) * ld + 4 * d);
+                sc[i] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, sc[i]))));
+            }
+        }
+        float mx = kNegInf;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int key = c + 4 * i;
+            float v = sc[i] * p.scale;
+            if (p.softcap > 0.f) v = p.softcap * tanhf(v / p.softcap);
+            sc[i] = offs[key] >= 0 && seen(start + key, pos, p.window, p.sinks) ? v : kNegInf;
+            mx = fmaxf(mx, sc[i]);
+        }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float m_new = fmaxf(m, mx), base = m_new == kNegInf ? 0.f : m_new;
+        const float alpha = ex2_approx((m - base) * kLog2e);
+        m = m_new;
+        l *= alpha;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            sc[i] = ex2_approx((sc[i] - base) * kLog2e);
+            l += sc[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            o[i].x *= alpha, o[i].y *= alpha, o[i].z *= alpha, o[i].w *= alpha;
+        }
+        // a key that a row does not see has p = 0, and 0 * v is left out where v may not be finite for it
+        const bool whole = all_seen(kt, start, end, p.window, p.sinks);
+        const int quad = tid & 28;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+            for (int cc = 0; cc < 4; ++cc) {
+                const float pr = __shfl_sync(0xffffffffu, sc[i], quad | cc);
+                if (!whole && pr == 0.f) continue;
+                const float* v = Vs + (cc + 4 * i) * ld + 4 * c;
+#pragma unroll
+                for (int d = 0; d < 16; ++d) {
+                    if (4 * c + 16 * d < D4) {
+                        const float4 y = *reinterpret_cast<const float4*>(v + 16 * d);
+                        o[d].x = fmaf(pr, y.x, o[d].x);
+                        o[d].y = fmaf(pr, y.y, o[d].y);
+                        o[d].z = fmaf(pr, y.z, o[d].z);
+                        o[d].w = fmaf(pr, y.w, o[d].w);
+                    }
+                }
+            }
+        }
+    }
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (!live) return;
+    const long long row = sq.row0 + rr / a.G;
+    const int h = kvh * a.G + rr % a.G;
+    const float inv = partial ? 1.f : (l > 0.f || l != l ? 1.f / l : 0.f);
+    const long long at = (static_cast<long long>(split) * p.batch.rows + row) * p.q_heads + h;
+    if (partial && c == 0) a.ml[at] = make_float2(m * kLog2e, l);  // base-2 exponents, as the other kernel's
+    T* out = static_cast<T*>(p.out) + row * p.ldo + static_cast<long long>(h) * D;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float v[4] = {o[i].x, o[i].y, o[i].z, o[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int d = 4 * c + 16 * i + e;
+            if (d >= D) continue;
+            if (partial) a.part[at * D + d] = v[e];
+            else out[d] = from_f<T>(v[e] * inv);
+        }
+    }
+}
+
+// --- tensor cores, mma.sync -------------------------------------------------------------------
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_bf2(float lo, float hi) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&b);
+}
+// A pair of bf16 with what is not finite replaced by zero; `bad` is set where something was.
+__device__ __forceinline__ uint32_t finite2(uint32_t x, bool& bad) {
+    if ((x & 0x7f80u) == 0x7f80u) x &= 0xffff0000u, bad = true;
+    if ((x & 0x7f800000u) == 0x7f800000u) x &= 0x0000ffffu, bad = true;
+    return x;
+}
+// cap * tanh(x / cap) * log2(e) from the hardware exponential: tanh z = 1 - 2 / (1 + e^2z), absolute
+// error a few 2^-24 for any z, which times the cap stays far below a bf16 probability's rounding.
+__device__ __forceinline__ float soft_cap_log2(float x, float two_log2e_over_cap, float cap_log2e) {
+    return fmaf(-2.f * cap_log2e, rcp_approx(1.f + ex2_approx(x * two_log2e_over_cap)), cap_log2e);
+}
+
+// DP: padded head size. WM warps share out the rows (16 each), 4 / WM warps each step's 64 keys:
+// a single token's few rows keep all four warps busy on different keys, and every warp runs its
+// own softmax; the warps' results are joined once at the end. Keys and values come by 16-byte
+// cp.async, ST tiles deep, into rows whose 16-byte chunks are swapped by the row number (c ^ (r &
+// 7)) so that ldmatrix meets no bank twice; the page lookups run ST tiles ahead of the loads. P is
+// rounded to bf16 for the second product, its sum is not.
+template <int DP>
+struct MmaShape {
+    static constexpr int kKeys = 64;
+    static constexpr int kStages = DP == 64 ? 4 : 3;
+    static constexpr int kTileBytes = kKeys * DP * 2;
+    static constexpr int smem(int rows) {
+        return rows * DP * 2 + kStages * 2 * kTileBytes + (kStages + 1) * kKeys * 8;
+    }
+};
+
+template <int DP, int WM>
+__global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ Args a) {
+    using Sh = MmaShape<DP>;
+    constexpr int BN = Sh::kKeys, ST = Sh::kStages, BM = 16 * WM, WK = 4 / WM, NT = BN / WK / 8, CH = DP / 8;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const PagedAttention& p = a.p;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wm = warp % WM, wk = warp / WM, D = p.cache.D;
+    const int tile = a.row_tiles - 1 - static_cast<int>(blockIdx.x % a.row_tiles);
+    const int rest = blockIdx.x / a.row_tiles, split = rest % a.splits, s = rest / a.splits, kvh = blockIdx.y;
+    const Sequence sq = sequence(p, s, blockIdx.x % (a.row_tiles * a.splits) == 0 && kvh == 0 && tid == 0);
+    const int rr0 = tile * BM, n_rows = sq.n_new * a.G;
+    if (!sq.ok || rr0 >= n_rows) return;
+    const KeyTiles kt = key_tiles(sq.past, sq.n_new, a.G, rr0, rr0 + BM, p.window, p.sinks, BN);
+    const int t0 = split * a.split_tiles, n = min(kt.n, t0 + a.split_tiles) - t0;
+    if (n <= 0) return;
+    const bool partial = kt.n > a.split_tiles;
+
+    const uint32_t q_s = smem_u32(smem), kv_s = q_s + BM * DP * 2;
+    long long* offs = reinterpret_cast<long long*>(smem + BM * DP * 2 + ST * 2 * Sh::kTileBytes);  // [ST + 1][BN]
+    auto swz = [](int row, int chunk) { return static_cast<uint32_t>(row * (DP * 2) + ((chunk ^ (row & 7)) << 4)); };
+
+    const bf16* q = static_cast<const bf16*>(p.q);
+    for (int i = tid; i < BM * CH; i += 128) {
+        const int r = i / CH, c = i % CH, rr = rr0 + r;
+        const bool in = rr < n_rows && c * 8 < D;
+        const int t = rr / a.G;
+        const bf16* src = in ? q + (sq.row0 + t) * p.ldq + static_cast<long long>(kvh * a.G + rr - t * a.G) * D + c * 8 : q;
+        cp_async16(q_s + swz(r, c), src, in);
+    }
+    const bf16* kc = static_cast<const bf16*>(p.cache.k) + kvh * p.cache.head_stride;
+    const bf16* vc = static_cast<const bf16*>(p.cache.v) + kvh * p.cache.head_stride;
+    auto offset_of = [&](int i) -> long long {  // of this thread's key (tid < BN) of tile i
+        int start, end;
+        key_range(kt, t0 + i, BN, start, end);
+        return start + tid < end ? key_offset(p, s, start + tid) : -1;
+    };
+    auto load = [&](int i) {
+        const long long* of = offs + (i % (ST + 1)) * BN;
+        const uint32_t ks = kv_s + (i % ST) * (2 * Sh::kTileBytes), vs = ks + Sh::kTileBytes;
+        constexpr int kRowsPerPass = 128 / CH < 1 ? 1 : 128 / CH;
+#pragma unroll
+        for (int x = 0; x < BN / kRowsPerPass; ++x) {
+            const int key = tid / CH + x * kRowsPerPass, c = tid % CH;
+            const long long off = of[key];
+            const bool in = off >= 0 && c * 8 < D;
+            const long long e = in ? off + c * 8 : 0;
+            cp_async16(ks + swz(key, c), kc + e, in);
+            cp_async16(vs + swz(key, c), vc + e, in);
+        }
+    };
+    if (tid < BN) {
+#pragma unroll
+        for (int i = 0; i < ST; ++i) offs[i * BN + tid] = i < n ? offset_of(i) : -1;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ST - 1; ++i) {
+        if (i < n) load(i);
+        cp_async_commit();
+    }
+
+    float o[DP / 8][4];
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f};
+    int pos[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int rr = rr0 + wm * 16 + (lane >> 2) + 8 * i;
+        pos[i] = rr < n_rows ? sq.past + rr / a.G : -1;
+    }
+    const float scale_log2 = p.scale * kLog2e;
+    const float cap_in = p.softcap > 0.f ? 2.f * scale_log2 / p.softcap : 0.f, cap_out = p.softcap * kLog2e;
+    const int kb = wk * (BN / WK);
+
+    for (int i = 0; i < n; ++i) {
+        cp_async_wait<ST - 2>();
+        __syncthreads();
+        if (i + ST - 1 < n) load(i + ST - 1);
+        cp_async_commit();
+        const long long next = tid < BN && i + ST < n ? offset_of(i + ST) : -1;
+
+        const uint32_t ks = kv_s + (i % ST) * (2 * Sh::kTileBytes), vs = ks + Sh::kTileBytes;
+        float sc[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+            if (kk * 16 < D) {
+                uint32_t qa[4];
+                ldmatrix4(qa, q_s + swz(wm * 16 + (lane & 15), kk * 2 + (lane >> 4)));
+#pragma unroll
+                for (int t = 0; t < NT / 2; ++t) {
+                    uint32_t b[4];
+                    ldmatrix4(b, ks + swz(kb + t * 16 + (lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)));
+                    mma16816(sc[2 * t], qa, b[0], b[1]);
+                    mma16816(sc[2 * t + 1], qa, b[2], b[3]);
+                }
+            }
+        }
+        int start, end;
+        key_range(kt, t0 + i, BN, start, end);
+        const long long* of = offs + (i % (ST + 1)) * BN;
+        const bool whole = !__any_sync(0xffffffffu, of[lane] < 0 || of[lane + 32] < 0) &&
+                           all_seen(kt, start, end, p.window, p.sinks);
+        if (p.softcap > 0.f) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[t][e] = soft_cap_log2(sc[t][e], cap_in, cap_out);
+        } else {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[t][e] *= scale_log2;
+        }
+        if (!whole) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int key = kb + t * 8 + (lane & 3) * 2 + (e & 1);
+                    if (of[key] < 0 || !seen(start + key, pos[e >> 1], p.window, p.sinks)) sc[t][e] = kNegInf;
+                }
+        }
+        float alpha[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            float mx = kNegInf;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) mx = fmaxf(mx, fmaxf(sc[t][2 * r], sc[t][2 * r + 1]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float m_new = fmaxf(m[r], mx), base = m_new == kNegInf ? 0.f : m_new;
+            alpha[r] = ex2_approx(m[r] - base);
+            m[r] = m_new;
+            float sum = 0.f;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                sc[t][2 * r] = ex2_approx(sc[t][2 * r] - base);
+                sc[t][2 * r + 1] = ex2_approx(sc[t][2 * r + 1] - base);
+                sum += sc[t][2 * r] + sc[t][2 * r + 1];
+            }
+            l[r] = fmaf(l[r], alpha[r], sum);
+        }
+        if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+            for (int d = 0; d < DP / 8; ++d) {
+                o[d][0] *= alpha[0], o[d][1] *= alpha[0];
+                o[d][2] *= alpha[1], o[d][3] *= alpha[1];
+            }
+        }
+        bool bad = false;
+#pragma unroll
+        for (int t = 0; t < NT / 2; ++t) {
+            const uint32_t pa[4] = {pack_bf2(sc[2 * t][0], sc[2 * t][1]), pack_bf2(sc[2 * t][2], sc[2 * t][3]),
+                                    pack_bf2(sc[2 * t + 1][0], sc[2 * t + 1][1]),
+                                    pack_bf2(sc[2 * t + 1][2], sc[2 * t + 1][3])};
+            const int row = kb + t * 16 + (lane & 15);
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d) {
+                if (d * 16 < D) {
+                    uint32_t b[4];
+                    ldmatrix4_t(b, vs + swz(row, d * 2 + (lane >> 4)));
+                    if (!whole) {  // 0 * v must be 0 for the rows that do not see v
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) b[x] = finite2(b[x], bad);
+                    }
+                    mma16816(o[2 * d], pa, b[0], b[1]);
+                    mma16816(o[2 * d + 1], pa, b[2], b[3]);
+                }
+            }
+        }
+        if (!whole && __any_sync(0xffffffffu, bad)) {
+            // what finite2 took out, given back to the rows that see it
+            for (int key = kb; key < kb + BN / WK; ++key) {
+                if (of[key] < 0) continue;
+                const bool s0 = seen(start + key, pos[0], p.window, p.sinks);
+                const bool s1 = seen(start + key, pos[1], p.window, p.sinks);
+                const unsigned char* vrow = smem + (vs - q_s);
+#pragma unroll
+                for (int d = 0; d < DP / 8; ++d) {
+                    const uint32_t x = *reinterpret_cast<const uint32_t*>(vrow + swz(key, d) + (lane & 3) * 4);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float v = __uint_as_float(e ? x & 0xffff0000u : x << 16);
+                        if ((__float_as_uint(v) & 0x7f800000u) != 0x7f800000u) continue;
+                        if (s0) o[d][e] += v;
+                        if (s1) o[d][2 + e] += v;
+                    }
+                }
+            }
+        }
+        if (tid < BN) offs[((i + ST) % (ST + 1)) * BN + tid] = next;
+    }
+    cp_async_wait<0>();
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    }
+    __syncthreads();
+    // [WK][BM] rows of DP fp32 over the tiles' memory, and (max, sum) over the lookups'
+    constexpr int LD = DP + 8;
+    static_assert(WK * BM * LD * 4 <= ST * 2 * Sh::kTileBytes, "the join fits the tiles' memory");
+    static_assert(WK * BM * 8 <= (ST + 1) * BN * 8, "the statistics fit the lookups' memory");
+    float* os = reinterpret_cast<float*>(smem + BM * DP * 2);
+    float2* st = reinterpret_cast<float2*>(offs);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const int row = wk * BM + wm * 16 + (lane >> 2) + 8 * r;
+        if ((lane & 3) == 0) st[row] = make_float2(m[r], l[r]);
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d)
+            *reinterpret_cast<float2*>(os + row * LD + d * 8 + (lane & 3) * 2) = make_float2(o[d][2 * r], o[d][2 * r + 1]);
+    }
+    __syncthreads();
+    const int d8 = D / 8;
+    for (int i = tid; i < BM * d8; i += 128) {
+        const int r = i / d8, d = (i - r * d8) * 8, rr = rr0 + r;
+        if (rr >= n_rows) break;
+        float mm = kNegInf, ll = 0.f, v[8] = {};
+#pragma unroll
+        for (int w = 0; w < WK; ++w) mm = fmaxf(mm, st[w * BM + r].x);
+        const float base = mm == kNegInf ? 0.f : mm;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) {
+            const float2 x = st[w * BM + r];
+            const float f = ex2_approx(x.x - base);
+            ll = fmaf(x.y, f, ll);
+            const float* src = os + (w * BM + r) * LD + d;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = fmaf(src[e], f, v[e]);
+        }
+        const int t = rr / a.G, h = kvh * a.G + rr - t * a.G;
+        const long long row = sq.row0 + t;
+        if (partial) {
+            const long long at = (static_cast<long long>(split) * p.batch.rows + row) * p.q_heads + h;
+            if (d == 0) a.ml[at] = make_float2(mm, ll);
+            float4* dst = reinterpret_cast<float4*>(a.part + at * D + d);
+            dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+            dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            const float inv = ll == 0.f ? 0.f : 1.f / ll;
+            *reinterpret_cast<uint4*>(static_cast<bf16*>(p.out) + row * p.ldo + static_cast<long long>(h) * D + d) =
+                make_uint4(pack_bf2(v[0] * inv, v[1] * inv), pack_bf2(v[2] * inv, v[3] * inv),
+                           pack_bf2(v[4] * inv, v[5] * inv), pack_bf2(v[6] * inv, v[7] * inv));
+        }
+    }
+}
+
+// --- joining the splits -----------------------------------------------------------------------
+// One block per row and four heads, one warp per head: the splits' maxima give the weights, then
+// each lane sums its channels over the splits in order.
+template <class T>
+__global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constant__ Args a) {
+    const PagedAttention& p = a.p;
+    const int row = blockIdx.x, lane = threadIdx.x & 31, h = blockIdx.y * 4 + (threadIdx.x >> 5), D = p.cache.D;
+    int s = 0;
+    for (int s0 = 0; s0 < p.batch.S; s0 += 128) {
+        const int i = s0 + static_cast<int>(threadIdx.x);
+        s += __syncthreads_count(i < p.batch.S && p.batch.row_start[i + 1] <= row);
+    }
+    if (s >= p.batch.S || h >= p.q_heads) return;
+    const Sequence sq = sequence(p, s, false);
+    if (!sq.ok || row < sq.row0) return;
+    const int rr = (row - sq.row0) * a.G + h % a.G, tile = rr / a.BM;
+    const KeyTiles kt = key_tiles(sq.past, sq.n_new, a.G, tile * a.BM, (tile + 1) * a.BM, p.window, p.sinks, a.BN);
+    const int active = (kt.n + a.split_tiles - 1) / a.split_tiles;
+    if (active <= 1) return;
+    const long long step = static_cast<long long>(p.batch.rows) * p.q_heads;
+    const long long at = static_cast<long long>(row) * p.q_heads + h;
+    float m = kNegInf;
+    for (int i = lane; i < active; i += 32) m = fmaxf(m, a.ml[at + i * step].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float base = m == kNegInf ? 0.f : m;
+    float acc[8] = {}, l = 0.f;
+    for (int i = 0; i < active; ++i) {
+        const float2 x = a.ml[at + i * step];
+        const float f = ex2_approx(x.x - base);
+        l = fmaf(x.y, f, l);
+        const float* src = a.part + (at + i * step) * D;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (lane + 32 * e < D) acc[e] = fmaf(src[lane + 32 * e], f, acc[e]);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* out = static_cast<T*>(p.out) + static_cast<long long>(row) * p.ldo + static_cast<long long>(h) * D;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (lane + 32 * e < D) out[lane + 32 * e] = from_f<T>(acc[e] * inv);
+}
+
+// --- plan and launch ----------------------------------------------------------------------------
+enum Kind { kSimt, kMma };
+
+bool cache_fits_mma(const PagedCache& c) {
+    return c.dtype == kBf16 && c.D % 8 == 0 && (reinterpret_cast<uintptr_t>(c.k) & 15) == 0 &&
+           (reinterpret_cast<uintptr_t>(c.v) & 15) == 0 && c.page_stride % 8 == 0 && c.token_stride % 8 == 0 &&
+           c.head_stride % 8 == 0;
+}
+
+// The launch of one kind: tiles and splits, by sizes that the host knows.
+Args plan(const PagedAttention& p, Kind kind, int num_sms) {
+    Args a{};
+    a.p = p;
+    a.G = p.q_heads / p.cache.kv_heads;
+    const long long packed = static_cast<long long>(p.batch.max_new) * a.G;
+    int resident;  // blocks per SM
+    if (kind == kSimt) {
+        a.BM = kSRows;
+        a.BN = kSKeys;
+        resident = 2;
+    } else {
+        a.BM = packed <= 16 ? 16 : packed <= 32 ? 32 : 64;
+        a.BN = 64;
+        resident = p.cache.D > 128 ? 1 : 2;
+    }
+    a.row_tiles = ceil_div(packed, a.BM);
+    const long long span = p.window > 0 ? std::min<long long>(p.batch.max_kv, static_cast<long long>(p.window) + p.batch.max_new +
+                                                                                 p.sinks)
+                                        : p.batch.max_kv;
+    const int tiles = ceil_div(span, a.BN) + (p.window > 0 ? 1 : 0);
+    const long long base = static_cast<long long>(p.batch.S) * p.cache.kv_heads * a.row_tiles;
+    // One sequence: one wave of equal blocks. Several: their lengths differ and only the longest is
+    // known here, so blocks of a few waves' size even them out.
+    const long long want = static_cast<long long>(num_sms) * resident * (p.batch.S == 1 ? 1 : 4);
+    const long long splits = std::max<long long>(1, std::min<long long>(want / std::max<long long>(base, 1), tiles / 2));
+    a.split_tiles = std::max(1, ceil_div(tiles, splits));
+    a.splits = ceil_div(tiles, a.split_tiles);
+    return a;
+}
+
+size_t part_bytes(const Args& a) {
+    if (a.splits <= 1) return 0;
+    const size_t n = static_cast<size_t>(a.splits) * a.p.batch.rows * a.p.q_heads;
+    const size_t ml = (n * sizeof(float2) + 15) & ~static_cast<size_t>(15);
+    return ml + n * a.p.cache.D * sizeof(float);
+}
+
+void raise_smem(const void* f, int bytes, PerDeviceOnce& once) {
+    if (!once.pending()) return;
+    SANA_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    once.mark();
+}
+
+template <int DP, int WM>
+void launch_mma(const Args& a, dim3 grid, cudaStream_t st) {
+    static PerDeviceOnce once;
+    constexpr int bytes = MmaShape<DP>::smem(16 * WM);
+    static_assert(bytes <= 232448, "shared memory of one block");
+    raise_smem(reinterpret_cast<const void*>(&paged_mma_kernel<DP, WM>), bytes, once);
+    paged_mma_kernel<DP, WM><<<grid, 128, bytes, st>>>(a);
+}
+
+template <int DP>
+void launch_mma_rows(const Args& a, dim3 grid, cudaStream_t st) {
+    if (a.BM == 16) launch_mma<DP, 1>(a, grid, st);
+    else if (a.BM == 32) launch_mma<DP, 2>(a, grid, st);
+    else launch_mma<DP, 4>(a, grid, st);
+}
+
+template <class T>
+void launch_simt(const Args& a, dim3 grid, cudaStream_t st) {
+    static PerDeviceOnce once;
+    constexpr int most = (kSRows + 2 * kSKeys) * (256 + 4) * 4;
+    raise_smem(reinterpret_cast<const void*>(&paged_simt_kernel<T>), most, once);
+    const int ld = ((a.p.cache.D + 3) & ~3) + 4;
+    paged_simt_kernel<T><<<grid, kSThreads, (kSRows + 2 * kSKeys) * ld * 4, st>>>(a);
+}
+
+}  // namespace
+}  // namespace pattn
+
+using namespace pattn;
+
+// Alignment of q and out is not known when the workspace is asked for: the larger of the two kinds' needs.
+size_t paged_attention_workspace(const PagedAttention& p, int num_sms) {
+    size_t n = part_bytes(plan(p, kSimt, num_sms));
+    if (cache_fits_mma(p.cache)) n = std::max(n, part_bytes(plan(p, kMma, num_sms)));
+    return n;
+}
+
+void paged_attention(const PagedAttention& p, int num_sms, cudaStream_t st) {
+    if (p.batch.S == 0 || p.batch.rows == 0 || p.batch.max_new == 0) return;
+    const bool mma = cache_fits_mma(p.cache) && (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 &&
+                     (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.ldq % 8 == 0 && p.ldo % 8 == 0;
+    Args a = plan(p, mma ? kMma : kSimt, num_sms);
+    const size_t n = static_cast<size_t>(a.splits) * p.batch.rows * p.q_heads;
+    a.ml = static_cast<float2*>(p.workspace);
+    a.part = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + ((n * sizeof(float2) + 15) & ~static_cast<size_t>(15)));
+    const long long blocks = static_cast<long long>(p.batch.S) * a.splits * a.row_tiles;
+    SANA_REQUIRE(blocks <= 0x7fffffffLL, "paged attention: too many sequences times row tiles for one launch");
+    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(p.cache.kv_heads));
+    if (mma) {
+        if (p.cache.D <= 64) launch_mma_rows<64>(a, grid, st);
+        else if (p.cache.D <= 128) launch_mma_rows<128>(a, grid, st);
+        else launch_mma_rows<256>(a, grid, st);
+    } else if (p.cache.dtype == kF32) {
+        launch_simt<float>(a, grid, st);
+    } else {
+        launch_simt<bf16>(a, grid, st);
+    }
+    SANA_CUDA(cudaGetLastError());
+    if (a.splits > 1) {
+        const dim3 cgrid(static_cast<unsigned>(p.batch.rows), static_cast<unsigned>((p.q_heads + 3) / 4));
+        if (p.cache.dtype == kF32) paged_combine_kernel<float><<<cgrid, 128, 0, st>>>(a);
+        else paged_combine_kernel<bf16><<<cgrid, 128, 0, st>>>(a);
+        SANA_CUDA(cudaGetLastError());
+    }
+}
+
+}  // namespace sana

@@ -1,0 +1,112 @@
+// What the paged-attention kernels share: the packing of rows, the key range of a row tile, the
+// checks of device data, and the plan of a launch.
+//
+// Rows. The new tokens of a sequence and the query heads that read one cache head are packed into
+// the rows of one tile, row = token * G + head: a cached key is then read once for the whole
+// group, and a single token fills G rows.
+//
+// Keys. A row at position p sees j <= p and, with a window W, of those j > p - W or j < sinks. A
+// tile of rows therefore walks the sinks' keys (if the window has moved past them) and then the
+// keys from the first row's window to the last row's position, BN at a time; only tiles that some
+// row sees in part are masked element by element.
+//
+// Splits. The key tiles of a row tile are shared out over blocks, `split_tiles` each; what a block
+// of several finds is left in the workspace as (sum p v, max, sum p) and joined by
+// paged_combine_kernel in a fixed order.
+#pragma once
+
+#include "encoder.h"
+
+namespace sana {
+namespace pattn {
+
+struct Args {
+    PagedAttention p;
+    int G;            // query heads per cache head
+    int row_tiles;    // of BM packed rows, per sequence
+    int BM, BN;
+    int splits, split_tiles;
+    float* part;      // [splits][rows][q_heads][D]
+    float2* ml;       // [splits][rows][q_heads]: (max, sum)
+};
+
+struct Sequence {
+    int row0, n_new, past;
+    bool ok;
+};
+// The checked lengths of sequence s; ok false: nothing of it is computed. `report`: this thread records why.
+__device__ __forceinline__ Sequence sequence(const PagedAttention& p, int s, bool report) {
+    Sequence q;
+    q.row0 = p.batch.row_start[s];
+    const int end = p.batch.row_start[s + 1], len = p.batch.kv_len[s];
+    // 64-bit differences: the inputs are unchecked
+    const long long n = static_cast<long long>(end) - q.row0;
+    const bool rows_ok = q.row0 >= 0 && n >= 0 && end <= p.batch.rows && n <= p.batch.max_new;
+    const bool len_ok = len >= 0 && len <= p.batch.max_kv && (n == 0 || len >= n);
+    if (report && !(rows_ok && len_ok)) record_bad(p.bad, rows_ok ? kBadLength : kBadRows);
+    q.ok = rows_ok && len_ok && n > 0;
+    q.n_new = static_cast<int>(n);
+    q.past = len - static_cast<int>(n);
+    return q;
+}
+
+// The key tiles of packed rows [rr0, rr1) of a sequence.
+struct KeyTiles {
+    int pmin, pmax;   // positions of the first and last row
+    int sink_end;     // keys [0, sink_end) apart from the rest (0: none)
+    int lo, hi;       // keys [lo, hi)
+    int n_sink, n;    // tiles of the sinks, of both
+};
+__host__ __device__ __forceinline__ KeyTiles key_tiles(int past, int n_new, int G, int rr0, int rr1, int window, int sinks,
+                                                       int BN) {
+    KeyTiles k;
+    const int last = n_new * G < rr1 ? n_new * G : rr1;
+    k.pmin = past + rr0 / G;
+    k.pmax = past + (last - 1) / G;
+    k.hi = k.pmax + 1;
+    k.lo = 0;
+    k.sink_end = 0;
+    if (window > 0) {
+        const int lo = k.pmin - window + 1;
+        const int s = sinks < k.hi ? sinks : k.hi;
+        if (lo > s) {
+            k.lo = lo;
+            k.sink_end = s;
+        }
+    }
+    k.n_sink = (k.sink_end + BN - 1) / BN;
+    k.n = k.n_sink + (k.hi - k.lo + BN - 1) / BN;
+    return k;
+}
+__device__ __forceinline__ void key_range(const KeyTiles& k, int i, int BN, int& start, int& end) {
+    if (i < k.n_sink) {
+        start = i * BN;
+        end = min(k.sink_end, start + BN);
+    } else {
+        start = k.lo + (i - k.n_sink) * BN;
+        end = min(k.hi, start + BN);
+    }
+}
+// Whether every row of the tile sees every key of [start, end).
+__device__ __forceinline__ bool all_seen(const KeyTiles& k, int start, int end, int window, int sinks) {
+    return end - 1 <= k.pmin && (window <= 0 || end <= sinks || start > k.pmax - window);
+}
+__device__ __forceinline__ bool seen(int j, int pos, int window, int sinks) {
+    return j <= pos && (window <= 0 || j > pos - window || j < sinks);
+}
+
+// Element offset of key j of sequence s in the cache (head 0), -1 if its page is not in the pool.
+__device__ __forceinline__ long long key_offset(const PagedAttention& p, int s, int j) {
+    const unsigned slot = static_cast<unsigned>(j) / static_cast<unsigned>(p.cache.page_size);
+    const int page = slot < static_cast<unsigned>(p.batch.table_width)
+                         ? p.batch.table[s * p.batch.table_stride + slot]
+                         : -1;
+    if (page < 0 || page >= p.cache.pages) {
+        record_bad(p.bad, kBadPage);
+        return -1;
+    }
+    return page * p.cache.page_stride + static_cast<long long>(j - static_cast<int>(slot) * p.cache.page_size) * p.cache.token_stride;
+}
+
+}  // namespace pattn
+}  // namespace sana

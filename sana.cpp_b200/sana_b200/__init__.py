@@ -15,6 +15,7 @@ from .capi import (  # noqa: F401
     load_library,
     prompt_pair_assemble,
     randn_torch_cpu,
+    rotary_frequencies,
     scheduler_config,
     scheduler_schedule,
     scheduler_schedule_config,

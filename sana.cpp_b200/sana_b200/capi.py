@@ -26,6 +26,28 @@ _i = ctypes.c_int
 _f = ctypes.c_float
 
 
+_ll = ctypes.c_longlong
+_vp = ctypes.c_void_p
+
+
+class sana_rotary(ctypes.Structure):
+    _fields_ = [("freq", _vp), ("rotated", _i), ("interleaved", _i), ("magnitude", _f)]
+
+
+class sana_paged_cache(ctypes.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("dtype", _i), ("pages", _i), ("page_size", _i), ("kv_heads", _i),
+                ("head_dim", _i), ("page_stride", _ll), ("token_stride", _ll), ("head_stride", _ll)]
+
+
+class sana_paged_batch(ctypes.Structure):
+    _fields_ = [("sequences", _i), ("rows", _i), ("max_new", _i), ("max_kv", _i), ("row_start", _vp), ("kv_len", _vp),
+                ("page_table", _vp), ("table_stride", _ll), ("table_width", _i)]
+
+
+SANA_DTYPE_F32, SANA_DTYPE_BF16, SANA_DTYPE_E4M3 = 0, 1, 2
+ROPE_SCALING = {"plain": 0, "linear": 1, "base": 2, "parts": 3}
+
+
 class SanaError(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"{_ERRS.get(code, code)}: {msg}")
@@ -70,6 +92,17 @@ def load_library():
                                               ctypes.POINTER(_i), ctypes.POINTER(_i),
                                               ctypes.POINTER(ctypes.c_int64), _i, ctypes.POINTER(ctypes.c_void_p),
                                               ctypes.POINTER(ctypes.c_uint64)]
+        _batch, _cache, _rot = (ctypes.POINTER(t) for t in (sana_paged_batch, sana_paged_cache, sana_rotary))
+        _d = ctypes.c_double
+        lib.sana_rotary_frequencies.argtypes = [_i, _d, _i, _d, _d, _d, _d, ctypes.POINTER(_d)]
+        lib.sana_op_add_rms_norm_device.argtypes = [_vp, _vp, _i, _ll, _vp, _i, _ll, _vp, _vp, _f, _f, _ll, _i, _vp, _i,
+                                                    _ll, _vp, _i]
+        lib.sana_op_rotary_device.argtypes = [_vp, _rot, _i, _ll, _i, _vp, _vp, _ll, _i, _vp, _vp, _ll, _i, _vp]
+        lib.sana_op_rotary_append_device.argtypes = [_vp, _rot, _batch, _cache, _vp, _ll, _i, _vp, _vp, _ll, _vp, _ll]
+        lib.sana_op_paged_attention_device.argtypes = [_vp, _batch, _cache, _vp, _ll, _i, _f, _i, _i, _f, _vp, _ll, _vp,
+                                                       ctypes.c_size_t]
+        lib.sana_op_paged_attention_workspace.argtypes = [_vp, _batch, _cache, _i, _i, _i]
+        lib.sana_op_paged_attention_workspace.restype = ctypes.c_size_t
         _LIB = lib
     return _LIB
 
@@ -183,6 +216,22 @@ def scheduler_schedule(n: int, flow_shift: float = 3.0):
     return ts, sg
 
 
+def rotary_frequencies(rotated: int, base: float = 10000.0, scaling: str = "plain", stretch: float = 1.0,
+                       context: float = 0.0, slow: float = 1.0, fast: float = 32.0) -> np.ndarray:
+    """sana_rotary_frequencies: radians per position of the rotated/2 pairs, float64. scaling
+    "plain", "linear", "base" or "parts" (SANA_ROPE_*). Put it on the device once
+    (torch.from_numpy(...).cuda()) for rotary_device / rotary_append_device."""
+    if scaling not in ROPE_SCALING:
+        raise ValueError(f"scaling must be one of {sorted(ROPE_SCALING)}")
+    out = np.empty(max(int(rotated), 0) // 2, np.float64)
+    rc = load_library().sana_rotary_frequencies(rotated, base, ROPE_SCALING[scaling], stretch, context, slow, fast,
+                                                out.ctypes.data_as(ctypes.POINTER(ctypes.c_double)))
+    if rc != 0:
+        raise ValueError("rotated must be even and at least 2, base positive, stretch at least 1 (and for parts "
+                         "context positive and slow below fast)")
+    return out
+
+
 class sana_scheduler_config(ctypes.Structure):
     """SanaSchedulerConfig (scheduler.h:9-20) as the C ABI carries it."""
     _fields_ = [("num_train_timesteps", _i), ("flow_shift", _f), ("use_flow_sigmas", _i), ("solver_order", _i),
@@ -233,6 +282,7 @@ class SanaCuda:
             self.close()
             raise SanaError(rc, msg)
         self.mode = mode
+        self.device = device
         self.dims: Optional[sana_dims] = None
         self._keep = None
 
@@ -350,6 +400,197 @@ class SanaCuda:
         return enc, bias
 
     # -- VAE decoder (vae.cpp:243-325) --------------------------------------------------
+    # -- operators of the text encoder's blocks, on torch CUDA tensors ------------------------
+    # They run on the handle's stream. Where that is not torch's current stream, the two are
+    # ordered by events on both sides of the call, so that inputs are ready and outputs (and
+    # memory that torch hands out again) are safe to use on torch's stream. torch's default
+    # stream is CUDA's legacy stream: set_stream(1) puts the handle on it.
+    def _run(self, name, *args):
+        import torch
+        current = torch.cuda.current_stream(self.device)
+        mine = self.stream
+        if mine == (current.cuda_stream or 1):
+            self._call(name, *args)
+            return
+        other = torch.cuda.ExternalStream(mine, device=self.device)
+        other.wait_stream(current)
+        try:
+            self._call(name, *args)
+        finally:
+            current.wait_stream(other)
+
+    def _dtype(self, t, what, allowed=("float32", "bfloat16")):
+        name = str(t.dtype).rpartition(".")[2]
+        if name not in allowed:
+            raise ValueError(f"{what} must be {' or '.join(allowed)}, not {name}")
+        if t.device.type != "cuda" or t.device.index != self.device:
+            raise ValueError(f"{what} must be on cuda:{self.device}, not {t.device}")
+        return {"float32": SANA_DTYPE_F32, "bfloat16": SANA_DTYPE_BF16}.get(name, -1)
+
+    @staticmethod
+    def _row_stride(t, what):
+        """Elements between the rows of t [rows, ...], whose rows must be contiguous."""
+        shape, stride = t.shape, t.stride()
+        width = 1
+        for n, st in zip(reversed(shape[1:]), reversed(stride[1:])):
+            if n != 1 and st != width:
+                raise ValueError(f"{what}: the elements of a row must be contiguous")
+            width *= n
+        return max(stride[0], width) if shape[0] <= 1 else stride[0]
+
+    def _vector(self, t, what, dtype, n=None):
+        self._dtype(t, what, (dtype,))
+        if t.dim() != 1 or (n is not None and t.shape[0] != n) or (t.shape[0] > 1 and t.stride(0) != 1):
+            raise ValueError(f"{what} must be a contiguous vector" + ("" if n is None else f" of {n}"))
+        return t.data_ptr()
+
+    def add_rms_norm_device(self, x, residual=None, weight=None, eps: float = 1e-6, weight_offset: float = 0.0,
+                            out_dtype=None, group: int = 0, inplace: bool = False):
+        """sana_op_add_rms_norm_device on x [rows, C]: (out, sum), or (out, scale, sum) for
+        out_dtype torch.float8_e4m3fn with one scale per `group` channels (0: per row); without a
+        residual the sum is left out of the answer. out_dtype defaults to x's. inplace writes the
+        sum over the residual."""
+        import torch
+        xt = self._dtype(x, "x")
+        if x.dim() != 2:
+            raise ValueError("x must be [rows, C]")
+        rows, C = x.shape
+        out_dtype = out_dtype or x.dtype
+        ot = {torch.float32: SANA_DTYPE_F32, torch.bfloat16: SANA_DTYPE_BF16, torch.float8_e4m3fn: SANA_DTYPE_E4M3}.get(out_dtype)
+        if ot is None:
+            raise ValueError("out_dtype must be float32, bfloat16 or float8_e4m3fn")
+        rt, ldr, rp, total, tp = 0, C, None, None, None
+        if residual is not None:
+            rt = self._dtype(residual, "residual")
+            if residual.shape != x.shape:
+                raise ValueError("residual must have x's shape")
+            ldr, rp = self._row_stride(residual, "residual"), residual.data_ptr()
+            total = residual if inplace else torch.empty_strided((rows, C), (ldr, 1), dtype=residual.dtype, device=x.device)
+            tp = total.data_ptr()
+        wp = None if weight is None else self._vector(weight, "weight", "float32", C)
+        out = torch.empty((rows, C), dtype=out_dtype, device=x.device)
+        scale = None
+        if ot == SANA_DTYPE_E4M3:
+            scale = torch.empty((rows, -(-C // group) if group > 0 else 1), dtype=torch.float32, device=x.device)
+        self._run("sana_op_add_rms_norm_device", x.data_ptr(), xt, self._row_stride(x, "x"), rp, rt, ldr, tp, wp,
+                  weight_offset, eps, rows, C, out.data_ptr(), ot, C, None if scale is None else scale.data_ptr(), group)
+        got = [out] + ([scale] if scale is not None else []) + ([total] if total is not None else [])
+        return got[0] if len(got) == 1 else tuple(got)
+
+    def _heads(self, t, what, rows=None, heads=None, dim=None, dtype=None):
+        dt = self._dtype(t, what)
+        if t.dim() != 3 or (rows is not None and t.shape[0] != rows) or (heads is not None and t.shape[1] != heads) or (
+                dim is not None and t.shape[2] != dim):
+            raise ValueError(f"{what} must be [{'rows' if rows is None else rows}, {'heads' if heads is None else heads}, "
+                             f"{'head_dim' if dim is None else dim}]")
+        if dtype is not None and dt != dtype:
+            raise ValueError(f"{what} must have the type of the others")
+        return dt, self._row_stride(t, what)
+
+    def _rotary(self, frequencies, interleaved, magnitude):
+        n = frequencies.shape[0] if frequencies.dim() == 1 else -1
+        return sana_rotary(self._vector(frequencies, "frequencies", "float64", n), 2 * n, 1 if interleaved else 0, magnitude)
+
+    def rotary_device(self, q, k, positions, frequencies, interleaved: bool = False, magnitude: float = 1.0,
+                      inplace: bool = False):
+        """sana_op_rotary_device: q [rows, q_heads, D] and k [rows, kv_heads, D] (or None) turned
+        at the int32 positions [rows]; frequencies float64 [rotated/2] on the device."""
+        import torch
+        dt, ldq = self._heads(q, "q")
+        rows, heads, D = q.shape
+        kv, ldk, kp, k_out = 0, 0, None, None
+        if k is not None:
+            _, ldk = self._heads(k, "k", rows, None, D, dt)
+            kv, kp = k.shape[1], k.data_ptr()
+            k_out = k if inplace else torch.empty_strided(k.shape, (ldk, D, 1), dtype=k.dtype, device=k.device)
+        q_out = q if inplace else torch.empty_strided(q.shape, (ldq, D, 1), dtype=q.dtype, device=q.device)
+        rot = self._rotary(frequencies, interleaved, magnitude)
+        self._run("sana_op_rotary_device", ctypes.byref(rot), dt, rows, D, self._vector(positions, "positions", "int32", rows),
+                  q.data_ptr(), ldq, heads, q_out.data_ptr(), kp, ldk, kv, None if k is None else k_out.data_ptr())
+        return q_out if k is None else (q_out, k_out)
+
+    def _cache(self, k_cache, v_cache):
+        dt = self._dtype(k_cache, "k_cache")
+        shape, st = k_cache.shape, k_cache.stride()
+        if len(shape) != 4 or v_cache.shape != shape or v_cache.stride() != st or v_cache.dtype != k_cache.dtype:
+            raise ValueError("k_cache and v_cache must be [pages, page_size, kv_heads, D] of one type and layout")
+        self._dtype(v_cache, "v_cache")
+        if shape[3] > 1 and st[3] != 1:
+            raise ValueError("a head's channels must be contiguous in the cache")
+        return sana_paged_cache(k_cache.data_ptr(), v_cache.data_ptr(), dt, shape[0], shape[1], shape[2], shape[3], st[0],
+                                st[1], st[2])
+
+    def _batch(self, rows, row_start, kv_len, page_table, max_new, max_kv):
+        S = kv_len.shape[0]
+        self._dtype(page_table, "page_table", ("int32",))
+        if page_table.dim() != 2 or page_table.shape[0] != S or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+            raise ValueError("page_table must be [sequences, pages of a sequence] with contiguous rows")
+        width = page_table.shape[1]
+        return sana_paged_batch(S, rows, max_new, max_kv, self._vector(row_start, "row_start", "int32", S + 1),
+                                self._vector(kv_len, "kv_len", "int32", S), page_table.data_ptr(),
+                                page_table.stride(0) if S > 1 else width, width)
+
+    def rotary_append_device(self, q, k, v, frequencies, k_cache, v_cache, row_start, kv_len, page_table, max_new: int,
+                             interleaved: bool = False, magnitude: float = 1.0, inplace: bool = False):
+        """sana_op_rotary_append_device: turns q [rows, q_heads, D] (returned) and k, and writes k
+        and v [rows, kv_heads, D] into their tokens' places in the caches [pages, page_size,
+        kv_heads, D]. row_start [S + 1], kv_len [S] (the new tokens included) and page_table
+        [S, pages of a sequence] are int32; frequencies None appends without turning (q is then
+        returned as it is)."""
+        import torch
+        cache = self._cache(k_cache, v_cache)
+        rows, heads = k.shape[0], 0
+        _, ldk = self._heads(k, "k", rows, cache.kv_heads, cache.head_dim, cache.dtype)
+        _, ldv = self._heads(v, "v", rows, cache.kv_heads, cache.head_dim, cache.dtype)
+        rot, qp, ldq, q_out, qo = None, None, 0, q, None
+        if frequencies is not None:
+            rot = ctypes.byref(self._rotary(frequencies, interleaved, magnitude))
+            if q is not None:
+                _, ldq = self._heads(q, "q", rows, None, cache.head_dim, cache.dtype)
+                heads, qp = q.shape[1], q.data_ptr()
+                q_out = q if inplace else torch.empty_strided(q.shape, (ldq, cache.head_dim, 1), dtype=q.dtype, device=q.device)
+                qo = q_out.data_ptr()
+        # the append reads each row's place from the lengths alone: any position of an int is within bounds
+        batch = self._batch(rows, row_start, kv_len, page_table, max_new, 0x7fffffff)
+        self._run("sana_op_rotary_append_device", rot, ctypes.byref(batch), ctypes.byref(cache), qp, ldq, heads, qo,
+                  k.data_ptr(), ldk, v.data_ptr(), ldv)
+        return q_out
+
+    def paged_attention_device(self, q, k_cache, v_cache, row_start, kv_len, page_table, max_new: int, max_kv: int,
+                               scale: Optional[float] = None, window: int = 0, sinks: int = 0, softcap: float = 0.0,
+                               out=None, workspace=None):
+        """sana_op_paged_attention_device: causal attention of the new rows q [rows, q_heads, D]
+        over the caches [pages, page_size, kv_heads, D] that hold their keys and values already.
+        scale defaults to 1/sqrt(D); max_new and max_kv bound the new and the cached tokens of
+        any sequence. Rows behind the last sequence keep what `out` holds (without `out`:
+        anything). workspace: a uint8 tensor to use instead of one of the call's own."""
+        import torch
+        cache = self._cache(k_cache, v_cache)
+        _, ldq = self._heads(q, "q", None, None, cache.head_dim, cache.dtype)
+        rows, heads, D = q.shape
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _, ldo = self._heads(out, "out", rows, heads, D, cache.dtype)
+        batch = self._batch(rows, row_start, kv_len, page_table, max_new, max_kv)
+        bp, cp = ctypes.byref(batch), ctypes.byref(cache)
+        if workspace is None:
+            need = self.lib.sana_op_paged_attention_workspace(self.h, bp, cp, heads, window, sinks)
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        else:
+            self._vector(workspace, "workspace", "uint8")
+        wp, wn = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.shape[0])
+        self._run("sana_op_paged_attention_device", bp, cp, q.data_ptr(), ldq, heads, D ** -0.5 if scale is None else scale,
+                  window, sinks, softcap, out.data_ptr(), ldo, wp, wn)
+        return out
+
+    def paged_attention_workspace(self, q, k_cache, v_cache, row_start, kv_len, page_table, max_new: int, max_kv: int,
+                                  window: int = 0, sinks: int = 0) -> int:
+        """Bytes of workspace that paged_attention_device needs for these sizes."""
+        batch = self._batch(q.shape[0], row_start, kv_len, page_table, max_new, max_kv)
+        return int(self.lib.sana_op_paged_attention_workspace(self.h, ctypes.byref(batch),
+                                                              ctypes.byref(self._cache(k_cache, v_cache)), q.shape[1],
+                                                              window, sinks))
+
     def vae_upload(self, dims, tensors):
         """dims: synthetic_vae.VaeDims; tensors: fp32 arrays in its upload order."""
         from .synthetic_vae import dims_struct
