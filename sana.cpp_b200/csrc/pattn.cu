@@ -2,7 +2,8 @@
 //   out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  s_j = scale q.k_j or cap tanh(scale q.k_j / cap),
 // in one pass over the keys with the running maximum m and sum; scores, statistics and sums fp32.
 // Two kernels here: a tensor-core one for bf16 (mma.sync; single tokens and short chunks, which
-// read much and compute little) and a CUDA-core one for fp32 and for what the first does not take.
+// read much and compute little) and a CUDA-core one for fp32 and for what the first does not take;
+// pattn_tc.cu has the one for chunks that fill 128-row tiles.
 // pattn.cuh has the packing of rows, the key ranges and the splits.
 #include <algorithm>
 #include <cmath>
@@ -508,7 +509,14 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
 }
 
 // --- plan and launch ----------------------------------------------------------------------------
-enum Kind { kSimt, kMma };
+enum Kind { kSimt, kMma, kTc };
+
+// The tcgen05 kernel's 128-row tiles take over from the mma.sync kernel's 64-row ones above this
+// many packed rows of the longest chunk.
+constexpr long long kTcRows = 64;
+bool wants_tc(const PagedAttention& p) {
+    return static_cast<long long>(p.batch.max_new) * (p.q_heads / p.cache.kv_heads) > kTcRows;
+}
 
 bool cache_fits_mma(const PagedCache& c) {
     return c.dtype == kBf16 && c.D % 8 == 0 && (reinterpret_cast<uintptr_t>(c.k) & 15) == 0 &&
@@ -527,6 +535,10 @@ Args plan(const PagedAttention& p, Kind kind, int num_sms) {
         a.BM = kSRows;
         a.BN = kSKeys;
         resident = 2;
+    } else if (kind == kTc) {
+        a.BM = tc_rows(p.cache.D);
+        a.BN = tc_keys(p.cache.D);
+        resident = 1;
     } else {
         a.BM = packed <= 16 ? 16 : packed <= 32 ? 32 : 64;
         a.BN = 64;
@@ -540,7 +552,7 @@ Args plan(const PagedAttention& p, Kind kind, int num_sms) {
     const long long base = static_cast<long long>(p.batch.S) * p.cache.kv_heads * a.row_tiles;
     // One sequence: one wave of equal blocks. Several: their lengths differ and only the longest is
     // known here, so blocks of a few waves' size even them out.
-    const long long want = static_cast<long long>(num_sms) * resident * (p.batch.S == 1 ? 1 : 4);
+    const long long want = static_cast<long long>(num_sms) * resident * (p.batch.S == 1 || kind == kTc ? 1 : 4);
     const long long splits = std::max<long long>(1, std::min<long long>(want / std::max<long long>(base, 1), tiles / 2));
     a.split_tiles = std::max(1, ceil_div(tiles, splits));
     a.splits = ceil_div(tiles, a.split_tiles);
@@ -590,10 +602,13 @@ void launch_simt(const Args& a, dim3 grid, cudaStream_t st) {
 
 using namespace pattn;
 
-// Alignment of q and out is not known when the workspace is asked for: the larger of the two kinds' needs.
+// Alignment of q and out, and the scale, are not known when the workspace is asked for: the largest of the kinds' needs.
 size_t paged_attention_workspace(const PagedAttention& p, int num_sms) {
     size_t n = part_bytes(plan(p, kSimt, num_sms));
-    if (cache_fits_mma(p.cache)) n = std::max(n, part_bytes(plan(p, kMma, num_sms)));
+    if (cache_fits_mma(p.cache)) {
+        n = std::max(n, part_bytes(plan(p, kMma, num_sms)));
+        if (wants_tc(p)) n = std::max(n, part_bytes(plan(p, kTc, num_sms)));
+    }
     return n;
 }
 
@@ -601,14 +616,18 @@ void paged_attention(const PagedAttention& p, int num_sms, cudaStream_t st) {
     if (p.batch.S == 0 || p.batch.rows == 0 || p.batch.max_new == 0) return;
     const bool mma = cache_fits_mma(p.cache) && (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 &&
                      (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.ldq % 8 == 0 && p.ldo % 8 == 0;
-    Args a = plan(p, mma ? kMma : kSimt, num_sms);
+    // the tcgen05 kernel maps a tile's largest score alone, which takes a map that rises: scale > 0
+    const Kind kind = !mma ? kSimt : wants_tc(p) && p.scale > 0.f ? kTc : kMma;
+    Args a = plan(p, kind, num_sms);
     const size_t n = static_cast<size_t>(a.splits) * p.batch.rows * p.q_heads;
     a.ml = static_cast<float2*>(p.workspace);
     a.part = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + ((n * sizeof(float2) + 15) & ~static_cast<size_t>(15)));
     const long long blocks = static_cast<long long>(p.batch.S) * a.splits * a.row_tiles;
     SANA_REQUIRE(blocks <= 0x7fffffffLL, "paged attention: too many sequences times row tiles for one launch");
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(p.cache.kv_heads));
-    if (mma) {
+    if (kind == kTc) {
+        launch_tc(a, grid, st);
+    } else if (mma) {
         if (p.cache.D <= 64) launch_mma_rows<64>(a, grid, st);
         else if (p.cache.D <= 128) launch_mma_rows<128>(a, grid, st);
         else launch_mma_rows<256>(a, grid, st);

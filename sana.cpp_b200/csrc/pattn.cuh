@@ -108,5 +108,10 @@ __device__ __forceinline__ long long key_offset(const PagedAttention& p, int s, 
     return page * p.cache.page_stride + static_cast<long long>(j - static_cast<int>(slot) * p.cache.page_size) * p.cache.token_stride;
 }
 
+// pattn_tc.cu: packed rows and keys of a block's tile for a head size, and the launch.
+int tc_rows(int D);
+int tc_keys(int D);
+void launch_tc(const Args& a, dim3 grid, cudaStream_t st);
+
 }  // namespace pattn
 }  // namespace sana

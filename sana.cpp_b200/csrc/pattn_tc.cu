@@ -1,0 +1,537 @@
+// Attention of a chunk of new tokens over a paged cache on the 5th-generation tensor cores
+// (tcgen05), for chunks whose packed rows fill 128-row tiles; pattn.cuh has the packing, key
+// ranges and splits, pattn.cu the other kernels and the choice between them.
+//
+// One block holds 256 packed rows as two tiles of 128 (one tile for head sizes above 128, whose
+// output fills the tensor memory, and where fewer rows are left) and walks the key tiles:
+//   S = Q K^T into tensor memory; a thread per row reads its scores, masks them where the tile is
+//   not seen whole, and writes P = 2^(s - m) as bf16 over S; O += P V with P from tensor memory.
+// The unit of work is one S tile: unit u uses slot u & 1 of two. With two row tiles, u is row tile
+// u & 1 at key tile u >> 1; with one, key tile u. The issuing thread runs S(0), S(1), then PV(u),
+// S(u + 2) for every u, so that the tensor cores have the other slot's products while the softmax
+// of one is under way, and S(u + 2) may overwrite P(u) since products run in order.
+//
+// The running maximum is a reference that moves only when a row's maximum passes it by 8 (a
+// factor of 256): the output is rescaled in tensor memory then, by the row's own threads, and
+// almost never after the first tiles. P stays below 2^8, its sum is fp32, its rounding to bf16 is
+// relative, and the division at the end takes the reference out.
+//
+// Keys and values come by 16-byte cp.async from 128 producer threads (pages end anywhere inside a
+// tile; what no row sees is not read but written as zeros), into the 128-byte-swizzled layout of
+// the matrix descriptors: slabs of 64 channels, 128-byte rows, chunk c of row r at c ^ (r & 7). K
+// and Q are K-major operands, V is MN-major (its channels contiguous).
+#include "pattn.cuh"
+#include "tcgen05.cuh"
+#include "tma.h"
+
+namespace sana {
+namespace pattn {
+namespace {
+
+using namespace tc;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kSoftmaxWarps = 8, kProducerWarps = 4;
+constexpr int kThreads = (kSoftmaxWarps + kProducerWarps + 1) * 32;
+constexpr int kMmaWarp = kSoftmaxWarps + kProducerWarps;
+constexpr int kProducers = kProducerWarps * 32;
+
+template <int DP>
+struct TcShape {
+    static constexpr int kTiles = DP <= 128 ? 2 : 1;     // row tiles of 128
+    static constexpr int kRows = 128 * kTiles;
+    static constexpr int kKeys = DP <= 128 ? 128 : 64;   // per key tile
+    static constexpr int kSlabs = DP / 64;
+    static constexpr int kStages = DP == 64 ? 4 : 2;
+    static constexpr int kQBytes = kTiles * 128 * DP * 2;
+    static constexpr int kTileBytes = kKeys * DP * 2;    // of K or of V
+    static constexpr int kBarriers = 4 * kStages + 6 + 1;
+    static constexpr int kSmem = 1024 + kQBytes + kStages * 2 * kTileBytes + 2 * kKeys * 8 + kBarriers * 8 + 64;
+    // tensor memory columns: S slots at 0 and kKeys, O behind them
+    static constexpr int kO = 2 * kKeys;
+    static constexpr int kCols = kO + kTiles * DP;
+    static_assert(kCols <= 512, "tensor memory");
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// D += A B with A (bf16 pairs) in tensor memory
+__device__ __forceinline__ void umma_bf16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                             uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Descriptor of an MN-major operand in the 128-byte swizzle: 64 channels of a row contiguous, groups
+// of eight rows 1024 bytes apart (the stride offset), slabs of 64 channels `slab` bytes apart (the
+// leading offset).
+__device__ __forceinline__ uint64_t mnmajor_sw128_desc(uint32_t smem_addr, uint32_t slab) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
+    d |= static_cast<uint64_t>((slab >> 4) & 0x3FFFu) << 16;
+    d |= static_cast<uint64_t>(1024u >> 4) << 32;
+    d |= static_cast<uint64_t>(1u) << 46;
+    d |= static_cast<uint64_t>(2u) << 61;
+    return d;
+}
+constexpr uint32_t kBTransposed = 1u << 16;  // instruction descriptor: B is MN-major
+
+__device__ __forceinline__ uint32_t pack_bf2(float lo, float hi) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&b);
+}
+// cap tanh(x / cap) log2(e), as in pattn.cu
+__device__ __forceinline__ float soft_cap_log2(float x, float in, float out) {
+    return fmaf(-2.f * out, rcp_approx(1.f + ex2_approx(x * in)), out);
+}
+
+// A bounded wait of a whole warp, with one answer for all its lanes.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* err) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, kTimeout));
+}
+// Barrier of the producer warps, with the conjunction of what they bring.
+__device__ __forceinline__ bool producers_all(bool ok) {
+    int all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.and.pred q, 1, %2, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+        : "=r"(all)
+        : "r"(ok ? 1 : 0), "n"(kProducers)
+        : "memory");
+    return all != 0;
+}
+
+template <int DP>
+__global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_constant__ Args a) {
+    using Sh = TcShape<DP>;
+    constexpr int BN = Sh::kKeys, ST = Sh::kStages;
+    extern __shared__ unsigned char smem_raw[];
+    const PagedAttention& p = a.p;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = p.cache.D;
+    const int tile = a.row_tiles - 1 - static_cast<int>(blockIdx.x % a.row_tiles);
+    const int rest = blockIdx.x / a.row_tiles, split = rest % a.splits, s = rest / a.splits, kvh = blockIdx.y;
+    const Sequence sq = sequence(p, s, blockIdx.x % (a.row_tiles * a.splits) == 0 && kvh == 0 && tid == 0);
+    const int rr0 = tile * Sh::kRows, n_rows = sq.n_new * a.G;
+    if (!sq.ok || rr0 >= n_rows) return;
+    const KeyTiles kt = key_tiles(sq.past, sq.n_new, a.G, rr0, rr0 + Sh::kRows, p.window, p.sinks, BN);
+    const int t0 = split * a.split_tiles, n = min(kt.n, t0 + a.split_tiles) - t0;
+    if (n <= 0) return;
+    const bool partial = kt.n > a.split_tiles;
+    const bool pair = Sh::kTiles == 2 && rr0 + 128 < n_rows;
+    const int units = pair ? 2 * n : n;
+
+    // shared memory, 1024-byte aligned for the swizzle
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    unsigned char* sm = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t q_s = base, kv_s = base + Sh::kQBytes;
+    constexpr int kOffs = Sh::kQBytes + ST * 2 * Sh::kTileBytes;
+    long long* offs = reinterpret_cast<long long*>(sm + kOffs);  // [2][BN]
+    const uint32_t bars = base + kOffs + 2 * BN * 8;
+    auto k_full = [&](int i) { return bars + 8u * i; };
+    auto v_full = [&](int i) { return bars + 8u * (ST + i); };
+    auto k_empty = [&](int i) { return bars + 8u * (2 * ST + i); };
+    auto v_empty = [&](int i) { return bars + 8u * (3 * ST + i); };
+    auto s_full = [&](int i) { return bars + 8u * (4 * ST + i); };
+    auto p_full = [&](int i) { return bars + 8u * (4 * ST + 2 + i); };
+    auto pv_done = [&](int i) { return bars + 8u * (4 * ST + 4 + i); };
+    const uint32_t drained = bars + 8u * (4 * ST + 6);
+    int* words = reinterpret_cast<int*>(sm + kOffs + 2 * BN * 8 + Sh::kBarriers * 8);  // [0] tensor memory, [1] bad page, [2] not finite
+
+    if (warp == kMmaWarp) {
+        tmem_alloc(smem_u32(words), 512);
+        tmem_relinquish();
+    }
+    if (tid == 0) {
+        for (int i = 0; i < ST; ++i) {
+            mbar_init(k_full(i), kProducerWarps);
+            mbar_init(v_full(i), kProducerWarps);
+            mbar_init(k_empty(i), 1);
+            mbar_init(v_empty(i), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(s_full(i), 1);
+            mbar_init(p_full(i), 4);
+            mbar_init(pv_done(i), 1);
+        }
+        mbar_init(drained, 1);
+        fence_barrier_init();
+        words[1] = 0;
+        words[2] = 0;
+    }
+    // Q: every thread helps
+    {
+        const bf16* q = static_cast<const bf16*>(p.q);
+        const int rows = pair ? 256 : 128;
+        for (int i = tid; i < rows * (DP / 8); i += kThreads) {
+            const int r = i / (DP / 8), c = i % (DP / 8), rr = rr0 + r;
+            const bool in = rr < n_rows && c * 8 < D;
+            const int t = rr / a.G;
+            const bf16* src = in ? q + (sq.row0 + t) * p.ldq + static_cast<long long>(kvh * a.G + rr - t * a.G) * D + c * 8 : q;
+            const int rt = r & 127;
+            cp_async16(q_s + (r >> 7) * (128 * DP * 2) + (c >> 3) * (128 * 128) + rt * 128 + (((c & 7) ^ (rt & 7)) << 4), src, in);
+        }
+        cp_async_commit();
+    }
+    __syncthreads();  // words[] are set; the pages of this block's keys are checked while Q is on its way
+    {
+        int lo, hi, unused;
+        const int b0 = max(t0, kt.n_sink);
+        if (t0 < kt.n_sink) {
+            key_range(kt, t0, BN, lo, unused);
+            key_range(kt, min(kt.n_sink, t0 + n) - 1, BN, unused, hi);
+            for (int j = lo / p.cache.page_size + tid; j <= (hi - 1) / p.cache.page_size; j += kThreads)
+                if (key_offset(p, s, min(max(j * p.cache.page_size, lo), hi - 1)) < 0) words[1] = 1;
+        }
+        if (b0 < t0 + n) {
+            key_range(kt, b0, BN, lo, unused);
+            key_range(kt, t0 + n - 1, BN, unused, hi);
+            for (int j = lo / p.cache.page_size + tid; j <= (hi - 1) / p.cache.page_size; j += kThreads)
+                if (key_offset(p, s, min(max(j * p.cache.page_size, lo), hi - 1)) < 0) words[1] = 1;
+        }
+    }
+    cp_async_wait<0>();
+    fence_proxy_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(words);
+    const bool bad_page = *reinterpret_cast<volatile int*>(words + 1) != 0;
+
+    float m = -INFINITY, l = 0.f;  // of a softmax thread's row
+    const int wg = warp >> 2;      // softmax: row tile; tensor memory lanes 32 (warp & 3) ..
+    const int my_rr = rr0 + wg * 128 + (tid & 127);
+    const int my_pos = warp < kSoftmaxWarps && my_rr < n_rows ? sq.past + my_rr / a.G : -1;
+    const uint32_t my_lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);
+    const bool softmax_on = warp < kSoftmaxWarps && (wg == 0 || pair);
+
+    if (warp < kSoftmaxWarps) {
+        if (softmax_on) {
+            const float scale_log2 = p.scale * kLog2e;
+            const float cap_in = p.softcap > 0.f ? 2.f * scale_log2 / p.softcap : 0.f, cap_out = p.softcap * kLog2e;
+            // positions of this row tile
+            const int last = min(n_rows, rr0 + wg * 128 + 128) - 1;
+            KeyTiles mine = kt;
+            mine.pmin = sq.past + (rr0 + wg * 128) / a.G;
+            mine.pmax = sq.past + last / a.G;
+            const uint32_t o_t = my_lanes + Sh::kO + wg * DP;
+            const int step = pair ? 2 : 1;
+            for (int u = pair ? wg : 0; u < units; u += step) {
+                const int slot = u & 1, kv = pair ? u >> 1 : u;
+                int start, end;
+                key_range(kt, t0 + kv, BN, start, end);
+                const bool whole = end - start == BN && !bad_page && all_seen(mine, start, end, p.window, p.sinks);
+                if (!warp_wait(s_full(slot), (u >> 1) & 1, p.err)) break;
+                tc_fence_after();
+                const uint32_t s_t = my_lanes + slot * BN;
+                auto visible = [&](int j) {
+                    return j < end && seen(j, my_pos, p.window, p.sinks) && (!bad_page || key_offset(p, s, j) >= 0);
+                };
+                float mx = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < BN / 32; ++c) {
+                    uint32_t r[32];
+                    tmem_ld32(s_t + c * 32, r);
+                    tmem_wait_ld();
+                    if (whole) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(r[i]));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (visible(start + c * 32 + i)) mx = fmaxf(mx, __uint_as_float(r[i]));
+                    }
+                }
+                // both maps rise with the score (scale > 0), so the maximum is mapped alone
+                if (mx != -INFINITY) mx = p.softcap > 0.f ? soft_cap_log2(mx, cap_in, cap_out) : mx * scale_log2;
+                const bool move = mx > m + 8.f || (m == -INFINITY && mx > -INFINITY);
+                float alpha = 1.f;
+                if (move) {
+                    alpha = ex2_approx(m - mx);
+                    m = mx;
+                    l *= alpha;
+                }
+                if (kv > 0 && __any_sync(0xffffffffu, move)) {  // O holds sums against the old reference
+                    const int before = u - step;
+                    if (!warp_wait(pv_done(before & 1), (before >> 1) & 1, p.err)) break;
+                    tc_fence_after();
+                    for (int c = 0; c < D; c += 16) {
+                        uint32_t r[16];
+                        tmem_ld16(o_t + c, r);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+                        tmem_st16(o_t + c, r);
+                    }
+                }
+                const float ref = m == -INFINITY ? 0.f : m;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < BN / 32; ++c) {
+                    uint32_t r[32], pk[16];
+                    tmem_ld32(s_t + c * 32, r);
+                    tmem_wait_ld();
+                    if (p.softcap > 0.f) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            r[i] = __float_as_uint(soft_cap_log2(__uint_as_float(r[i]), cap_in, cap_out) - ref);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            r[i] = __float_as_uint(fmaf(__uint_as_float(r[i]), scale_log2, -ref));
+                    }
+                    if (!whole) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (!visible(start + c * 32 + i)) r[i] = 0xff800000u;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float x = ex2_approx(__uint_as_float(r[2 * i])), y = ex2_approx(__uint_as_float(r[2 * i + 1]));
+                        sum[(2 * i) & 3] += x;
+                        sum[(2 * i + 1) & 3] += y;
+                        pk[i] = pack_bf2(x, y);
+                    }
+                    tmem_st16(s_t + c * 16, pk);  // over scores that this row has read
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full(slot));
+            }
+        }
+    } else if (warp < kMmaWarp) {
+        const int pt = tid - kSoftmaxWarps * 32;
+        const bf16* kc = static_cast<const bf16*>(p.cache.k) + kvh * p.cache.head_stride;
+        const bf16* vc = static_cast<const bf16*>(p.cache.v) + kvh * p.cache.head_stride;
+        const int slabs = (D + 63) / 64;
+        auto offset_of = [&](int i) -> long long {
+            int start, end;
+            key_range(kt, t0 + i, BN, start, end);
+            return start + pt < end ? key_offset(p, s, start + pt) : -1;
+        };
+        auto chunk_at = [&](int slab, int key) { return slab * (BN * 128) + key * 128 + (((pt & 7) ^ (key & 7)) << 4); };
+        auto load = [&](uint32_t dst, const bf16* src, const long long* of) {
+            for (int slab = 0; slab < slabs; ++slab) {
+                const int d = slab * 64 + (pt & 7) * 8;
+#pragma unroll
+                for (int x = 0; x < BN / 16; ++x) {
+                    const int key = x * 16 + (pt >> 3);
+                    const long long off = of[key];
+                    const bool in = off >= 0 && d < D;
+                    cp_async16(dst + chunk_at(slab, key), in ? src + off + d : src, in);
+                }
+            }
+            cp_async_commit();
+        };
+        auto publish = [&](uint32_t bar) {  // this warp's part of a tile has landed
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
+        // Values that are not finite, in a tile that not every row sees whole, would reach the rows that do
+        // not see them as 0 * v: zeros take their place, and the rows that see them get them at the end.
+        auto clean = [&](int i) {
+            int start, end;
+            key_range(kt, t0 + i, BN, start, end);
+            if (all_seen(kt, start, end, p.window, p.sinks)) return;
+            unsigned char* v = sm + Sh::kQBytes + (i % ST) * (2 * Sh::kTileBytes) + Sh::kTileBytes;
+            for (int slab = 0; slab < slabs; ++slab) {
+#pragma unroll
+                for (int x = 0; x < BN / 16; ++x) {
+                    uint4* w = reinterpret_cast<uint4*>(v + chunk_at(slab, x * 16 + (pt >> 3)));
+                    uint4 c = *w;
+                    uint32_t e[4] = {c.x, c.y, c.z, c.w};
+                    bool bad = false;
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        if ((e[y] & 0x7f80u) == 0x7f80u) e[y] &= 0xffff0000u, bad = true;
+                        if ((e[y] & 0x7f800000u) == 0x7f800000u) e[y] &= 0x0000ffffu, bad = true;
+                    }
+                    if (bad) {
+                        *w = make_uint4(e[0], e[1], e[2], e[3]);
+                        words[2] = 1;
+                    }
+                }
+            }
+        };
+        long long next = pt < BN ? offset_of(0) : -1;
+        bool ok = true;
+        for (int i = 0; i < n; ++i) {
+            const int st = i % ST, use = i / ST;
+            long long* of = offs + (i & 1) * BN;
+            if (pt < BN) of[pt] = next;
+            ok = producers_all(ok);  // after a failed wait the warps leave together
+            if (!ok) break;
+            next = pt < BN && i + 1 < n ? offset_of(i + 1) : -1;
+            const uint32_t ks = kv_s + st * (2 * Sh::kTileBytes);
+            ok = warp_wait(k_empty(st), (use & 1) ^ 1, p.err);
+            if (ok) load(ks, kc, of);
+            else cp_async_commit();
+            if (i > 0) {
+                cp_async_wait<1>();
+                clean(i - 1);
+                publish(v_full((i - 1) % ST));
+            }
+            ok = ok && warp_wait(v_empty(st), (use & 1) ^ 1, p.err);
+            if (ok) load(ks + Sh::kTileBytes, vc, of);
+            else cp_async_commit();
+            cp_async_wait<1>();
+            if (ok) publish(k_full(st));
+        }
+        cp_async_wait<0>();
+        if (ok) {
+            clean(n - 1);
+            publish(v_full((n - 1) % ST));
+        }
+    } else if (lane == 0) {
+        const int d16 = (D + 15) & ~15;
+        const uint32_t idesc_s = idesc_bf16_f32(128, BN);
+        const uint32_t idesc_o = idesc_bf16_f32(128, d16) | kBTransposed;
+        auto scores = [&](int u) -> bool {
+            const int slot = u & 1, kv = pair ? u >> 1 : u, t = pair ? u & 1 : 0, st = kv % ST;
+            if (!mbar_wait(k_full(st), (kv / ST) & 1, p.err, kTimeout)) return false;
+            tc_fence_after();
+            const uint32_t qa = q_s + t * (128 * DP * 2), ka = kv_s + st * (2 * Sh::kTileBytes);
+            for (int k = 0; k < d16 / 16; ++k) {
+                const uint32_t in = (k & 3) * 32;
+                umma_bf16(tmem + slot * BN, kmajor_sw128_desc(qa + (k >> 2) * (128 * 128) + in),
+                          kmajor_sw128_desc(ka + (k >> 2) * (BN * 128) + in), idesc_s, k > 0);
+            }
+            umma_commit(s_full(slot));
+            if (!pair || t == 1) umma_commit(k_empty(st));
+            return true;
+        };
+        bool ok = scores(0) && (units < 2 || scores(1));
+        for (int u = 0; u < units && ok; ++u) {
+            const int slot = u & 1, kv = pair ? u >> 1 : u, t = pair ? u & 1 : 0, st = kv % ST;
+            ok = mbar_wait(v_full(st), (kv / ST) & 1, p.err, kTimeout) && mbar_wait(p_full(slot), (u >> 1) & 1, p.err, kTimeout);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t va = kv_s + st * (2 * Sh::kTileBytes) + Sh::kTileBytes;
+#pragma unroll
+            for (int k = 0; k < BN / 16; ++k)
+                umma_bf16_ta(tmem + Sh::kO + t * DP, tmem + slot * BN + k * 8, mnmajor_sw128_desc(va + k * 2048, BN * 128),
+                             idesc_o, kv > 0 || k > 0);
+            umma_commit(pv_done(slot));
+            if (!pair || t == 1) umma_commit(v_empty(st));
+            if (u + 2 < units) ok = scores(u + 2);
+        }
+        umma_commit(drained);  // whatever was issued has run before the tensor memory is given back
+        mbar_wait_quiet(drained, 0);
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+
+    if (softmax_on) {
+        const int h_in = my_rr % a.G;
+        const long long row = sq.row0 + my_rr / a.G;
+        const int h = kvh * a.G + h_in;
+        const bool live = my_rr < n_rows;
+        const long long at = (static_cast<long long>(split) * p.batch.rows + row) * p.q_heads + h;
+        const float inv = partial ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+        if (partial && live) a.ml[at] = make_float2(m, l);
+        const bool repair = *reinterpret_cast<volatile int*>(words + 2) != 0;
+        bf16* out = static_cast<bf16*>(p.out) + row * p.ldo + static_cast<long long>(h) * D;
+        for (int c = 0; c < D; c += 16) {
+            uint32_t r[16];
+            tmem_ld16(my_lanes + Sh::kO + wg * DP + c, r);
+            tmem_wait_ld();
+            float o[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __uint_as_float(r[i]) * inv;
+            if (repair && live) {
+                const bf16* vc = static_cast<const bf16*>(p.cache.v) + kvh * p.cache.head_stride;
+                for (int t = 0; t < n; ++t) {
+                    int start, end;
+                    key_range(kt, t0 + t, BN, start, end);
+                    if (all_seen(kt, start, end, p.window, p.sinks)) continue;
+                    for (int j = start; j < end; ++j) {
+                        if (!seen(j, my_pos, p.window, p.sinks)) continue;
+                        const long long off = key_offset(p, s, j);
+                        if (off < 0) continue;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            if (c + i >= D) continue;
+                            const float v = __bfloat162float(vc[off + c + i]);
+                            if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) o[i] += v;
+                        }
+                    }
+                }
+            }
+            if (!live) continue;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                if (c + 8 * b >= D) continue;
+                const float* x = o + 8 * b;
+                if (partial) {
+                    float4* dst = reinterpret_cast<float4*>(a.part + at * D + c + 8 * b);
+                    dst[0] = make_float4(x[0], x[1], x[2], x[3]);
+                    dst[1] = make_float4(x[4], x[5], x[6], x[7]);
+                } else {
+                    *reinterpret_cast<uint4*>(out + c + 8 * b) =
+                        make_uint4(pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3]), pack_bf2(x[4], x[5]), pack_bf2(x[6], x[7]));
+                }
+            }
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
+}
+
+template <int DP>
+void launch(const Args& a, dim3 grid, cudaStream_t st) {
+    static PerDeviceOnce once;
+    using Sh = TcShape<DP>;
+    static_assert(Sh::kSmem <= 232448, "shared memory of one block");
+    if (once.pending()) {
+        SANA_CUDA(cudaFuncSetAttribute(paged_tc_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem));
+        once.mark();
+    }
+    paged_tc_kernel<DP><<<grid, kThreads, Sh::kSmem, st>>>(a);
+}
+
+}  // namespace
+
+int tc_rows(int D) { return D <= 128 ? 256 : 128; }
+int tc_keys(int D) { return D <= 128 ? 128 : 64; }
+void launch_tc(const Args& a, dim3 grid, cudaStream_t st) {
+    if (a.p.cache.D <= 64) launch<64>(a, grid, st);
+    else if (a.p.cache.D <= 128) launch<128>(a, grid, st);
+    else launch<256>(a, grid, st);
+}
+
+}  // namespace pattn
+}  // namespace sana
