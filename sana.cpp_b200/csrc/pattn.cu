@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(kSThreads) paged_simt_kernel(const __grid_cons
     const Sequence sq = sequence(p, s, blockIdx.x % (a.row_tiles * a.splits) == 0 && kvh == 0 && tid == 0);
     const int rr0 = tile * kSRows;
     if (!sq.ok || rr0 >= sq.n_new * a.G) return;
-    const KeyTiles kt = key_tiles(sq.past, sq.n_new, a.G, rr0, rr0 + kSRows, p.window, p.sinks, kSKeys);
+    const KeyTiles kt = key_tiles(sq.past, sq.n_new, a.G, rr0, rr0 + kSRows, p.window, p.sinks, kSKeys, 1);
     const int t0 = split * a.split_tiles, t1 = min(kt.n, t0 + a.split_tiles);
     if (t0 >= t1) return;
     const bool partial = kt.n > a.split_tiles;
@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
     const Sequence sq = sequence(p, s, blockIdx.x % (a.row_tiles * a.splits) == 0 && kvh == 0 && tid == 0);
     const int rr0 = tile * BM, n_rows = sq.n_new * a.G;
     if (!sq.ok || rr0 >= n_rows) return;
-    const KeyTiles kt = key_tiles(sq.past, sq.n_new, a.G, rr0, rr0 + BM, p.window, p.sinks, BN);
+    const KeyTiles kt = key_tiles(sq.past, sq.n_new, a.G, rr0, rr0 + BM, p.window, p.sinks, BN, 1);
     const int t0 = split * a.split_tiles, n = min(kt.n, t0 + a.split_tiles) - t0;
     if (n <= 0) return;
     const bool partial = kt.n > a.split_tiles;
@@ -481,7 +481,8 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
     const Sequence sq = sequence(p, s, false);
     if (!sq.ok || row < sq.row0) return;
     const int rr = (row - sq.row0) * a.G + h % a.G, tile = rr / a.BM;
-    const KeyTiles kt = key_tiles(sq.past, sq.n_new, a.G, tile * a.BM, (tile + 1) * a.BM, p.window, p.sinks, a.BN);
+    const KeyTiles kt = key_tiles(sq.past, sq.n_new, a.G, tile * a.BM, (tile + 1) * a.BM, p.window, p.sinks, a.BN,
+                                  a.align);
     const int active = (kt.n + a.split_tiles - 1) / a.split_tiles;
     if (active <= 1) return;
     const long long step = static_cast<long long>(p.batch.rows) * p.q_heads;
@@ -530,6 +531,7 @@ Args plan(const PagedAttention& p, Kind kind, int num_sms) {
     a.p = p;
     a.G = p.q_heads / p.cache.kv_heads;
     const long long packed = static_cast<long long>(p.batch.max_new) * a.G;
+    a.align = 1;
     int resident;  // blocks per SM
     if (kind == kSimt) {
         a.BM = kSRows;
@@ -538,6 +540,7 @@ Args plan(const PagedAttention& p, Kind kind, int num_sms) {
     } else if (kind == kTc) {
         a.BM = tc_rows(p.cache.D);
         a.BN = tc_keys(p.cache.D);
+        a.align = std::max(1, tc_box(p.cache));
         resident = 1;
     } else {
         a.BM = packed <= 16 ? 16 : packed <= 32 ? 32 : 64;
@@ -548,7 +551,8 @@ Args plan(const PagedAttention& p, Kind kind, int num_sms) {
     const long long span = p.window > 0 ? std::min<long long>(p.batch.max_kv, static_cast<long long>(p.window) + p.batch.max_new +
                                                                                  p.sinks)
                                         : p.batch.max_kv;
-    const int tiles = ceil_div(span, a.BN) + (p.window > 0 ? 1 : 0);
+    // a window's sinks and its start, rounded down to `align`, may each take part of one tile more
+    const int tiles = ceil_div(span, a.BN) + (p.window > 0 ? (a.align > 1 ? 2 : 1) : 0);
     const long long base = static_cast<long long>(p.batch.S) * p.cache.kv_heads * a.row_tiles;
     // One sequence: one wave of equal blocks. Several: their lengths differ and only the longest is
     // known here, so blocks of a few waves' size even them out.

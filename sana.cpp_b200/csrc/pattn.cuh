@@ -26,6 +26,7 @@ struct Args {
     int row_tiles;    // of BM packed rows, per sequence
     int BM, BN;
     int splits, split_tiles;
+    int align;        // the keys of a window start at a multiple of it (a power of two)
     float* part;      // [splits][rows][q_heads][D]
     float2* ml;       // [splits][rows][q_heads]: (max, sum)
 };
@@ -58,7 +59,7 @@ struct KeyTiles {
     int n_sink, n;    // tiles of the sinks, of both
 };
 __host__ __device__ __forceinline__ KeyTiles key_tiles(int past, int n_new, int G, int rr0, int rr1, int window, int sinks,
-                                                       int BN) {
+                                                       int BN, int align) {
     KeyTiles k;
     const int last = n_new * G < rr1 ? n_new * G : rr1;
     k.pmin = past + rr0 / G;
@@ -67,7 +68,7 @@ __host__ __device__ __forceinline__ KeyTiles key_tiles(int past, int n_new, int 
     k.lo = 0;
     k.sink_end = 0;
     if (window > 0) {
-        const int lo = k.pmin - window + 1;
+        const int lo = (k.pmin - window + 1) & -align;
         const int s = sinks < k.hi ? sinks : k.hi;
         if (lo > s) {
             k.lo = lo;
@@ -111,6 +112,7 @@ __device__ __forceinline__ long long key_offset(const PagedAttention& p, int s, 
 // pattn_tc.cu: packed rows and keys of a block's tile for a head size, and the launch.
 int tc_rows(int D);
 int tc_keys(int D);
+int tc_box(const PagedCache& c);  // keys that one tensor copy brings (0: copies of 16 bytes)
 void launch_tc(const Args& a, dim3 grid, cudaStream_t st);
 
 }  // namespace pattn

@@ -16,10 +16,12 @@
 // almost never after the first tiles. P stays below 2^8, its sum is fp32, its rounding to bf16 is
 // relative, and the division at the end takes the reference out.
 //
-// Keys and values come by 16-byte cp.async from 128 producer threads (pages end anywhere inside a
-// tile; what no row sees is not read but written as zeros), into the 128-byte-swizzled layout of
-// the matrix descriptors: slabs of 64 channels, 128-byte rows, chunk c of row r at c ^ (r & 7). K
-// and Q are K-major operands, V is MN-major (its channels contiguous).
+// Keys and values come into the 128-byte-swizzled layout of the matrix descriptors: slabs of 64
+// channels, 128-byte rows, chunk c of row r at c ^ (r & 7); K and Q are K-major operands, V is
+// MN-major (its channels contiguous). Where pages divide a tile or tiles divide a page, one tensor
+// copy (TMA) per page and slab brings them; other page sizes end anywhere inside a tile and come by
+// 16-byte cp.async. Both by 64 producer threads. Measured on 2048 tokens after 8192 (16 heads of 128
+// over 4): 281 us with cp.async alone, whose issue bound the kernel.
 #include "pattn.cuh"
 #include "tcgen05.cuh"
 #include "tma.h"
@@ -31,7 +33,7 @@ namespace {
 using namespace tc;
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kSoftmaxWarps = 8, kProducerWarps = 4;
+constexpr int kSoftmaxWarps = 8, kProducerWarps = 2;
 constexpr int kThreads = (kSoftmaxWarps + kProducerWarps + 1) * 32;
 constexpr int kMmaWarp = kSoftmaxWarps + kProducerWarps;
 constexpr int kProducers = kProducerWarps * 32;
@@ -45,7 +47,7 @@ struct TcShape {
     static constexpr int kStages = DP == 64 ? 4 : 2;
     static constexpr int kQBytes = kTiles * 128 * DP * 2;
     static constexpr int kTileBytes = kKeys * DP * 2;    // of K or of V
-    static constexpr int kBarriers = 4 * kStages + 6 + 1;
+    static constexpr int kBarriers = 4 * kStages + 8 + 2;
     static constexpr int kSmem = 1024 + kQBytes + kStages * 2 * kTileBytes + 2 * kKeys * 8 + kBarriers * 8 + 64;
     // tensor memory columns: S slots at 0 and kKeys, O behind them
     static constexpr int kO = 2 * kKeys;
@@ -62,7 +64,7 @@ __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
         "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -115,6 +117,10 @@ __device__ __forceinline__ float soft_cap_log2(float x, float in, float out) {
     return fmaf(-2.f * out, rcp_approx(1.f + ex2_approx(x * in)), out);
 }
 
+// One arrival of this thread on `bar` once all its copies so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
 // A bounded wait of a whole warp, with one answer for all its lanes.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* err) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, kTimeout));
@@ -130,8 +136,20 @@ __device__ __forceinline__ bool producers_all(bool ok) {
     return all != 0;
 }
 
+// Bit i: the row at position pos sees key j0 + i, below `end`.
+__device__ __forceinline__ uint32_t low_bits(int n) {  // the n lowest bits, n of any sign and size
+    return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+}
+__device__ __forceinline__ uint32_t seen_bits(int j0, int end, int pos, int window, int sinks) {
+    uint32_t bits = low_bits(pos + 1 - j0);
+    if (window > 0) bits &= ~low_bits(max(pos - window + 1, 0) - j0) | low_bits(sinks - j0);
+    return bits & low_bits(end - j0);
+}
+
 template <int DP>
-__global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_constant__ Args a,
+                                                               const __grid_constant__ CUtensorMap k_map,
+                                                               const __grid_constant__ CUtensorMap v_map, const int box) {
     using Sh = TcShape<DP>;
     constexpr int BN = Sh::kKeys, ST = Sh::kStages;
     extern __shared__ unsigned char smem_raw[];
@@ -142,7 +160,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     const Sequence sq = sequence(p, s, blockIdx.x % (a.row_tiles * a.splits) == 0 && kvh == 0 && tid == 0);
     const int rr0 = tile * Sh::kRows, n_rows = sq.n_new * a.G;
     if (!sq.ok || rr0 >= n_rows) return;
-    const KeyTiles kt = key_tiles(sq.past, sq.n_new, a.G, rr0, rr0 + Sh::kRows, p.window, p.sinks, BN);
+    const KeyTiles kt = key_tiles(sq.past, sq.n_new, a.G, rr0, rr0 + Sh::kRows, p.window, p.sinks, BN, a.align);
     const int t0 = split * a.split_tiles, n = min(kt.n, t0 + a.split_tiles) - t0;
     if (n <= 0) return;
     const bool partial = kt.n > a.split_tiles;
@@ -163,7 +181,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     auto s_full = [&](int i) { return bars + 8u * (4 * ST + i); };
     auto p_full = [&](int i) { return bars + 8u * (4 * ST + 2 + i); };
     auto pv_done = [&](int i) { return bars + 8u * (4 * ST + 4 + i); };
-    const uint32_t drained = bars + 8u * (4 * ST + 6);
+    auto p_half = [&](int i) { return bars + 8u * (4 * ST + 6 + i); };
+    const uint32_t drained = bars + 8u * (4 * ST + 8), v_raw = drained + 8u;
     int* words = reinterpret_cast<int*>(sm + kOffs + 2 * BN * 8 + Sh::kBarriers * 8);  // [0] tensor memory, [1] bad page, [2] not finite
 
     if (warp == kMmaWarp) {
@@ -172,17 +191,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     }
     if (tid == 0) {
         for (int i = 0; i < ST; ++i) {
-            mbar_init(k_full(i), kProducerWarps);
-            mbar_init(v_full(i), kProducerWarps);
+            mbar_init(k_full(i), kProducers);
+            mbar_init(v_full(i), kProducers);
             mbar_init(k_empty(i), 1);
             mbar_init(v_empty(i), 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(s_full(i), 1);
             mbar_init(p_full(i), 4);
+            mbar_init(p_half(i), 4);
             mbar_init(pv_done(i), 1);
         }
         mbar_init(drained, 1);
+        mbar_init(v_raw, kProducers);
         fence_barrier_init();
         words[1] = 0;
         words[2] = 0;
@@ -252,24 +273,31 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 if (!warp_wait(s_full(slot), (u >> 1) & 1, p.err)) break;
                 tc_fence_after();
                 const uint32_t s_t = my_lanes + slot * BN;
-                auto visible = [&](int j) {
-                    return j < end && seen(j, my_pos, p.window, p.sinks) && (!bad_page || key_offset(p, s, j) >= 0);
-                };
-                float mx = -INFINITY;
+                // the whole row in registers: the loads are in flight together
+                uint32_t x[BN];
 #pragma unroll
-                for (int c = 0; c < BN / 32; ++c) {
-                    uint32_t r[32];
-                    tmem_ld32(s_t + c * 32, r);
-                    tmem_wait_ld();
-                    if (whole) {
+                for (int c = 0; c < BN / 32; ++c) tmem_ld32(s_t + c * 32, &x[c * 32]);
+                tmem_wait_ld();
+                if (!whole) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(r[i]));
-                    } else {
+                    for (int c = 0; c < BN / 32; ++c) {
+                        uint32_t bits = seen_bits(start + c * 32, end, my_pos, p.window, p.sinks);
+                        if (bad_page) {
+                            for (int i = 0; i < 32; ++i)
+                                if ((bits >> i & 1u) && key_offset(p, s, start + c * 32 + i) < 0) bits &= ~(1u << i);
+                        }
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
-                            if (visible(start + c * 32 + i)) mx = fmaxf(mx, __uint_as_float(r[i]));
+                            if (!(bits & (1u << i))) x[c * 32 + i] = 0xff800000u;
                     }
                 }
+                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < BN; i += 8)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        mx4[c] = fmaxf(mx4[c], fmaxf(__uint_as_float(x[i + c]), __uint_as_float(x[i + 4 + c])));
+                float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
                 // both maps rise with the score (scale > 0), so the maximum is mapped alone
                 if (mx != -INFINITY) mx = p.softcap > 0.f ? soft_cap_log2(mx, cap_in, cap_out) : mx * scale_log2;
                 const bool move = mx > m + 8.f || (m == -INFINITY && mx > -INFINITY);
@@ -293,36 +321,43 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     }
                 }
                 const float ref = m == -INFINITY ? 0.f : m;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                if (p.softcap > 0.f) {
+#pragma unroll
+                    for (int i = 0; i < BN; ++i) {
+                        const float v = soft_cap_log2(__uint_as_float(x[i]), cap_in, cap_out) - ref;
+                        // the cap maps what is masked to a number: it stays masked
+                        x[i] = x[i] == 0xff800000u ? x[i] : __float_as_uint(v);
+                    }
+                } else {
+                    const uint64_t k2 = f2_make(scale_log2, scale_log2), r2 = f2_make(-ref, -ref);
+#pragma unroll
+                    for (int i = 0; i < BN; i += 2) {
+                        const float2 v = f2_split(fma2(f2_make(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), k2, r2));
+                        x[i] = __float_as_uint(v.x);
+                        x[i + 1] = __float_as_uint(v.y);
+                    }
+                }
+                uint64_t sum[2] = {0, 0};
 #pragma unroll
                 for (int c = 0; c < BN / 32; ++c) {
-                    uint32_t r[32], pk[16];
-                    tmem_ld32(s_t + c * 32, r);
-                    tmem_wait_ld();
-                    if (p.softcap > 0.f) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            r[i] = __float_as_uint(soft_cap_log2(__uint_as_float(r[i]), cap_in, cap_out) - ref);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            r[i] = __float_as_uint(fmaf(__uint_as_float(r[i]), scale_log2, -ref));
-                    }
-                    if (!whole) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (!visible(start + c * 32 + i)) r[i] = 0xff800000u;
-                    }
+                    uint32_t pk[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float x = ex2_approx(__uint_as_float(r[2 * i])), y = ex2_approx(__uint_as_float(r[2 * i + 1]));
-                        sum[(2 * i) & 3] += x;
-                        sum[(2 * i + 1) & 3] += y;
-                        pk[i] = pack_bf2(x, y);
+                        const float e0 = ex2_approx(__uint_as_float(x[c * 32 + 2 * i]));
+                        const float e1 = ex2_approx(__uint_as_float(x[c * 32 + 2 * i + 1]));
+                        sum[i & 1] = add2(sum[i & 1], f2_make(e0, e1));
+                        pk[i] = pack_bf2(e0, e1);
                     }
-                    tmem_st16(s_t + c * 16, pk);  // over scores that this row has read
+                    tmem_st16(s_t + c * 16, pk);  // over the scores, which this row has read
+                    if (c == BN / 64 - 1) {       // the products over the first half of the keys may start
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(p_half(slot));
+                    }
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                const float2 total = f2_split(add2(sum[0], sum[1]));
+                l += total.x + total.y;
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -334,42 +369,46 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         const bf16* kc = static_cast<const bf16*>(p.cache.k) + kvh * p.cache.head_stride;
         const bf16* vc = static_cast<const bf16*>(p.cache.v) + kvh * p.cache.head_stride;
         const int slabs = (D + 63) / 64;
-        auto offset_of = [&](int i) -> long long {
+        // this thread's keys of tile i: pt, pt + 64
+        constexpr int kOwn = BN / kProducers;
+        static_assert(BN % kProducers == 0, "keys per producer");
+        auto offsets = [&](int i, long long (&o)[kOwn]) {
             int start, end;
             key_range(kt, t0 + i, BN, start, end);
-            return start + pt < end ? key_offset(p, s, start + pt) : -1;
+#pragma unroll
+            for (int x = 0; x < kOwn; ++x) {
+                const int j = start + pt + x * kProducers;
+                o[x] = j < end ? key_offset(p, s, j) : -1;
+            }
         };
+        constexpr int kRowsPerPass = kProducers / 8;
         auto chunk_at = [&](int slab, int key) { return slab * (BN * 128) + key * 128 + (((pt & 7) ^ (key & 7)) << 4); };
         auto load = [&](uint32_t dst, const bf16* src, const long long* of) {
             for (int slab = 0; slab < slabs; ++slab) {
                 const int d = slab * 64 + (pt & 7) * 8;
 #pragma unroll
-                for (int x = 0; x < BN / 16; ++x) {
-                    const int key = x * 16 + (pt >> 3);
+                for (int x = 0; x < BN / kRowsPerPass; ++x) {
+                    const int key = x * kRowsPerPass + (pt >> 3);
                     const long long off = of[key];
                     const bool in = off >= 0 && d < D;
                     cp_async16(dst + chunk_at(slab, key), in ? src + off + d : src, in);
                 }
             }
-            cp_async_commit();
-        };
-        auto publish = [&](uint32_t bar) {  // this warp's part of a tile has landed
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar);
         };
         // Values that are not finite, in a tile that not every row sees whole, would reach the rows that do
         // not see them as 0 * v: zeros take their place, and the rows that see them get them at the end.
-        auto clean = [&](int i) {
-            int start, end;
-            key_range(kt, t0 + i, BN, start, end);
-            if (all_seen(kt, start, end, p.window, p.sinks)) return;
-            unsigned char* v = sm + Sh::kQBytes + (i % ST) * (2 * Sh::kTileBytes) + Sh::kTileBytes;
+        // Keys from `keys` on, and those of bad pages, are zeros outright (a tensor copy brought what lies there).
+        auto clean = [&](unsigned char* v, int start, int keys) {
             for (int slab = 0; slab < slabs; ++slab) {
-#pragma unroll
-                for (int x = 0; x < BN / 16; ++x) {
-                    uint4* w = reinterpret_cast<uint4*>(v + chunk_at(slab, x * 16 + (pt >> 3)));
-                    uint4 c = *w;
+#pragma unroll 4
+                for (int x = 0; x < BN / kRowsPerPass; ++x) {
+                    const int key = x * kRowsPerPass + (pt >> 3);
+                    uint4* w = reinterpret_cast<uint4*>(v + chunk_at(slab, key));
+                    if (key >= keys || (bad_page && key_offset(p, s, start + key) < 0)) {
+                        *w = make_uint4(0, 0, 0, 0);
+                        continue;
+                    }
+                    const uint4 c = *w;
                     uint32_t e[4] = {c.x, c.y, c.z, c.w};
                     bool bad = false;
 #pragma unroll
@@ -384,48 +423,117 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 }
             }
         };
-        long long next = pt < BN ? offset_of(0) : -1;
         bool ok = true;
-        for (int i = 0; i < n; ++i) {
-            const int st = i % ST, use = i / ST;
-            long long* of = offs + (i & 1) * BN;
-            if (pt < BN) of[pt] = next;
-            ok = producers_all(ok);  // after a failed wait the warps leave together
-            if (!ok) break;
-            next = pt < BN && i + 1 < n ? offset_of(i + 1) : -1;
-            const uint32_t ks = kv_s + st * (2 * Sh::kTileBytes);
-            ok = warp_wait(k_empty(st), (use & 1) ^ 1, p.err);
-            if (ok) load(ks, kc, of);
-            else cp_async_commit();
-            if (i > 0) {
-                cp_async_wait<1>();
-                clean(i - 1);
-                publish(v_full((i - 1) % ST));
+        if (box > 0) {
+            // Producer thread b < BN / box copies box b of a tile, `box` keys of one page. Every producer arrives once
+            // on a tile's barrier, those that copy with the bytes to come.
+            const int boxes = BN / box;
+            const uint32_t bytes = static_cast<uint32_t>(box) * 128 * slabs;
+            int issued = 0, raw = 0;
+            bool in_flight = false;  // on v_raw
+            for (int i = 0; i < n; ++i) {
+                const int st = i % ST, use = i / ST;
+                int start, end;
+                key_range(kt, t0 + i, BN, start, end);
+                const int key = start + pt * box;
+                int page = -1, at = 0;
+                if (pt < boxes && key < end) {
+                    const int slot = key / p.cache.page_size;
+                    page = slot < p.batch.table_width ? p.batch.table[s * p.batch.table_stride + slot] : -1;
+                    if (page >= p.cache.pages) page = -1;
+                    at = key - slot * p.cache.page_size;
+                }
+                auto copy = [&](const CUtensorMap* map, uint32_t dst, uint32_t bar) {
+                    if (page < 0) {
+                        mbar_arrive(bar);
+                        return;
+                    }
+                    mbar_arrive_expect_tx(bar, bytes);
+                    for (int slab = 0; slab < slabs; ++slab)
+                        tma_load_4d(map, dst + slab * (BN * 128) + pt * box * 128, bar, slab * 64, at, kvh, page);
+                };
+                const uint32_t ks = kv_s + st * (2 * Sh::kTileBytes);
+                ok = warp_wait(k_empty(st), (use & 1) ^ 1, p.err);
+                if (!ok) break;
+                copy(&k_map, ks, k_full(st));
+                issued = i + 1;
+                ok = warp_wait(v_empty(st), (use & 1) ^ 1, p.err);
+                if (!ok) break;
+                if (end - start == BN && !bad_page && all_seen(kt, start, end, p.window, p.sinks)) {
+                    copy(&v_map, ks + Sh::kTileBytes, v_full(st));
+                    continue;
+                }
+                copy(&v_map, ks + Sh::kTileBytes, v_raw);
+                in_flight = true;
+                ok = warp_wait(v_raw, raw & 1, p.err);
+                if (!ok) break;
+                in_flight = false;
+                ++raw;
+                clean(sm + Sh::kQBytes + st * (2 * Sh::kTileBytes) + Sh::kTileBytes, start, end - start);
+                fence_proxy_async_smem();
+                mbar_arrive(v_full(st));
             }
-            ok = ok && warp_wait(v_empty(st), (use & 1) ^ 1, p.err);
-            if (ok) load(ks + Sh::kTileBytes, vc, of);
-            else cp_async_commit();
-            cp_async_wait<1>();
-            if (ok) publish(k_full(st));
-        }
-        cp_async_wait<0>();
-        if (ok) {
-            clean(n - 1);
-            publish(v_full((n - 1) % ST));
+            if (!ok) {  // what is on its way lands (or is waited for as long as a wait may last) before the block ends
+                if (in_flight) mbar_wait_quiet(v_raw, raw & 1);
+                for (int i = issued > ST ? issued - ST : 0; i < issued; ++i) {
+                    mbar_wait_quiet(k_full(i % ST), (i / ST) & 1);
+                    if (i + 1 < issued) mbar_wait_quiet(v_full(i % ST), (i / ST) & 1);
+                }
+            }
+        } else {
+            long long next[kOwn];
+            offsets(0, next);
+            for (int i = 0; i < n; ++i) {
+                const int st = i % ST, use = i / ST;
+                long long* of = offs + (i & 1) * BN;
+    #pragma unroll
+                for (int x = 0; x < kOwn; ++x) of[pt + x * kProducers] = next[x];
+                ok = producers_all(ok);  // after a failed wait the warps leave together
+                if (!ok) break;
+                if (i + 1 < n) offsets(i + 1, next);
+                const uint32_t ks = kv_s + st * (2 * Sh::kTileBytes);
+                ok = warp_wait(k_empty(st), (use & 1) ^ 1, p.err);
+                if (!ok) continue;
+                load(ks, kc, of);
+                cp_async_arrive(k_full(st));
+                ok = warp_wait(v_empty(st), (use & 1) ^ 1, p.err);
+                if (!ok) continue;
+                load(ks + Sh::kTileBytes, vc, of);
+                int start, end;
+                key_range(kt, t0 + i, BN, start, end);
+                if (all_seen(kt, start, end, p.window, p.sinks)) {
+                    cp_async_arrive(v_full(st));
+                } else {
+                    cp_async_commit();
+                    cp_async_wait<0>();
+                    clean(sm + Sh::kQBytes + st * (2 * Sh::kTileBytes) + Sh::kTileBytes, start, end - start);
+                    mbar_arrive(v_full(st));
+                }
+            }
+            cp_async_commit();
+            cp_async_wait<0>();
         }
     } else if (lane == 0) {
         const int d16 = (D + 15) & ~15;
         const uint32_t idesc_s = idesc_bf16_f32(128, BN);
         const uint32_t idesc_o = idesc_bf16_f32(128, d16) | kBTransposed;
+        // descriptors of the first operands; the others differ in the address field alone (16-byte units)
+        const uint64_t q_desc = kmajor_sw128_desc(q_s), k_desc = kmajor_sw128_desc(kv_s);
+        const uint64_t v_desc = mnmajor_sw128_desc(kv_s + Sh::kTileBytes, BN * 128);
         auto scores = [&](int u) -> bool {
             const int slot = u & 1, kv = pair ? u >> 1 : u, t = pair ? u & 1 : 0, st = kv % ST;
             if (!mbar_wait(k_full(st), (kv / ST) & 1, p.err, kTimeout)) return false;
+            // cp.async writes through the generic proxy, the products read through the async one: ordered here, by
+            // the thread that has seen the copies land
+            if (box == 0) fence_proxy_async_smem();
             tc_fence_after();
-            const uint32_t qa = q_s + t * (128 * DP * 2), ka = kv_s + st * (2 * Sh::kTileBytes);
-            for (int k = 0; k < d16 / 16; ++k) {
-                const uint32_t in = (k & 3) * 32;
-                umma_bf16(tmem + slot * BN, kmajor_sw128_desc(qa + (k >> 2) * (128 * 128) + in),
-                          kmajor_sw128_desc(ka + (k >> 2) * (BN * 128) + in), idesc_s, k > 0);
+            const uint64_t qd = q_desc + static_cast<uint64_t>(t * (128 * DP * 2) >> 4);
+            const uint64_t kd = k_desc + static_cast<uint64_t>(st * (2 * Sh::kTileBytes) >> 4);
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+                if (k * 16 < D)
+                    umma_bf16(tmem + slot * BN, qd + (((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4),
+                              kd + (((k >> 2) * (BN * 128) + (k & 3) * 32) >> 4), idesc_s, k > 0);
             }
             umma_commit(s_full(slot));
             if (!pair || t == 1) umma_commit(k_empty(st));
@@ -434,14 +542,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         bool ok = scores(0) && (units < 2 || scores(1));
         for (int u = 0; u < units && ok; ++u) {
             const int slot = u & 1, kv = pair ? u >> 1 : u, t = pair ? u & 1 : 0, st = kv % ST;
-            ok = mbar_wait(v_full(st), (kv / ST) & 1, p.err, kTimeout) && mbar_wait(p_full(slot), (u >> 1) & 1, p.err, kTimeout);
+            const uint64_t vd = v_desc + static_cast<uint64_t>(st * (2 * Sh::kTileBytes) >> 4);
+            ok = mbar_wait(v_full(st), (kv / ST) & 1, p.err, kTimeout) && mbar_wait(p_half(slot), (u >> 1) & 1, p.err, kTimeout);
+            if (!ok) break;
+            if (box == 0) fence_proxy_async_smem();
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < BN / 32; ++k)
+                umma_bf16_ta(tmem + Sh::kO + t * DP, tmem + slot * BN + k * 8, vd + (k * 2048 >> 4), idesc_o, kv > 0 || k > 0);
+            ok = mbar_wait(p_full(slot), (u >> 1) & 1, p.err, kTimeout);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t va = kv_s + st * (2 * Sh::kTileBytes) + Sh::kTileBytes;
 #pragma unroll
-            for (int k = 0; k < BN / 16; ++k)
-                umma_bf16_ta(tmem + Sh::kO + t * DP, tmem + slot * BN + k * 8, mnmajor_sw128_desc(va + k * 2048, BN * 128),
-                             idesc_o, kv > 0 || k > 0);
+            for (int k = BN / 32; k < BN / 16; ++k)
+                umma_bf16_ta(tmem + Sh::kO + t * DP, tmem + slot * BN + k * 8, vd + (k * 2048 >> 4), idesc_o, 1);
             umma_commit(pv_done(slot));
             if (!pair || t == 1) umma_commit(v_empty(st));
             if (u + 2 < units) ok = scores(u + 2);
@@ -511,6 +625,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
 }
 
+// The pool as a tensor [pages][kv_heads][page_size][D], boxes of `box` tokens of one head x 64 channels.
+CUtensorMap pool_map(const PagedCache& c, const void* base, int box) {
+    CUtensorMap m;
+    auto stride = [](long long elements) { return static_cast<cuuint64_t>(elements > 8 ? elements * 2 : 16); };
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.D), static_cast<cuuint64_t>(c.page_size),
+                                static_cast<cuuint64_t>(c.kv_heads), static_cast<cuuint64_t>(c.pages)};
+    const cuuint64_t strides[3] = {stride(c.token_stride), stride(c.head_stride), stride(c.page_stride)};
+    const cuuint32_t b[4] = {64, static_cast<cuuint32_t>(box), 1, 1};
+    tma_encode_tiled(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides, b, CU_TENSOR_MAP_SWIZZLE_128B);
+    return m;
+}
+
 template <int DP>
 void launch(const Args& a, dim3 grid, cudaStream_t st) {
     static PerDeviceOnce once;
@@ -520,13 +646,31 @@ void launch(const Args& a, dim3 grid, cudaStream_t st) {
         SANA_CUDA(cudaFuncSetAttribute(paged_tc_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem));
         once.mark();
     }
-    paged_tc_kernel<DP><<<grid, kThreads, Sh::kSmem, st>>>(a);
+    const int box = tc_box(a.p.cache);
+    CUtensorMap k{}, v{};
+    if (box > 0) {
+        k = pool_map(a.p.cache, a.p.cache.k, box);
+        v = pool_map(a.p.cache, a.p.cache.v, box);
+    }
+    paged_tc_kernel<DP><<<grid, kThreads, Sh::kSmem, st>>>(a, k, v, box);
 }
 
 }  // namespace
 
 int tc_rows(int D) { return D <= 128 ? 256 : 128; }
 int tc_keys(int D) { return D <= 128 ? 128 : 64; }
+// A box is a page, or a key tile where pages are multiples of tiles; whole groups of eight rows, which the
+// swizzle needs. The strides of a tensor map end at 2^40 bytes; a stride of 0 (or of a size 1) is not encoded.
+int tc_box(const PagedCache& c) {
+    const int keys = tc_keys(c.D);
+    const long long most = 1LL << 38;
+    const bool strides_ok = c.page_stride < most && c.token_stride < most && c.head_stride < most &&
+                            (c.page_stride >= 8 || c.pages == 1) && (c.token_stride >= 8 || c.page_size == 1) &&
+                            (c.head_stride >= 8 || c.kv_heads == 1);
+    if (!strides_ok || c.pages < 1) return 0;
+    if (c.page_size % keys == 0) return keys;
+    return c.page_size % 8 == 0 && keys % c.page_size == 0 ? c.page_size : 0;
+}
 void launch_tc(const Args& a, dim3 grid, cudaStream_t st) {
     if (a.p.cache.D <= 64) launch<64>(a, grid, st);
     else if (a.p.cache.D <= 128) launch<128>(a, grid, st);
