@@ -22,6 +22,8 @@
 // copy (TMA) per page and slab brings them; other page sizes end anywhere inside a tile and come by
 // 16-byte cp.async. Both by 64 producer threads. Measured on 2048 tokens after 8192 (16 heads of 128
 // over 4): 281 us with cp.async alone, whose issue bound the kernel.
+#include <type_traits>
+
 #include "pattn.cuh"
 #include "tcgen05.cuh"
 #include "tma.h"
@@ -117,6 +119,11 @@ __device__ __forceinline__ float soft_cap_log2(float x, float in, float out) {
     return fmaf(-2.f * out, rcp_approx(1.f + ex2_approx(x * in)), out);
 }
 
+__device__ __forceinline__ bool elect_one() {
+    uint32_t on;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(on));
+    return on != 0;
+}
 // One arrival of this thread on `bar` once all its copies so far have landed.
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
@@ -146,12 +153,18 @@ __device__ __forceinline__ uint32_t seen_bits(int j0, int end, int pos, int wind
     return bits & low_bits(end - j0);
 }
 
-template <int DP>
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+template <int DP, bool CAP>
 __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_constant__ Args a,
                                                                const __grid_constant__ CUtensorMap k_map,
                                                                const __grid_constant__ CUtensorMap v_map, const int box) {
     using Sh = TcShape<DP>;
     constexpr int BN = Sh::kKeys, ST = Sh::kStages;
+    constexpr int kEarly = BN == 128 ? 3 : 1;  // quarters (halves) of a tile's P handed over before the rest
     extern __shared__ unsigned char smem_raw[];
     const PagedAttention& p = a.p;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = p.cache.D;
@@ -257,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     if (warp < kSoftmaxWarps) {
         if (softmax_on) {
             const float scale_log2 = p.scale * kLog2e;
-            const float cap_in = p.softcap > 0.f ? 2.f * scale_log2 / p.softcap : 0.f, cap_out = p.softcap * kLog2e;
+            const float cap_in = CAP ? 2.f * scale_log2 / p.softcap : 0.f, cap_out = p.softcap * kLog2e;
             // positions of this row tile
             const int last = min(n_rows, rr0 + wg * 128 + 128) - 1;
             KeyTiles mine = kt;
@@ -291,15 +304,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                             if (!(bits & (1u << i))) x[c * 32 + i] = 0xff800000u;
                     }
                 }
-                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                float mx4[4];
 #pragma unroll
-                for (int i = 0; i < BN; i += 8)
+                for (int c = 0; c < 4; ++c) mx4[c] = __uint_as_float(x[c]);
+#pragma unroll
+                for (int i = 4; i + 8 <= BN; i += 8)
 #pragma unroll
                     for (int c = 0; c < 4; ++c)
-                        mx4[c] = fmaxf(mx4[c], fmaxf(__uint_as_float(x[i + c]), __uint_as_float(x[i + 4 + c])));
-                float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+                        mx4[c] = max3(mx4[c], __uint_as_float(x[i + c]), __uint_as_float(x[i + 4 + c]));
+                float mx = max3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3]));
+                mx = max3(mx, fmaxf(__uint_as_float(x[BN - 1]), __uint_as_float(x[BN - 2])),
+                          fmaxf(__uint_as_float(x[BN - 3]), __uint_as_float(x[BN - 4])));
                 // both maps rise with the score (scale > 0), so the maximum is mapped alone
-                if (mx != -INFINITY) mx = p.softcap > 0.f ? soft_cap_log2(mx, cap_in, cap_out) : mx * scale_log2;
+                if (mx != -INFINITY) mx = CAP ? soft_cap_log2(mx, cap_in, cap_out) : mx * scale_log2;
                 const bool move = mx > m + 8.f || (m == -INFINITY && mx > -INFINITY);
                 float alpha = 1.f;
                 if (move) {
@@ -321,39 +338,35 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     }
                 }
                 const float ref = m == -INFINITY ? 0.f : m;
-                if (p.softcap > 0.f) {
-#pragma unroll
-                    for (int i = 0; i < BN; ++i) {
-                        const float v = soft_cap_log2(__uint_as_float(x[i]), cap_in, cap_out) - ref;
-                        // the cap maps what is masked to a number: it stays masked
-                        x[i] = x[i] == 0xff800000u ? x[i] : __float_as_uint(v);
-                    }
-                } else {
+                uint64_t sum[2] = {0, 0};
+                {
                     const uint64_t k2 = f2_make(scale_log2, scale_log2), r2 = f2_make(-ref, -ref);
 #pragma unroll
-                    for (int i = 0; i < BN; i += 2) {
-                        const float2 v = f2_split(fma2(f2_make(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), k2, r2));
-                        x[i] = __float_as_uint(v.x);
-                        x[i + 1] = __float_as_uint(v.y);
-                    }
-                }
-                uint64_t sum[2] = {0, 0};
+                    for (int c = 0; c < BN / 32; ++c) {
+                        uint32_t pk[16];
 #pragma unroll
-                for (int c = 0; c < BN / 32; ++c) {
-                    uint32_t pk[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float e0 = ex2_approx(__uint_as_float(x[c * 32 + 2 * i]));
-                        const float e1 = ex2_approx(__uint_as_float(x[c * 32 + 2 * i + 1]));
-                        sum[i & 1] = add2(sum[i & 1], f2_make(e0, e1));
-                        pk[i] = pack_bf2(e0, e1);
-                    }
-                    tmem_st16(s_t + c * 16, pk);  // over the scores, which this row has read
-                    if (c == BN / 64 - 1) {       // the products over the first half of the keys may start
-                        tmem_wait_st();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(p_half(slot));
+                        for (int i = 0; i < 16; ++i) {
+                            const float x0 = __uint_as_float(x[c * 32 + 2 * i]), x1 = __uint_as_float(x[c * 32 + 2 * i + 1]);
+                            uint64_t e;
+                            if constexpr (CAP) {
+                                e = add2(f2_make(soft_cap_log2(x0, cap_in, cap_out), soft_cap_log2(x1, cap_in, cap_out)), r2);
+                                const float2 v = f2_split(e);  // the cap maps what is masked to a number: it stays masked
+                                if (!whole) e = f2_make(x0 == -INFINITY ? x0 : v.x, x1 == -INFINITY ? x1 : v.y);
+                            } else {
+                                e = fma2(f2_make(x0, x1), k2, r2);
+                            }
+                            const float2 v = f2_split(e);
+                            const float e0 = ex2_approx(v.x), e1 = ex2_approx(v.y);
+                            sum[i & 1] = add2(sum[i & 1], f2_make(e0, e1));
+                            pk[i] = pack_bf2(e0, e1);
+                        }
+                        tmem_st16(s_t + c * 16, pk);  // over the scores, which this row has read
+                        if (c == kEarly - 1) {        // the products over these keys may start
+                            tmem_wait_st();
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(p_half(slot));
+                        }
                     }
                 }
                 const float2 total = f2_split(add2(sum[0], sum[1]));
@@ -513,54 +526,80 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             cp_async_commit();
             cp_async_wait<0>();
         }
-    } else if (lane == 0) {
-        const int d16 = (D + 15) & ~15;
+    } else {
+        // The whole warp walks the units, so that all it computes is uniform; one elected thread issues.
+        const int d16 = (D + 15) & ~15, k_steps = d16 / 16;
+        const uint32_t t_mem = __shfl_sync(0xffffffffu, tmem, 0);
         const uint32_t idesc_s = idesc_bf16_f32(128, BN);
         const uint32_t idesc_o = idesc_bf16_f32(128, d16) | kBTransposed;
         // descriptors of the first operands; the others differ in the address field alone (16-byte units)
         const uint64_t q_desc = kmajor_sw128_desc(q_s), k_desc = kmajor_sw128_desc(kv_s);
         const uint64_t v_desc = mnmajor_sw128_desc(kv_s + Sh::kTileBytes, BN * 128);
-        auto scores = [&](int u) -> bool {
-            const int slot = u & 1, kv = pair ? u >> 1 : u, t = pair ? u & 1 : 0, st = kv % ST;
-            if (!mbar_wait(k_full(st), (kv / ST) & 1, p.err, kTimeout)) return false;
-            // cp.async writes through the generic proxy, the products read through the async one: ordered here, by
-            // the thread that has seen the copies land
-            if (box == 0) fence_proxy_async_smem();
-            tc_fence_after();
-            const uint64_t qd = q_desc + static_cast<uint64_t>(t * (128 * DP * 2) >> 4);
-            const uint64_t kd = k_desc + static_cast<uint64_t>(st * (2 * Sh::kTileBytes) >> 4);
+        const bool leader = elect_one();
+        auto walk = [&](auto two) {
+            constexpr bool kPair = decltype(two)::value;
+            auto scores = [&](int u, int slot) -> bool {
+                const int kv = kPair ? u >> 1 : u, t = kPair ? slot : 0, st = kv % ST;
+                if (!warp_wait(k_full(st), (kv / ST) & 1, p.err)) return false;
+                // cp.async writes through the generic proxy, the products read through the async one: ordered here, by
+                // the threads that have seen the copies land
+                if (box == 0) fence_proxy_async_smem();
+                tc_fence_after();
+                const uint64_t qd = q_desc + static_cast<uint64_t>(t * (128 * DP * 2) >> 4);
+                const uint64_t kd = k_desc + static_cast<uint64_t>(st * (2 * Sh::kTileBytes) >> 4);
+                if (leader) {
+                    auto step = [&](int k) {
+                        umma_bf16(t_mem + slot * BN, qd + (((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4),
+                                  kd + (((k >> 2) * (BN * 128) + (k & 3) * 32) >> 4), idesc_s, k > 0);
+                    };
+                    if (k_steps == DP / 16) {
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k) {
-                if (k * 16 < D)
-                    umma_bf16(tmem + slot * BN, qd + (((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4),
-                              kd + (((k >> 2) * (BN * 128) + (k & 3) * 32) >> 4), idesc_s, k > 0);
+                        for (int k = 0; k < DP / 16; ++k) step(k);
+                    } else {
+                        for (int k = 0; k < k_steps; ++k) step(k);
+                    }
+                    umma_commit(s_full(slot));
+                    if (!kPair || t == 1) umma_commit(k_empty(st));
+                }
+                __syncwarp();
+                return true;
+            };
+            auto values = [&](int u, int slot) -> bool {
+                const int kv = kPair ? u >> 1 : u, t = kPair ? slot : 0, st = kv % ST;
+                const uint64_t vd = v_desc + static_cast<uint64_t>(st * (2 * Sh::kTileBytes) >> 4);
+                const uint32_t o = t_mem + Sh::kO + t * DP, pa = t_mem + slot * BN;
+                if (!kPair || t == 0) {  // the second row tile's products read what the first one's have waited for
+                    if (!warp_wait(v_full(st), (kv / ST) & 1, p.err)) return false;
+                    if (box == 0) fence_proxy_async_smem();
+                }
+                if (!warp_wait(p_half(slot), (u >> 1) & 1, p.err)) return false;
+                tc_fence_after();
+                if (leader) {
+#pragma unroll
+                    for (int k = 0; k < 2 * kEarly; ++k) umma_bf16_ta(o, pa + k * 8, vd + (k * 2048 >> 4), idesc_o, k > 0 || kv > 0);
+                }
+                __syncwarp();
+                if (!warp_wait(p_full(slot), (u >> 1) & 1, p.err)) return false;
+                tc_fence_after();
+                if (leader) {
+#pragma unroll
+                    for (int k = 2 * kEarly; k < BN / 16; ++k) umma_bf16_ta(o, pa + k * 8, vd + (k * 2048 >> 4), idesc_o, 1);
+                    umma_commit(pv_done(slot));
+                    if (!kPair || t == 1) umma_commit(v_empty(st));
+                }
+                __syncwarp();
+                return true;
+            };
+            bool ok = scores(0, 0) && (units < 2 || scores(1, 1));
+            for (int u = 0; u < units && ok; u += 2) {
+                ok = values(u, 0) && (u + 2 >= units || scores(u + 2, 0));
+                if (ok && u + 1 < units) ok = values(u + 1, 1) && (u + 3 >= units || scores(u + 3, 1));
             }
-            umma_commit(s_full(slot));
-            if (!pair || t == 1) umma_commit(k_empty(st));
-            return true;
         };
-        bool ok = scores(0) && (units < 2 || scores(1));
-        for (int u = 0; u < units && ok; ++u) {
-            const int slot = u & 1, kv = pair ? u >> 1 : u, t = pair ? u & 1 : 0, st = kv % ST;
-            const uint64_t vd = v_desc + static_cast<uint64_t>(st * (2 * Sh::kTileBytes) >> 4);
-            ok = mbar_wait(v_full(st), (kv / ST) & 1, p.err, kTimeout) && mbar_wait(p_half(slot), (u >> 1) & 1, p.err, kTimeout);
-            if (!ok) break;
-            if (box == 0) fence_proxy_async_smem();
-            tc_fence_after();
-#pragma unroll
-            for (int k = 0; k < BN / 32; ++k)
-                umma_bf16_ta(tmem + Sh::kO + t * DP, tmem + slot * BN + k * 8, vd + (k * 2048 >> 4), idesc_o, kv > 0 || k > 0);
-            ok = mbar_wait(p_full(slot), (u >> 1) & 1, p.err, kTimeout);
-            if (!ok) break;
-            tc_fence_after();
-#pragma unroll
-            for (int k = BN / 32; k < BN / 16; ++k)
-                umma_bf16_ta(tmem + Sh::kO + t * DP, tmem + slot * BN + k * 8, vd + (k * 2048 >> 4), idesc_o, 1);
-            umma_commit(pv_done(slot));
-            if (!pair || t == 1) umma_commit(v_empty(st));
-            if (u + 2 < units) ok = scores(u + 2);
-        }
-        umma_commit(drained);  // whatever was issued has run before the tensor memory is given back
+        if (Sh::kTiles == 2 && pair) walk(std::true_type{});
+        else walk(std::false_type{});
+        if (leader) umma_commit(drained);  // whatever was issued has run before the tensor memory is given back
+        __syncwarp();
         mbar_wait_quiet(drained, 0);
     }
     __syncwarp();
@@ -637,13 +676,13 @@ CUtensorMap pool_map(const PagedCache& c, const void* base, int box) {
     return m;
 }
 
-template <int DP>
+template <int DP, bool CAP>
 void launch(const Args& a, dim3 grid, cudaStream_t st) {
     static PerDeviceOnce once;
     using Sh = TcShape<DP>;
     static_assert(Sh::kSmem <= 232448, "shared memory of one block");
     if (once.pending()) {
-        SANA_CUDA(cudaFuncSetAttribute(paged_tc_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem));
+        SANA_CUDA(cudaFuncSetAttribute(paged_tc_kernel<DP, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem));
         once.mark();
     }
     const int box = tc_box(a.p.cache);
@@ -652,7 +691,7 @@ void launch(const Args& a, dim3 grid, cudaStream_t st) {
         k = pool_map(a.p.cache, a.p.cache.k, box);
         v = pool_map(a.p.cache, a.p.cache.v, box);
     }
-    paged_tc_kernel<DP><<<grid, kThreads, Sh::kSmem, st>>>(a, k, v, box);
+    paged_tc_kernel<DP, CAP><<<grid, kThreads, Sh::kSmem, st>>>(a, k, v, box);
 }
 
 }  // namespace
@@ -672,9 +711,10 @@ int tc_box(const PagedCache& c) {
     return c.page_size % 8 == 0 && keys % c.page_size == 0 ? c.page_size : 0;
 }
 void launch_tc(const Args& a, dim3 grid, cudaStream_t st) {
-    if (a.p.cache.D <= 64) launch<64>(a, grid, st);
-    else if (a.p.cache.D <= 128) launch<128>(a, grid, st);
-    else launch<256>(a, grid, st);
+    const bool cap = a.p.softcap > 0.f;
+    if (a.p.cache.D <= 64) cap ? launch<64, true>(a, grid, st) : launch<64, false>(a, grid, st);
+    else if (a.p.cache.D <= 128) cap ? launch<128, true>(a, grid, st) : launch<128, false>(a, grid, st);
+    else cap ? launch<256, true>(a, grid, st) : launch<256, false>(a, grid, st);
 }
 
 }  // namespace pattn
