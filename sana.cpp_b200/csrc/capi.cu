@@ -1704,7 +1704,7 @@ sana::PagedAttention paged_attention_of(const sana_paged_batch* batch, const san
     p.batch = paged_batch_of(batch);
     p.cache = paged_cache_of(cache);
     SANA_REQUIRE(p.cache.D <= 256, "head_dim must be at most 256");
-    SANA_REQUIRE(p.cache.kv_heads <= 65535, "too many cache heads");
+    SANA_REQUIRE(q_heads <= 65535, "too many heads");
     SANA_REQUIRE(q_heads >= 1 && q_heads % p.cache.kv_heads == 0, "q_heads must be a multiple of kv_heads");
     SANA_REQUIRE(window >= 0 && sinks >= 0, "window and sinks must not be negative");
     SANA_REQUIRE(static_cast<long long>(p.batch.max_new) * (q_heads / p.cache.kv_heads) <= 0x3fffffffLL &&

@@ -9,6 +9,7 @@
 #include <cmath>
 
 #include "pattn.cuh"
+#include "tma.h"
 
 namespace sana {
 namespace pattn {
@@ -35,6 +36,7 @@ __global__ void __launch_bounds__(kSThreads) paged_simt_kernel(const __grid_cons
     float* Vs = Ks + kSKeys * ld;
     const int tile = a.row_tiles - 1 - static_cast<int>(blockIdx.x % a.row_tiles);
     const int rest = blockIdx.x / a.row_tiles, split = rest % a.splits, s = rest / a.splits, kvh = blockIdx.y;
+    cudaTriggerProgrammaticLaunchCompletion();  // the join's blocks may take their places
     const Sequence sq = sequence(p, s, blockIdx.x % (a.row_tiles * a.splits) == 0 && kvh == 0 && tid == 0);
     const int rr0 = tile * kSRows;
     if (!sq.ok || rr0 >= sq.n_new * a.G) return;
@@ -198,81 +200,163 @@ __device__ __forceinline__ float soft_cap_log2(float x, float two_log2e_over_cap
     return fmaf(-2.f * cap_log2e, rcp_approx(1.f + ex2_approx(x * two_log2e_over_cap)), cap_log2e);
 }
 
-// DP: padded head size. WM warps share out the rows (16 each), 4 / WM warps each step's 64 keys:
-// a single token's few rows keep all four warps busy on different keys, and every warp runs its
-// own softmax; the warps' results are joined once at the end. Keys and values come by 16-byte
-// cp.async, ST tiles deep, into rows whose 16-byte chunks are swapped by the row number (c ^ (r &
-// 7)) so that ldmatrix meets no bank twice; the page lookups run ST tiles ahead of the loads. P is
-// rounded to bf16 for the second product, its sum is not.
+// DP: padded head size. Groups of WM warps (16 rows each) share out each step's 64 keys, 4 / WM
+// groups: a single token's few rows keep all four warps busy on different keys. Every group runs
+// on its own: it brings its keys and values into its own ring of ST tiles, waits for them alone
+// (no block barrier in the loop), and every warp has its own softmax; the groups' results are
+// joined once at the end. P is rounded to bf16 for the second product, its sum is not.
+//
+// Keys and values sit in slabs of 64 channels, rows of 128 bytes whose 16-byte chunks are swapped
+// by the row number (c ^ (r & 7)), so that ldmatrix meets no bank twice. TMA: a page's keys come by
+// one tensor copy per slab, which lays them out so. Otherwise (pages that end inside a group's
+// keys) by 16-byte cp.async; the page lookups run a tile ahead of the loads.
+// What bounds a decoding step is HBM, and short of it the latency of the loop's instructions.
 template <int DP>
 struct MmaShape {
     static constexpr int kKeys = 64;
     static constexpr int kStages = DP == 64 ? 4 : 3;
     static constexpr int kTileBytes = kKeys * DP * 2;
-    static constexpr int smem(int rows) {
-        return rows * DP * 2 + kStages * 2 * kTileBytes + (kStages + 1) * kKeys * 8;
+    // behind the tiles: the keys' offsets (cp.async; [kStages + 1][kKeys]) or the copies' barriers (TMA), and in the
+    // end the statistics of up to 64 rows
+    static __host__ __device__ constexpr int tail(bool tma) { return tma ? 512 + 4 * kStages * 8 : (kStages + 1) * kKeys * 8; }
+    static __host__ __device__ constexpr int align(bool tma) { return tma ? 1024 : 128; }  // tensor copies: the swizzle's period
+    static __host__ __device__ constexpr int smem(int rows, bool tma) {
+        return align(tma) + rows * DP * 2 + kStages * 2 * kTileBytes + tail(tma);
     }
 };
 
-template <int DP, int WM>
-__global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ Args a) {
+template <int DP, int WM, bool TMA>
+__global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ Args a,
+                                                        const __grid_constant__ CUtensorMap k_map,
+                                                        const __grid_constant__ CUtensorMap v_map, const int box) {
     using Sh = MmaShape<DP>;
-    constexpr int BN = Sh::kKeys, ST = Sh::kStages, BM = 16 * WM, WK = 4 / WM, NT = BN / WK / 8, CH = DP / 8;
-    extern __shared__ __align__(128) unsigned char smem[];
+    constexpr int BN = Sh::kKeys, ST = Sh::kStages, BM = 16 * WM, WK = 4 / WM, GK = BN / WK, NT = GK / 8;
+    extern __shared__ unsigned char smem_raw[];
     const PagedAttention& p = a.p;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wm = warp % WM, wk = warp / WM, D = p.cache.D;
     const int tile = a.row_tiles - 1 - static_cast<int>(blockIdx.x % a.row_tiles);
     const int rest = blockIdx.x / a.row_tiles, split = rest % a.splits, s = rest / a.splits, kvh = blockIdx.y;
+    cudaTriggerProgrammaticLaunchCompletion();  // the join's blocks may take their places
     const Sequence sq = sequence(p, s, blockIdx.x % (a.row_tiles * a.splits) == 0 && kvh == 0 && tid == 0);
     const int rr0 = tile * BM, n_rows = sq.n_new * a.G;
     if (!sq.ok || rr0 >= n_rows) return;
-    const KeyTiles kt = key_tiles(sq.past, sq.n_new, a.G, rr0, rr0 + BM, p.window, p.sinks, BN, 1);
+    const KeyTiles kt = key_tiles(sq.past, sq.n_new, a.G, rr0, rr0 + BM, p.window, p.sinks, BN, a.align);
     const int t0 = split * a.split_tiles, n = min(kt.n, t0 + a.split_tiles) - t0;
     if (n <= 0) return;
     const bool partial = kt.n > a.split_tiles;
 
-    const uint32_t q_s = smem_u32(smem), kv_s = q_s + BM * DP * 2;
-    long long* offs = reinterpret_cast<long long*>(smem + BM * DP * 2 + ST * 2 * Sh::kTileBytes);  // [ST + 1][BN]
-    auto swz = [](int row, int chunk) { return static_cast<uint32_t>(row * (DP * 2) + ((chunk ^ (row & 7)) << 4)); };
+    constexpr uint32_t kAlign = Sh::align(TMA);
+    const uint32_t q_s = (smem_u32(smem_raw) + kAlign - 1) & ~(kAlign - 1), kv_s = q_s + BM * DP * 2;
+    unsigned char* smem = smem_raw + (q_s - smem_u32(smem_raw));
+    constexpr int kOffs = BM * DP * 2 + ST * 2 * Sh::kTileBytes;
+    // this group's part of all of it
+    constexpr int kGroupTile = GK * DP * 2;
+    const int gt = tid - wk * (32 * WM), kb = wk * GK;  // thread within the group; its first key of a tile
+    const uint32_t ring = kv_s + wk * (ST * 2 * kGroupTile);
+    long long* offs = reinterpret_cast<long long*>(smem + kOffs) + wk * (ST + 1) * GK;  // [ST + 1][GK], cp.async
+    const uint32_t full = q_s + kOffs + 512 + wk * (ST * 8);                            // [ST] barriers, TMA
+    auto group_all = [&](bool ok) -> bool {  // barrier of the group, with the conjunction of what its threads bring
+        if (WM == 1) return __all_sync(0xffffffffu, ok);
+        int all;
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.and.pred q, %2, %3, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+            : "=r"(all)
+            : "r"(ok ? 1 : 0), "r"(1 + wk), "n"(32 * WM)
+            : "memory");
+        return all != 0;
+    };
+    auto swz = [](int rows, int row, int chunk) {
+        return static_cast<uint32_t>((chunk >> 3) * (rows * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+    };
+    const int slabs = (D + 63) / 64;
 
     const bf16* q = static_cast<const bf16*>(p.q);
-    for (int i = tid; i < BM * CH; i += 128) {
-        const int r = i / CH, c = i % CH, rr = rr0 + r;
+    for (int i = tid; i < BM * (DP / 8); i += 128) {
+        const int r = i / (DP / 8), c = i % (DP / 8), rr = rr0 + r;
         const bool in = rr < n_rows && c * 8 < D;
         const int t = rr / a.G;
         const bf16* src = in ? q + (sq.row0 + t) * p.ldq + static_cast<long long>(kvh * a.G + rr - t * a.G) * D + c * 8 : q;
-        cp_async16(q_s + swz(r, c), src, in);
+        cp_async16(q_s + swz(BM, r, c), src, in);
     }
+    if (TMA) cp_async_commit();
     const bf16* kc = static_cast<const bf16*>(p.cache.k) + kvh * p.cache.head_stride;
     const bf16* vc = static_cast<const bf16*>(p.cache.v) + kvh * p.cache.head_stride;
-    auto offset_of = [&](int i) -> long long {  // of this thread's key (tid < BN) of tile i
+    // cp.async: offset of this thread's key (gt < GK) of tile i
+    auto offset_of = [&](int i) -> long long {
         int start, end;
         key_range(kt, t0 + i, BN, start, end);
-        return start + tid < end ? key_offset(p, s, start + tid) : -1;
+        return start + kb + gt < end ? key_offset(p, s, start + kb + gt) : -1;
     };
     auto load = [&](int i) {
-        const long long* of = offs + (i % (ST + 1)) * BN;
-        const uint32_t ks = kv_s + (i % ST) * (2 * Sh::kTileBytes), vs = ks + Sh::kTileBytes;
-        constexpr int kRowsPerPass = 128 / CH < 1 ? 1 : 128 / CH;
+        const long long* of = offs + (i % (ST + 1)) * GK;
+        const uint32_t ks = ring + (i % ST) * (2 * kGroupTile), vs = ks + kGroupTile;
+        for (int slab = 0; slab < slabs; ++slab) {
+            const int c = slab * 8 + (gt & 7);
 #pragma unroll
-        for (int x = 0; x < BN / kRowsPerPass; ++x) {
-            const int key = tid / CH + x * kRowsPerPass, c = tid % CH;
-            const long long off = of[key];
-            const bool in = off >= 0 && c * 8 < D;
-            const long long e = in ? off + c * 8 : 0;
-            cp_async16(ks + swz(key, c), kc + e, in);
-            cp_async16(vs + swz(key, c), vc + e, in);
+            for (int x = 0; x < 4; ++x) {
+                const int key = x * (4 * WM) + (gt >> 3);
+                const long long off = of[key];
+                const bool in = off >= 0 && c * 8 < D;
+                const long long e = in ? off + c * 8 : 0;
+                cp_async16(ks + swz(GK, key, c), kc + e, in);
+                cp_async16(vs + swz(GK, key, c), vc + e, in);
+            }
         }
     };
-    if (tid < BN) {
+    // TMA, the group's first warp: the page of this lane's box (lane < GK / box) of tile i, -1 for none; and the tile's copies
+    auto page_of = [&](int i) -> int {
+        int start, end;
+        key_range(kt, t0 + i, BN, start, end);
+        const int key = start + kb + lane * box;
+        if (lane >= GK / box || key >= end) return -1;
+        const int slot = key / p.cache.page_size;
+        const int page = slot < p.batch.table_width ? p.batch.table[s * p.batch.table_stride + slot] : -1;
+        return page < p.cache.pages ? page : -1;
+    };
+    auto copy = [&](int i, int page) {
+        const uint32_t bar = full + 8u * (i % ST);
+        const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
+        if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(__popc(there)) * box * 128 * 2 * slabs);
+        __syncwarp();
+        if (page < 0) return;
+        int start, end;
+        key_range(kt, t0 + i, BN, start, end);
+        const int at = (start + kb + lane * box) % p.cache.page_size;
+        const uint32_t ks = ring + (i % ST) * (2 * kGroupTile) + lane * box * 128;
+        for (int slab = 0; slab < slabs; ++slab) {
+            tma_load_4d(&k_map, ks + slab * (GK * 128), bar, slab * 64, at, kvh, page);
+            tma_load_4d(&v_map, ks + kGroupTile + slab * (GK * 128), bar, slab * 64, at, kvh, page);
+        }
+    };
+    bool bad_page = false;
+    int next_page = -1;
+    if (TMA) {
+        if (tid == 0) {
+            for (int i = 0; i < WK * ST; ++i) mbar_init(q_s + kOffs + 512 + 8u * i, 1);
+            fence_barrier_init();
+        }
+        bad_page = __syncthreads_or(any_bad_page(p, s, kt, t0, n, BN));
+        if (wm == 0) {
 #pragma unroll
-        for (int i = 0; i < ST; ++i) offs[i * BN + tid] = i < n ? offset_of(i) : -1;
-    }
-    __syncthreads();
+            for (int i = 0; i < ST - 1; ++i)
+                if (i < n) copy(i, page_of(i));
+            if (ST - 1 < n) next_page = page_of(ST - 1);
+        }
+        cp_async_wait<0>();
+        __syncthreads();  // q is there
+    } else {
+        if (gt < GK) {
 #pragma unroll
-    for (int i = 0; i < ST - 1; ++i) {
-        if (i < n) load(i);
-        cp_async_commit();
+            for (int i = 0; i < ST; ++i) offs[i * GK + gt] = i < n ? offset_of(i) : -1;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < ST - 1; ++i) {
+            if (i < n) load(i);
+            cp_async_commit();
+        }
+        cp_async_wait<ST - 2>();
+        __syncthreads();  // every thread's part of q (and of tile 0) is there
     }
 
     float o[DP / 8][4];
@@ -287,38 +371,64 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
     }
     const float scale_log2 = p.scale * kLog2e;
     const float cap_in = p.softcap > 0.f ? 2.f * scale_log2 / p.softcap : 0.f, cap_out = p.softcap * kLog2e;
-    const int kb = wk * (BN / WK);
 
     for (int i = 0; i < n; ++i) {
-        cp_async_wait<ST - 2>();
-        __syncthreads();
-        if (i + ST - 1 < n) load(i + ST - 1);
-        cp_async_commit();
-        const long long next = tid < BN && i + ST < n ? offset_of(i + ST) : -1;
+        long long next = -1;
+        if (TMA) {
+            const bool ok = mbar_wait(full + 8u * (i % ST), (i / ST) & 1, p.err, kTimeout);
+            if (!group_all(ok)) {  // the group leaves together; what is on its way lands first
+                for (int x = i; x < min(n, i + ST - 1); ++x) mbar_wait_quiet(full + 8u * (x % ST), (x / ST) & 1);
+                break;
+            }
+            if (wm == 0) {
+                if (i + ST - 1 < n) copy(i + ST - 1, next_page);
+                if (i + ST < n) next_page = page_of(i + ST);
+            }
+        } else {
+            cp_async_wait<ST - 2>();
+            group_all(true);
+            if (i + ST - 1 < n) load(i + ST - 1);
+            cp_async_commit();
+            if (gt < GK && i + ST < n) next = offset_of(i + ST);
+        }
 
-        const uint32_t ks = kv_s + (i % ST) * (2 * Sh::kTileBytes), vs = ks + Sh::kTileBytes;
-        float sc[NT][4];
+        const uint32_t ks = ring + (i % ST) * (2 * kGroupTile), vs = ks + kGroupTile;
+        // two chains of products per score where a warp has few scores
+        float sc[NT][4], sd[NT == 2 ? NT : 1][4];
 #pragma unroll
         for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
+        if (NT == 2) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) sd[t % (NT == 2 ? 2 : 1)][0] = sd[t % (NT == 2 ? 2 : 1)][1] = sd[t % (NT == 2 ? 2 : 1)][2] = sd[t % (NT == 2 ? 2 : 1)][3] = 0.f;
+        }
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {
             if (kk * 16 < D) {
                 uint32_t qa[4];
-                ldmatrix4(qa, q_s + swz(wm * 16 + (lane & 15), kk * 2 + (lane >> 4)));
+                ldmatrix4(qa, q_s + swz(BM, wm * 16 + (lane & 15), kk * 2 + (lane >> 4)));
 #pragma unroll
                 for (int t = 0; t < NT / 2; ++t) {
                     uint32_t b[4];
-                    ldmatrix4(b, ks + swz(kb + t * 16 + (lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)));
-                    mma16816(sc[2 * t], qa, b[0], b[1]);
-                    mma16816(sc[2 * t + 1], qa, b[2], b[3]);
+                    ldmatrix4(b, ks + swz(GK, t * 16 + (lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)));
+                    mma16816(NT == 2 && (kk & 1) ? sd[0] : sc[2 * t], qa, b[0], b[1]);
+                    mma16816(NT == 2 && (kk & 1) ? sd[NT == 2 ? 1 : 0] : sc[2 * t + 1], qa, b[2], b[3]);
                 }
             }
         }
+        if (NT == 2) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[0][e] += sd[0][e], sc[NT - 1][e] += sd[NT == 2 ? 1 : 0][e];
+        }
         int start, end;
         key_range(kt, t0 + i, BN, start, end);
-        const long long* of = offs + (i % (ST + 1)) * BN;
-        const bool whole = !__any_sync(0xffffffffu, of[lane] < 0 || of[lane + 32] < 0) &&
-                           all_seen(kt, start, end, p.window, p.sinks);
+        start += kb;  // of the group
+        const long long* of = offs + (i % (ST + 1)) * GK;
+        auto there = [&](int key) {  // key of the tile exists: it is in the range and its page in the pool
+            return TMA ? start + key < end && (!bad_page || key_offset(p, s, start + key) >= 0) : of[key] >= 0;
+        };
+        const bool missing = TMA ? end - start < GK || bad_page
+                                 : __any_sync(0xffffffffu, of[lane % GK] < 0 || (GK == 64 && of[(lane + 32) % GK] < 0));
+        const bool whole = !missing && all_seen(kt, start, min(end, start + GK), p.window, p.sinks);
         if (p.softcap > 0.f) {
 #pragma unroll
             for (int t = 0; t < NT; ++t)
@@ -335,8 +445,8 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int key = kb + t * 8 + (lane & 3) * 2 + (e & 1);
-                    if (of[key] < 0 || !seen(start + key, pos[e >> 1], p.window, p.sinks)) sc[t][e] = kNegInf;
+                    const int key = t * 8 + (lane & 3) * 2 + (e & 1);
+                    if (!there(key) || !seen(start + key, pos[e >> 1], p.window, p.sinks)) sc[t][e] = kNegInf;
                 }
         }
         float alpha[2];
@@ -372,12 +482,12 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
             const uint32_t pa[4] = {pack_bf2(sc[2 * t][0], sc[2 * t][1]), pack_bf2(sc[2 * t][2], sc[2 * t][3]),
                                     pack_bf2(sc[2 * t + 1][0], sc[2 * t + 1][1]),
                                     pack_bf2(sc[2 * t + 1][2], sc[2 * t + 1][3])};
-            const int row = kb + t * 16 + (lane & 15);
+            const int row = t * 16 + (lane & 15);
 #pragma unroll
             for (int d = 0; d < DP / 16; ++d) {
                 if (d * 16 < D) {
                     uint32_t b[4];
-                    ldmatrix4_t(b, vs + swz(row, d * 2 + (lane >> 4)));
+                    ldmatrix4_t(b, vs + swz(GK, row, d * 2 + (lane >> 4)));
                     if (!whole) {  // 0 * v must be 0 for the rows that do not see v
 #pragma unroll
                         for (int x = 0; x < 4; ++x) b[x] = finite2(b[x], bad);
@@ -389,14 +499,14 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
         }
         if (!whole && __any_sync(0xffffffffu, bad)) {
             // what finite2 took out, given back to the rows that see it
-            for (int key = kb; key < kb + BN / WK; ++key) {
-                if (of[key] < 0) continue;
+            for (int key = 0; key < GK; ++key) {
+                if (!there(key)) continue;
                 const bool s0 = seen(start + key, pos[0], p.window, p.sinks);
                 const bool s1 = seen(start + key, pos[1], p.window, p.sinks);
                 const unsigned char* vrow = smem + (vs - q_s);
 #pragma unroll
                 for (int d = 0; d < DP / 8; ++d) {
-                    const uint32_t x = *reinterpret_cast<const uint32_t*>(vrow + swz(key, d) + (lane & 3) * 4);
+                    const uint32_t x = *reinterpret_cast<const uint32_t*>(vrow + swz(GK, key, d) + (lane & 3) * 4);
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const float v = __uint_as_float(e ? x & 0xffff0000u : x << 16);
@@ -407,7 +517,7 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
                 }
             }
         }
-        if (tid < BN) offs[((i + ST) % (ST + 1)) * BN + tid] = next;
+        if (!TMA && gt < GK) offs[((i + ST) % (ST + 1)) * GK + gt] = next;
     }
     cp_async_wait<0>();
 #pragma unroll
@@ -416,12 +526,12 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
         l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     }
     __syncthreads();
-    // [WK][BM] rows of DP fp32 over the tiles' memory, and (max, sum) over the lookups'
+    // [WK][BM] rows of DP fp32 over the tiles' memory, and (max, sum) behind it
     constexpr int LD = DP + 8;
     static_assert(WK * BM * LD * 4 <= ST * 2 * Sh::kTileBytes, "the join fits the tiles' memory");
-    static_assert(WK * BM * 8 <= (ST + 1) * BN * 8, "the statistics fit the lookups' memory");
+    static_assert(WK * BM * 8 <= 512, "the statistics fit the memory behind the tiles");
     float* os = reinterpret_cast<float*>(smem + BM * DP * 2);
-    float2* st = reinterpret_cast<float2*>(offs);
+    float2* st = reinterpret_cast<float2*>(smem + kOffs);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         const int row = wk * BM + wm * 16 + (lane >> 2) + 8 * r;
@@ -466,50 +576,83 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
 }
 
 // --- joining the splits -----------------------------------------------------------------------
-// One block per row and four heads, one warp per head: the splits' maxima give the weights, then
-// each lane sums its channels over the splits in order.
+// One block per row and head. The splits' maxima give their weights (shared memory, kSome at a time);
+// the warps share out the splits, and each lane sums its channels over its warp's, then over the warps
+// in order. It is launched beside the kernel before it and waits for that one's end on the device, so
+// that its own start is not added to a decoding step.
+constexpr int kSome = 128;
 template <class T>
 __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constant__ Args a) {
+    __shared__ float weight[kSome];
+    __shared__ float red[4];
+    __shared__ float sums[4][256];
     const PagedAttention& p = a.p;
-    const int row = blockIdx.x, lane = threadIdx.x & 31, h = blockIdx.y * 4 + (threadIdx.x >> 5), D = p.cache.D;
+    const int row = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = p.cache.D;
     int s = 0;
     for (int s0 = 0; s0 < p.batch.S; s0 += 128) {
-        const int i = s0 + static_cast<int>(threadIdx.x);
+        const int i = s0 + tid;
         s += __syncthreads_count(i < p.batch.S && p.batch.row_start[i + 1] <= row);
     }
-    if (s >= p.batch.S || h >= p.q_heads) return;
-    const Sequence sq = sequence(p, s, false);
-    if (!sq.ok || row < sq.row0) return;
-    const int rr = (row - sq.row0) * a.G + h % a.G, tile = rr / a.BM;
-    const KeyTiles kt = key_tiles(sq.past, sq.n_new, a.G, tile * a.BM, (tile + 1) * a.BM, p.window, p.sinks, a.BN,
-                                  a.align);
-    const int active = (kt.n + a.split_tiles - 1) / a.split_tiles;
-    if (active <= 1) return;
+    int active = 0;
+    if (s < p.batch.S) {
+        const Sequence sq = sequence(p, s, false);
+        if (sq.ok && row >= sq.row0) {
+            const int rr = (row - sq.row0) * a.G + h % a.G, tile = rr / a.BM;
+            const KeyTiles kt = key_tiles(sq.past, sq.n_new, a.G, tile * a.BM, (tile + 1) * a.BM, p.window, p.sinks, a.BN, a.align);
+            active = (kt.n + a.split_tiles - 1) / a.split_tiles;
+        }
+    }
+    cudaGridDependencySynchronize();
+    if (active <= 1) return;  // written already, or not to be written
     const long long step = static_cast<long long>(p.batch.rows) * p.q_heads;
     const long long at = static_cast<long long>(row) * p.q_heads + h;
     float m = kNegInf;
-    for (int i = lane; i < active; i += 32) m = fmaxf(m, a.ml[at + i * step].x);
+    for (int i = tid; i < active; i += 128) m = fmaxf(m, a.ml[at + i * step].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) red[warp] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     const float base = m == kNegInf ? 0.f : m;
     float acc[8] = {}, l = 0.f;
-    for (int i = 0; i < active; ++i) {
-        const float2 x = a.ml[at + i * step];
-        const float f = ex2_approx(x.x - base);
-        l = fmaf(x.y, f, l);
-        const float* src = a.part + (at + i * step) * D;
+    for (int i0 = 0; i0 < active; i0 += kSome) {
+        __syncthreads();
+        if (i0 + tid < active) {
+            const float2 x = a.ml[at + (i0 + tid) * step];
+            const float f = ex2_approx(x.x - base);
+            weight[tid] = f;
+            l = fmaf(x.y, f, l);
+        }
+        __syncthreads();
+        const int n = min(kSome, active - i0);
+#pragma unroll 4
+        for (int i = warp; i < n; i += 4) {
+            const float f = weight[i];
+            const float* src = a.part + (at + (i0 + i) * step) * D;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (lane + 32 * e < D) acc[e] = fmaf(src[lane + 32 * e], f, acc[e]);
+            for (int e = 0; e < 8; ++e)
+                if (lane + 32 * e < D) acc[e] = fmaf(src[lane + 32 * e], f, acc[e]);
+        }
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    __syncthreads();
+    if (lane == 0) red[warp] = l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[warp][lane + 32 * e] = acc[e];
+    __syncthreads();
+    l = (red[0] + red[1]) + (red[2] + red[3]);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T* out = static_cast<T*>(p.out) + static_cast<long long>(row) * p.ldo + static_cast<long long>(h) * D;
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (lane + 32 * e < D) out[lane + 32 * e] = from_f<T>(acc[e] * inv);
+    for (int d = tid; d < D; d += 128)
+        out[d] = from_f<T>(((sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d])) * inv);
 }
 
 // --- plan and launch ----------------------------------------------------------------------------
+#ifndef SPLITW
+#define SPLITW 16
+#define SPLITT 2
+#endif
 enum Kind { kSimt, kMma, kTc };
 
 // The tcgen05 kernel's 128-row tiles take over from the mma.sync kernel's 64-row ones above this
@@ -540,11 +683,12 @@ Args plan(const PagedAttention& p, Kind kind, int num_sms) {
     } else if (kind == kTc) {
         a.BM = tc_rows(p.cache.D);
         a.BN = tc_keys(p.cache.D);
-        a.align = std::max(1, tc_box(p.cache));
+        a.align = std::max(1, copy_box(p.cache, a.BN));
         resident = 1;
     } else {
         a.BM = packed <= 16 ? 16 : packed <= 32 ? 32 : 64;
         a.BN = 64;
+        a.align = std::max(1, copy_box(p.cache, a.BM));  // a group brings as many keys as a block has rows
         resident = p.cache.D > 128 ? 1 : 2;
     }
     a.row_tiles = ceil_div(packed, a.BM);
@@ -556,8 +700,8 @@ Args plan(const PagedAttention& p, Kind kind, int num_sms) {
     const long long base = static_cast<long long>(p.batch.S) * p.cache.kv_heads * a.row_tiles;
     // One sequence: one wave of equal blocks. Several: their lengths differ and only the longest is
     // known here, so blocks of a few waves' size even them out.
-    const long long want = static_cast<long long>(num_sms) * resident * (p.batch.S == 1 || kind == kTc ? 1 : 4);
-    const long long splits = std::max<long long>(1, std::min<long long>(want / std::max<long long>(base, 1), tiles / 2));
+    const long long want = static_cast<long long>(num_sms) * resident * (p.batch.S == 1 || kind == kTc ? 1 : SPLITW);
+    const long long splits = std::max<long long>(1, std::min<long long>(want / std::max<long long>(base, 1), tiles / SPLITT));
     a.split_tiles = std::max(1, ceil_div(tiles, splits));
     a.splits = ceil_div(tiles, a.split_tiles);
     return a;
@@ -576,13 +720,25 @@ void raise_smem(const void* f, int bytes, PerDeviceOnce& once) {
     once.mark();
 }
 
+template <int DP, int WM, bool TMA>
+void launch_mma(const Args& a, int box, dim3 grid, cudaStream_t st) {
+    static PerDeviceOnce once;
+    constexpr int bytes = MmaShape<DP>::smem(16 * WM, TMA);
+    static_assert(bytes <= 232448, "shared memory of one block");
+    raise_smem(reinterpret_cast<const void*>(&paged_mma_kernel<DP, WM, TMA>), bytes, once);
+    CUtensorMap k{}, v{};
+    if (TMA) {
+        k = pool_map(a.p.cache, a.p.cache.k, box);
+        v = pool_map(a.p.cache, a.p.cache.v, box);
+    }
+    paged_mma_kernel<DP, WM, TMA><<<grid, 128, bytes, st>>>(a, k, v, box);
+}
+
 template <int DP, int WM>
 void launch_mma(const Args& a, dim3 grid, cudaStream_t st) {
-    static PerDeviceOnce once;
-    constexpr int bytes = MmaShape<DP>::smem(16 * WM);
-    static_assert(bytes <= 232448, "shared memory of one block");
-    raise_smem(reinterpret_cast<const void*>(&paged_mma_kernel<DP, WM>), bytes, once);
-    paged_mma_kernel<DP, WM><<<grid, 128, bytes, st>>>(a);
+    const int box = copy_box(a.p.cache, 16 * WM);  // within a group's keys
+    if (box > 0) launch_mma<DP, WM, true>(a, box, grid, st);
+    else launch_mma<DP, WM, false>(a, 0, grid, st);
 }
 
 template <int DP>
@@ -602,6 +758,29 @@ void launch_simt(const Args& a, dim3 grid, cudaStream_t st) {
 }
 
 }  // namespace
+
+// Boxes are whole groups of eight rows, which the swizzle needs. A tensor map's strides end at 2^40 bytes; a stride of 0
+// (other than of a size 1) is not encoded.
+int copy_box(const PagedCache& c, int keys) {
+    const long long most = 1LL << 38;
+    const bool strides_ok = c.page_stride < most && c.token_stride < most && c.head_stride < most &&
+                            (c.page_stride >= 8 || c.pages == 1) && (c.token_stride >= 8 || c.page_size == 1) &&
+                            (c.head_stride >= 8 || c.kv_heads == 1);
+    if (!strides_ok || c.pages < 1) return 0;
+    if (c.page_size % keys == 0) return keys;
+    return c.page_size % 8 == 0 && keys % c.page_size == 0 ? c.page_size : 0;
+}
+
+CUtensorMap pool_map(const PagedCache& c, const void* base, int box) {
+    CUtensorMap m;
+    auto stride = [](long long elements) { return static_cast<cuuint64_t>(elements > 8 ? elements * 2 : 16); };
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.D), static_cast<cuuint64_t>(c.page_size),
+                                static_cast<cuuint64_t>(c.kv_heads), static_cast<cuuint64_t>(c.pages)};
+    const cuuint64_t strides[3] = {stride(c.token_stride), stride(c.head_stride), stride(c.page_stride)};
+    const cuuint32_t b[4] = {64, static_cast<cuuint32_t>(box), 1, 1};
+    tma_encode_tiled(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides, b, CU_TENSOR_MAP_SWIZZLE_128B);
+    return m;
+}
 }  // namespace pattn
 
 using namespace pattn;
@@ -642,9 +821,17 @@ void paged_attention(const PagedAttention& p, int num_sms, cudaStream_t st) {
     }
     SANA_CUDA(cudaGetLastError());
     if (a.splits > 1) {
-        const dim3 cgrid(static_cast<unsigned>(p.batch.rows), static_cast<unsigned>((p.q_heads + 3) / 4));
-        if (p.cache.dtype == kF32) paged_combine_kernel<float><<<cgrid, 128, 0, st>>>(a);
-        else paged_combine_kernel<bf16><<<cgrid, 128, 0, st>>>(a);
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(static_cast<unsigned>(p.batch.rows), static_cast<unsigned>(p.q_heads));
+        cfg.blockDim = dim3(128);
+        cfg.stream = st;
+        cudaLaunchAttribute early{};
+        early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        early.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &early;
+        cfg.numAttrs = 1;
+        if (p.cache.dtype == kF32) SANA_CUDA(cudaLaunchKernelEx(&cfg, paged_combine_kernel<float>, a));
+        else SANA_CUDA(cudaLaunchKernelEx(&cfg, paged_combine_kernel<bf16>, a));
         SANA_CUDA(cudaGetLastError());
     }
 }

@@ -15,6 +15,8 @@
 // paged_combine_kernel in a fixed order.
 #pragma once
 
+#include <cuda.h>
+
 #include "encoder.h"
 
 namespace sana {
@@ -109,10 +111,41 @@ __device__ __forceinline__ long long key_offset(const PagedAttention& p, int s, 
     return page * p.cache.page_stride + static_cast<long long>(j - static_cast<int>(slot) * p.cache.page_size) * p.cache.token_stride;
 }
 
+// Whether the page of any of the keys [lo, hi) is not in the pool; the block's threads share out the pages.
+__device__ __forceinline__ bool any_bad_page(const PagedAttention& p, int s, int lo, int hi) {
+    bool bad = false;
+    for (int j = lo / p.cache.page_size + static_cast<int>(threadIdx.x); j <= (hi - 1) / p.cache.page_size;
+         j += static_cast<int>(blockDim.x))
+        bad = key_offset(p, s, min(max(j * p.cache.page_size, lo), hi - 1)) < 0 || bad;
+    return bad;
+}
+// The same for the key tiles [t0, t0 + n) of a row tile.
+__device__ __forceinline__ bool any_bad_page(const PagedAttention& p, int s, const KeyTiles& kt, int t0, int n, int BN) {
+    bool bad = false;
+    int lo, hi, unused;
+    if (t0 < kt.n_sink) {
+        key_range(kt, t0, BN, lo, unused);
+        key_range(kt, min(kt.n_sink, t0 + n) - 1, BN, unused, hi);
+        bad = any_bad_page(p, s, lo, hi);
+    }
+    if (t0 + n > kt.n_sink) {
+        key_range(kt, max(t0, kt.n_sink), BN, lo, unused);
+        key_range(kt, t0 + n - 1, BN, unused, hi);
+        bad = any_bad_page(p, s, lo, hi) || bad;
+    }
+    return bad;
+}
+
+// Keys that one tensor copy (TMA) brings of tiles of `keys` keys: a page, or a key tile where pages are multiples of
+// tiles; 0 where a page ends inside a tile or the pool's strides do not fit a tensor map.
+int copy_box(const PagedCache& c, int keys);
+// The pool's k or v as a tensor [pages][kv_heads][page_size][D] of boxes of `box` tokens of one head x 64 channels, in
+// the 128-byte swizzle.
+CUtensorMap pool_map(const PagedCache& c, const void* base, int box);
+
 // pattn_tc.cu: packed rows and keys of a block's tile for a head size, and the launch.
 int tc_rows(int D);
 int tc_keys(int D);
-int tc_box(const PagedCache& c);  // keys that one tensor copy brings (0: copies of 16 bytes)
 void launch_tc(const Args& a, dim3 grid, cudaStream_t st);
 
 }  // namespace pattn

@@ -170,6 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = p.cache.D;
     const int tile = a.row_tiles - 1 - static_cast<int>(blockIdx.x % a.row_tiles);
     const int rest = blockIdx.x / a.row_tiles, split = rest % a.splits, s = rest / a.splits, kvh = blockIdx.y;
+    cudaTriggerProgrammaticLaunchCompletion();  // the join's blocks may take their places
     const Sequence sq = sequence(p, s, blockIdx.x % (a.row_tiles * a.splits) == 0 && kvh == 0 && tid == 0);
     const int rr0 = tile * Sh::kRows, n_rows = sq.n_new * a.G;
     if (!sq.ok || rr0 >= n_rows) return;
@@ -236,22 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         cp_async_commit();
     }
     __syncthreads();  // words[] are set; the pages of this block's keys are checked while Q is on its way
-    {
-        int lo, hi, unused;
-        const int b0 = max(t0, kt.n_sink);
-        if (t0 < kt.n_sink) {
-            key_range(kt, t0, BN, lo, unused);
-            key_range(kt, min(kt.n_sink, t0 + n) - 1, BN, unused, hi);
-            for (int j = lo / p.cache.page_size + tid; j <= (hi - 1) / p.cache.page_size; j += kThreads)
-                if (key_offset(p, s, min(max(j * p.cache.page_size, lo), hi - 1)) < 0) words[1] = 1;
-        }
-        if (b0 < t0 + n) {
-            key_range(kt, b0, BN, lo, unused);
-            key_range(kt, t0 + n - 1, BN, unused, hi);
-            for (int j = lo / p.cache.page_size + tid; j <= (hi - 1) / p.cache.page_size; j += kThreads)
-                if (key_offset(p, s, min(max(j * p.cache.page_size, lo), hi - 1)) < 0) words[1] = 1;
-        }
-    }
+    if (any_bad_page(p, s, kt, t0, n, BN)) words[1] = 1;
     cp_async_wait<0>();
     fence_proxy_async_smem();
     tc_fence_before();
@@ -664,18 +650,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
 }
 
-// The pool as a tensor [pages][kv_heads][page_size][D], boxes of `box` tokens of one head x 64 channels.
-CUtensorMap pool_map(const PagedCache& c, const void* base, int box) {
-    CUtensorMap m;
-    auto stride = [](long long elements) { return static_cast<cuuint64_t>(elements > 8 ? elements * 2 : 16); };
-    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.D), static_cast<cuuint64_t>(c.page_size),
-                                static_cast<cuuint64_t>(c.kv_heads), static_cast<cuuint64_t>(c.pages)};
-    const cuuint64_t strides[3] = {stride(c.token_stride), stride(c.head_stride), stride(c.page_stride)};
-    const cuuint32_t b[4] = {64, static_cast<cuuint32_t>(box), 1, 1};
-    tma_encode_tiled(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides, b, CU_TENSOR_MAP_SWIZZLE_128B);
-    return m;
-}
-
 template <int DP, bool CAP>
 void launch(const Args& a, dim3 grid, cudaStream_t st) {
     static PerDeviceOnce once;
@@ -685,7 +659,7 @@ void launch(const Args& a, dim3 grid, cudaStream_t st) {
         SANA_CUDA(cudaFuncSetAttribute(paged_tc_kernel<DP, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem));
         once.mark();
     }
-    const int box = tc_box(a.p.cache);
+    const int box = copy_box(a.p.cache, Sh::kKeys);
     CUtensorMap k{}, v{};
     if (box > 0) {
         k = pool_map(a.p.cache, a.p.cache.k, box);
@@ -698,18 +672,6 @@ void launch(const Args& a, dim3 grid, cudaStream_t st) {
 
 int tc_rows(int D) { return D <= 128 ? 256 : 128; }
 int tc_keys(int D) { return D <= 128 ? 128 : 64; }
-// A box is a page, or a key tile where pages are multiples of tiles; whole groups of eight rows, which the
-// swizzle needs. The strides of a tensor map end at 2^40 bytes; a stride of 0 (or of a size 1) is not encoded.
-int tc_box(const PagedCache& c) {
-    const int keys = tc_keys(c.D);
-    const long long most = 1LL << 38;
-    const bool strides_ok = c.page_stride < most && c.token_stride < most && c.head_stride < most &&
-                            (c.page_stride >= 8 || c.pages == 1) && (c.token_stride >= 8 || c.page_size == 1) &&
-                            (c.head_stride >= 8 || c.kv_heads == 1);
-    if (!strides_ok || c.pages < 1) return 0;
-    if (c.page_size % keys == 0) return keys;
-    return c.page_size % 8 == 0 && keys % c.page_size == 0 ? c.page_size : 0;
-}
 void launch_tc(const Args& a, dim3 grid, cudaStream_t st) {
     const bool cap = a.p.softcap > 0.f;
     if (a.p.cache.D <= 64) cap ? launch<64, true>(a, grid, st) : launch<64, false>(a, grid, st);

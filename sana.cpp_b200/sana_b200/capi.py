@@ -45,6 +45,21 @@ class sana_paged_batch(ctypes.Structure):
 
 
 SANA_DTYPE_F32, SANA_DTYPE_BF16, SANA_DTYPE_E4M3 = 0, 1, 2
+_DTYPES: dict = {}  # torch's types -> SANA_DTYPE_*, filled when torch is first needed
+_TORCH = None
+
+
+def _torch():
+    """torch, imported when a method on its tensors is first called."""
+    global _TORCH
+    if _TORCH is None:
+        import torch
+        _DTYPES.update({torch.float32: SANA_DTYPE_F32, torch.bfloat16: SANA_DTYPE_BF16,
+                        torch.float8_e4m3fn: SANA_DTYPE_E4M3})
+        _TORCH = torch
+    return _TORCH
+
+
 ROPE_SCALING = {"plain": 0, "linear": 1, "base": 2, "parts": 3}
 
 
@@ -406,12 +421,12 @@ class SanaCuda:
     # memory that torch hands out again) are safe to use on torch's stream. torch's default
     # stream is CUDA's legacy stream: set_stream(1) puts the handle on it.
     def _run(self, name, *args):
-        import torch
-        current = torch.cuda.current_stream(self.device)
+        torch = _torch()
         mine = self.stream
-        if mine == (current.cuda_stream or 1):
+        if mine == (torch._C._cuda_getCurrentRawStream(self.device) or 1):
             self._call(name, *args)
             return
+        current = torch.cuda.current_stream(self.device)
         other = torch.cuda.ExternalStream(mine, device=self.device)
         other.wait_stream(current)
         try:
@@ -419,19 +434,22 @@ class SanaCuda:
         finally:
             current.wait_stream(other)
 
-    def _dtype(self, t, what, allowed=("float32", "bfloat16")):
-        name = str(t.dtype).rpartition(".")[2]
-        if name not in allowed:
-            raise ValueError(f"{what} must be {' or '.join(allowed)}, not {name}")
-        if t.device.type != "cuda" or t.device.index != self.device:
+    def _dtype(self, t, what, allowed="float32 or bfloat16"):
+        """The SANA_DTYPE of a tensor on the handle's device, of a type named in `allowed`."""
+        if t.get_device() != self.device:
             raise ValueError(f"{what} must be on cuda:{self.device}, not {t.device}")
-        return {"float32": SANA_DTYPE_F32, "bfloat16": SANA_DTYPE_BF16}.get(name, -1)
+        dt = (_DTYPES or _torch() and _DTYPES).get(t.dtype)
+        if dt is None or dt > SANA_DTYPE_BF16:
+            raise ValueError(f"{what} must be {allowed}, not {t.dtype}")
+        return dt
 
     @staticmethod
     def _row_stride(t, what):
         """Elements between the rows of t [rows, ...], whose rows must be contiguous."""
-        shape, stride = t.shape, t.stride()
-        width = 1
+        shape = t.shape
+        if shape[0] and t.is_contiguous():
+            return t.numel() // shape[0]
+        stride, width = t.stride(), 1
         for n, st in zip(reversed(shape[1:]), reversed(stride[1:])):
             if n != 1 and st != width:
                 raise ValueError(f"{what}: the elements of a row must be contiguous")
@@ -439,8 +457,10 @@ class SanaCuda:
         return max(stride[0], width) if shape[0] <= 1 else stride[0]
 
     def _vector(self, t, what, dtype, n=None):
-        self._dtype(t, what, (dtype,))
-        if t.dim() != 1 or (n is not None and t.shape[0] != n) or (t.shape[0] > 1 and t.stride(0) != 1):
+        """The address of a contiguous vector of n elements (any number for None)."""
+        if t.dtype is not dtype or t.get_device() != self.device:
+            raise ValueError(f"{what} must be {dtype} on cuda:{self.device}, not {t.dtype} on {t.device}")
+        if t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n):
             raise ValueError(f"{what} must be a contiguous vector" + ("" if n is None else f" of {n}"))
         return t.data_ptr()
 
@@ -450,85 +470,104 @@ class SanaCuda:
         out_dtype torch.float8_e4m3fn with one scale per `group` channels (0: per row); without a
         residual the sum is left out of the answer. out_dtype defaults to x's. inplace writes the
         sum over the residual."""
-        import torch
+        torch = _torch()
         xt = self._dtype(x, "x")
         if x.dim() != 2:
             raise ValueError("x must be [rows, C]")
         rows, C = x.shape
-        out_dtype = out_dtype or x.dtype
-        ot = {torch.float32: SANA_DTYPE_F32, torch.bfloat16: SANA_DTYPE_BF16, torch.float8_e4m3fn: SANA_DTYPE_E4M3}.get(out_dtype)
-        if ot is None:
-            raise ValueError("out_dtype must be float32, bfloat16 or float8_e4m3fn")
+        if out_dtype is None:
+            out_dtype, ot = x.dtype, xt
+        else:
+            ot = _DTYPES.get(out_dtype)
+            if ot is None:
+                raise ValueError("out_dtype must be float32, bfloat16 or float8_e4m3fn")
         rt, ldr, rp, total, tp = 0, C, None, None, None
         if residual is not None:
             rt = self._dtype(residual, "residual")
             if residual.shape != x.shape:
                 raise ValueError("residual must have x's shape")
             ldr, rp = self._row_stride(residual, "residual"), residual.data_ptr()
-            total = residual if inplace else torch.empty_strided((rows, C), (ldr, 1), dtype=residual.dtype, device=x.device)
+            if inplace:
+                total = residual
+            elif residual.is_contiguous():
+                total = torch.empty_like(residual)
+            else:
+                total = torch.empty_strided((rows, C), (ldr, 1), dtype=residual.dtype, device=x.device)
             tp = total.data_ptr()
-        wp = None if weight is None else self._vector(weight, "weight", "float32", C)
-        out = torch.empty((rows, C), dtype=out_dtype, device=x.device)
-        scale = None
+        wp = None if weight is None else self._vector(weight, "weight", torch.float32, C)
+        out = torch.empty_like(x, dtype=out_dtype, memory_format=torch.contiguous_format)
+        scale, sp = None, None
         if ot == SANA_DTYPE_E4M3:
-            scale = torch.empty((rows, -(-C // group) if group > 0 else 1), dtype=torch.float32, device=x.device)
+            scale = x.new_empty((rows, -(-C // group) if group > 0 else 1), dtype=torch.float32)
+            sp = scale.data_ptr()
         self._run("sana_op_add_rms_norm_device", x.data_ptr(), xt, self._row_stride(x, "x"), rp, rt, ldr, tp, wp,
-                  weight_offset, eps, rows, C, out.data_ptr(), ot, C, None if scale is None else scale.data_ptr(), group)
-        got = [out] + ([scale] if scale is not None else []) + ([total] if total is not None else [])
-        return got[0] if len(got) == 1 else tuple(got)
+                  weight_offset, eps, rows, C, out.data_ptr(), ot, C, sp, group)
+        if total is None:
+            return out if scale is None else (out, scale)
+        return (out, total) if scale is None else (out, scale, total)
 
     def _heads(self, t, what, rows=None, heads=None, dim=None, dtype=None):
         dt = self._dtype(t, what)
-        if t.dim() != 3 or (rows is not None and t.shape[0] != rows) or (heads is not None and t.shape[1] != heads) or (
-                dim is not None and t.shape[2] != dim):
+        shape = t.shape
+        if len(shape) != 3 or (rows is not None and shape[0] != rows) or (heads is not None and shape[1] != heads) or (
+                dim is not None and shape[2] != dim):
             raise ValueError(f"{what} must be [{'rows' if rows is None else rows}, {'heads' if heads is None else heads}, "
                              f"{'head_dim' if dim is None else dim}]")
         if dtype is not None and dt != dtype:
             raise ValueError(f"{what} must have the type of the others")
         return dt, self._row_stride(t, what)
 
+    @staticmethod
+    def _like_rows(t, ld):
+        """Uninitialised memory for t's rows [rows, heads, D], rows ld elements apart."""
+        if t.is_contiguous():
+            return _torch().empty_like(t)
+        return _torch().empty_strided(t.shape, (ld, t.shape[2], 1), dtype=t.dtype, device=t.device)
+
     def _rotary(self, frequencies, interleaved, magnitude):
         n = frequencies.shape[0] if frequencies.dim() == 1 else -1
-        return sana_rotary(self._vector(frequencies, "frequencies", "float64", n), 2 * n, 1 if interleaved else 0, magnitude)
+        return sana_rotary(self._vector(frequencies, "frequencies", _torch().float64, n), 2 * n, 1 if interleaved else 0,
+                           magnitude)
 
     def rotary_device(self, q, k, positions, frequencies, interleaved: bool = False, magnitude: float = 1.0,
                       inplace: bool = False):
         """sana_op_rotary_device: q [rows, q_heads, D] and k [rows, kv_heads, D] (or None) turned
         at the int32 positions [rows]; frequencies float64 [rotated/2] on the device."""
-        import torch
         dt, ldq = self._heads(q, "q")
         rows, heads, D = q.shape
-        kv, ldk, kp, k_out = 0, 0, None, None
+        kv, ldk, kp, kop, k_out = 0, 0, None, None, None
         if k is not None:
             _, ldk = self._heads(k, "k", rows, None, D, dt)
             kv, kp = k.shape[1], k.data_ptr()
-            k_out = k if inplace else torch.empty_strided(k.shape, (ldk, D, 1), dtype=k.dtype, device=k.device)
-        q_out = q if inplace else torch.empty_strided(q.shape, (ldq, D, 1), dtype=q.dtype, device=q.device)
+            k_out = k if inplace else self._like_rows(k, ldk)
+            kop = k_out.data_ptr()
+        q_out = q if inplace else self._like_rows(q, ldq)
         rot = self._rotary(frequencies, interleaved, magnitude)
-        self._run("sana_op_rotary_device", ctypes.byref(rot), dt, rows, D, self._vector(positions, "positions", "int32", rows),
-                  q.data_ptr(), ldq, heads, q_out.data_ptr(), kp, ldk, kv, None if k is None else k_out.data_ptr())
+        self._run("sana_op_rotary_device", ctypes.byref(rot), dt, rows, D,
+                  self._vector(positions, "positions", _torch().int32, rows), q.data_ptr(), ldq, heads, q_out.data_ptr(), kp,
+                  ldk, kv, kop)
         return q_out if k is None else (q_out, k_out)
 
     def _cache(self, k_cache, v_cache):
         dt = self._dtype(k_cache, "k_cache")
         shape, st = k_cache.shape, k_cache.stride()
-        if len(shape) != 4 or v_cache.shape != shape or v_cache.stride() != st or v_cache.dtype != k_cache.dtype:
-            raise ValueError("k_cache and v_cache must be [pages, page_size, kv_heads, D] of one type and layout")
-        self._dtype(v_cache, "v_cache")
+        if len(shape) != 4 or v_cache.shape != shape or v_cache.stride() != st or v_cache.dtype is not k_cache.dtype or (
+                v_cache.get_device() != self.device):
+            raise ValueError("k_cache and v_cache must be [pages, page_size, kv_heads, D] of one type, layout and device")
         if shape[3] > 1 and st[3] != 1:
             raise ValueError("a head's channels must be contiguous in the cache")
-        return sana_paged_cache(k_cache.data_ptr(), v_cache.data_ptr(), dt, shape[0], shape[1], shape[2], shape[3], st[0],
-                                st[1], st[2])
+        return sana_paged_cache(k_cache.data_ptr(), v_cache.data_ptr(), dt, *shape, st[0], st[1], st[2])
 
     def _batch(self, rows, row_start, kv_len, page_table, max_new, max_kv):
+        int32 = _torch().int32
         S = kv_len.shape[0]
-        self._dtype(page_table, "page_table", ("int32",))
-        if page_table.dim() != 2 or page_table.shape[0] != S or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
-            raise ValueError("page_table must be [sequences, pages of a sequence] with contiguous rows")
-        width = page_table.shape[1]
-        return sana_paged_batch(S, rows, max_new, max_kv, self._vector(row_start, "row_start", "int32", S + 1),
-                                self._vector(kv_len, "kv_len", "int32", S), page_table.data_ptr(),
-                                page_table.stride(0) if S > 1 else width, width)
+        shape = page_table.shape
+        if page_table.dtype is not int32 or page_table.get_device() != self.device or len(shape) != 2 or shape[0] != S or (
+                shape[1] > 1 and page_table.stride(1) != 1):
+            raise ValueError(f"page_table must be int32 [sequences, pages of a sequence] with contiguous rows on cuda:{self.device}")
+        return sana_paged_batch(S, rows, max_new, max_kv, self._vector(row_start, "row_start", int32, S + 1),
+                                self._vector(kv_len, "kv_len", int32, S), page_table.data_ptr(),
+                                page_table.stride(0) if S > 1 else shape[1], shape[1])
 
     def rotary_append_device(self, q, k, v, frequencies, k_cache, v_cache, row_start, kv_len, page_table, max_new: int,
                              interleaved: bool = False, magnitude: float = 1.0, inplace: bool = False):
@@ -537,20 +576,20 @@ class SanaCuda:
         kv_heads, D]. row_start [S + 1], kv_len [S] (the new tokens included) and page_table
         [S, pages of a sequence] are int32; frequencies None appends without turning (q is then
         returned as it is)."""
-        import torch
         cache = self._cache(k_cache, v_cache)
         rows, heads = k.shape[0], 0
-        _, ldk = self._heads(k, "k", rows, cache.kv_heads, cache.head_dim, cache.dtype)
-        _, ldv = self._heads(v, "v", rows, cache.kv_heads, cache.head_dim, cache.dtype)
+        kv, D, dt = cache.kv_heads, cache.head_dim, cache.dtype
+        _, ldk = self._heads(k, "k", rows, kv, D, dt)
+        _, ldv = self._heads(v, "v", rows, kv, D, dt)
         rot, qp, ldq, q_out, qo = None, None, 0, q, None
         if frequencies is not None:
             rot = ctypes.byref(self._rotary(frequencies, interleaved, magnitude))
             if q is not None:
-                _, ldq = self._heads(q, "q", rows, None, cache.head_dim, cache.dtype)
+                _, ldq = self._heads(q, "q", rows, None, D, dt)
                 heads, qp = q.shape[1], q.data_ptr()
-                q_out = q if inplace else torch.empty_strided(q.shape, (ldq, cache.head_dim, 1), dtype=q.dtype, device=q.device)
+                q_out = q if inplace else self._like_rows(q, ldq)
                 qo = q_out.data_ptr()
-        # the append reads each row's place from the lengths alone: any position of an int is within bounds
+        # the append reads each row's place from the lengths alone: any kv_len of the table is within bounds
         batch = self._batch(rows, row_start, kv_len, page_table, max_new, 0x7fffffff)
         self._run("sana_op_rotary_append_device", rot, ctypes.byref(batch), ctypes.byref(cache), qp, ldq, heads, qo,
                   k.data_ptr(), ldk, v.data_ptr(), ldv)
@@ -564,21 +603,25 @@ class SanaCuda:
         scale defaults to 1/sqrt(D); max_new and max_kv bound the new and the cached tokens of
         any sequence. Rows behind the last sequence keep what `out` holds (without `out`:
         anything). workspace: a uint8 tensor to use instead of one of the call's own."""
-        import torch
+        torch = _torch()
         cache = self._cache(k_cache, v_cache)
-        _, ldq = self._heads(q, "q", None, None, cache.head_dim, cache.dtype)
-        rows, heads, D = q.shape
+        D = cache.head_dim
+        _, ldq = self._heads(q, "q", None, None, D, cache.dtype)
+        rows, heads, _ = q.shape
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _, ldo = self._heads(out, "out", rows, heads, D, cache.dtype)
+            out, ldo = torch.empty_like(q, memory_format=torch.contiguous_format), heads * D
+        else:
+            _, ldo = self._heads(out, "out", rows, heads, D, cache.dtype)
         batch = self._batch(rows, row_start, kv_len, page_table, max_new, max_kv)
         bp, cp = ctypes.byref(batch), ctypes.byref(cache)
+        wp, wn = None, 0
         if workspace is None:
-            need = self.lib.sana_op_paged_attention_workspace(self.h, bp, cp, heads, window, sinks)
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+            wn = self.lib.sana_op_paged_attention_workspace(self.h, bp, cp, heads, window, sinks)
+            if wn:
+                workspace = q.new_empty(wn, dtype=torch.uint8)
+                wp = workspace.data_ptr()
         else:
-            self._vector(workspace, "workspace", "uint8")
-        wp, wn = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.shape[0])
+            wp, wn = self._vector(workspace, "workspace", torch.uint8), workspace.shape[0]
         self._run("sana_op_paged_attention_device", bp, cp, q.data_ptr(), ldq, heads, D ** -0.5 if scale is None else scale,
                   window, sinks, softcap, out.data_ptr(), ldo, wp, wn)
         return out
