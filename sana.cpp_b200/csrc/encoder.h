@@ -74,6 +74,10 @@ struct RotaryRows {
 };
 void rotary_rows(const RotaryRows& p, bool append, cudaStream_t st);
 
+struct PageDivisor {  // division by the page size as a product (pattn.cu)
+    uint32_t magic;
+    int shift;
+};
 struct PagedAttention {
     PagedBatch batch;
     PagedCache cache;
@@ -85,10 +89,11 @@ struct PagedAttention {
     void* workspace;
     int* bad;
     int* err;  // the handle's error word (bounded waits)
+    PageDivisor page_div;  // set by paged_attention
 };
 // Bytes of workspace of a call (0: none), and the call. The two take the same decisions from the
 // same sizes.
 size_t paged_attention_workspace(const PagedAttention& p, int num_sms);
-void paged_attention(const PagedAttention& p, int num_sms, cudaStream_t st);
+void paged_attention(PagedAttention p, int num_sms, cudaStream_t st);
 
 }  // namespace sana

@@ -7,6 +7,7 @@
 // pattn.cuh has the packing of rows, the key ranges and the splits.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "pattn.cuh"
 #include "tma.h"
@@ -309,7 +310,7 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
         key_range(kt, t0 + i, BN, start, end);
         const int key = start + kb + lane * box;
         if (lane >= GK / box || key >= end) return -1;
-        const int slot = key / p.cache.page_size;
+        const int slot = page_slot(p, key);
         const int page = slot < p.batch.table_width ? p.batch.table[s * p.batch.table_stride + slot] : -1;
         return page < p.cache.pages ? page : -1;
     };
@@ -321,7 +322,7 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
         if (page < 0) return;
         int start, end;
         key_range(kt, t0 + i, BN, start, end);
-        const int at = (start + kb + lane * box) % p.cache.page_size;
+        const int key = start + kb + lane * box, at = key - page_slot(p, key) * p.cache.page_size;
         const uint32_t ks = ring + (i % ST) * (2 * kGroupTile) + lane * box * 128;
         for (int slab = 0; slab < slabs; ++slab) {
             tma_load_4d(&k_map, ks + slab * (GK * 128), bar, slab * 64, at, kvh, page);
@@ -372,6 +373,18 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
     const float scale_log2 = p.scale * kLog2e;
     const float cap_in = p.softcap > 0.f ? 2.f * scale_log2 / p.softcap : 0.f, cap_out = p.softcap * kLog2e;
 
+    // A lane's part of the ldmatrix addresses: its row, and its chunk of the first 16 channels of a slab, swapped by the
+    // row; the other channels' chunks differ in bits 5 and 6 (^ 32 per 16 channels).
+    const uint32_t q_lane = swz(BM, wm * 16 + (lane & 15), lane >> 4);
+    const uint32_t k_lane = swz(GK, (lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1);
+    const uint32_t v_lane = swz(GK, lane & 15, lane >> 4);
+    constexpr bool kQRegs = DP <= 128;  // q's operands stay in registers
+    uint32_t qf[kQRegs ? DP / 16 : 1][4];
+    if constexpr (kQRegs) {
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) ldmatrix4(qf[kk], q_s + (kk >> 2) * (BM * 128) + (q_lane ^ ((kk & 3) << 5)));
+    }
+
     for (int i = 0; i < n; ++i) {
         long long next = -1;
         if (TMA) {
@@ -393,31 +406,39 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
         }
 
         const uint32_t ks = ring + (i % ST) * (2 * kGroupTile), vs = ks + kGroupTile;
-        // two chains of products per score where a warp has few scores
-        float sc[NT][4], sd[NT == 2 ? NT : 1][4];
+        // Scores; two chains of products per score where a warp has few scores.
+        float sc[NT][4], sd[2][4];
 #pragma unroll
         for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
-        if (NT == 2) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) sd[t % (NT == 2 ? 2 : 1)][0] = sd[t % (NT == 2 ? 2 : 1)][1] = sd[t % (NT == 2 ? 2 : 1)][2] = sd[t % (NT == 2 ? 2 : 1)][3] = 0.f;
-        }
+        for (int t = 0; t < 2; ++t) sd[t][0] = sd[t][1] = sd[t][2] = sd[t][3] = 0.f;
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {
-            if (kk * 16 < D) {
+            if (kk < 12 || slabs == 4) {  // channels of a slab behind D are zeros
                 uint32_t qa[4];
-                ldmatrix4(qa, q_s + swz(BM, wm * 16 + (lane & 15), kk * 2 + (lane >> 4)));
+                if constexpr (kQRegs) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) qa[x] = qf[kk][x];
+                } else {
+                    ldmatrix4(qa, q_s + (kk >> 2) * (BM * 128) + (q_lane ^ ((kk & 3) << 5)));
+                }
 #pragma unroll
                 for (int t = 0; t < NT / 2; ++t) {
                     uint32_t b[4];
-                    ldmatrix4(b, ks + swz(GK, t * 16 + (lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)));
-                    mma16816(NT == 2 && (kk & 1) ? sd[0] : sc[2 * t], qa, b[0], b[1]);
-                    mma16816(NT == 2 && (kk & 1) ? sd[NT == 2 ? 1 : 0] : sc[2 * t + 1], qa, b[2], b[3]);
+                    ldmatrix4(b, ks + (kk >> 2) * (GK * 128) + t * 2048 + (k_lane ^ ((kk & 3) << 5)));
+                    if (NT == 2 && (kk & 1)) {
+                        mma16816(sd[0], qa, b[0], b[1]);
+                        mma16816(sd[1], qa, b[2], b[3]);
+                    } else {
+                        mma16816(sc[2 * t], qa, b[0], b[1]);
+                        mma16816(sc[2 * t + 1], qa, b[2], b[3]);
+                    }
                 }
             }
         }
         if (NT == 2) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sc[0][e] += sd[0][e], sc[NT - 1][e] += sd[NT == 2 ? 1 : 0][e];
+            for (int e = 0; e < 4; ++e) sc[0][e] += sd[0][e], sc[1][e] += sd[1][e];
         }
         int start, end;
         key_range(kt, t0 + i, BN, start, end);
@@ -449,17 +470,35 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
                     if (!there(key) || !seen(start + key, pos[e >> 1], p.window, p.sinks)) sc[t][e] = kNegInf;
                 }
         }
-        float alpha[2];
+        // The maximum that the exponents are taken against moves only when a score passes it by 8 (a factor of 256):
+        // every lane looks at its own scores, and the rows' maxima are shared out among lanes when one has to.
+        float mx[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            float mx = kNegInf;
+            mx[r] = fmaxf(sc[0][2 * r], sc[0][2 * r + 1]);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) mx = fmaxf(mx, fmaxf(sc[t][2 * r], sc[t][2 * r + 1]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float m_new = fmaxf(m[r], mx), base = m_new == kNegInf ? 0.f : m_new;
-            alpha[r] = ex2_approx(m[r] - base);
-            m[r] = m_new;
+            for (int t = 1; t < NT; ++t) mx[r] = fmaxf(mx[r], fmaxf(sc[t][2 * r], sc[t][2 * r + 1]));
+        }
+        if (__any_sync(0xffffffffu, mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f)) {  // (-inf + 8 is passed by any score)
+            float alpha[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+                const bool move = mx[r] > m[r] + 8.f;
+                alpha[r] = move ? ex2_approx(m[r] - mx[r]) : 1.f;
+                m[r] = move ? mx[r] : m[r];
+                l[r] *= alpha[r];
+            }
+#pragma unroll
+            for (int d = 0; d < DP / 8; ++d) {
+                o[d][0] *= alpha[0], o[d][1] *= alpha[0];
+                o[d][2] *= alpha[1], o[d][3] *= alpha[1];
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const float base = m[r] == kNegInf ? 0.f : m[r];
             float sum = 0.f;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
@@ -467,36 +506,32 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
                 sc[t][2 * r + 1] = ex2_approx(sc[t][2 * r + 1] - base);
                 sum += sc[t][2 * r] + sc[t][2 * r + 1];
             }
-            l[r] = fmaf(l[r], alpha[r], sum);
-        }
-        if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-            for (int d = 0; d < DP / 8; ++d) {
-                o[d][0] *= alpha[0], o[d][1] *= alpha[0];
-                o[d][2] *= alpha[1], o[d][3] *= alpha[1];
-            }
+            l[r] += sum;
         }
         bool bad = false;
+        auto values = [&](auto clean) {
 #pragma unroll
-        for (int t = 0; t < NT / 2; ++t) {
-            const uint32_t pa[4] = {pack_bf2(sc[2 * t][0], sc[2 * t][1]), pack_bf2(sc[2 * t][2], sc[2 * t][3]),
-                                    pack_bf2(sc[2 * t + 1][0], sc[2 * t + 1][1]),
-                                    pack_bf2(sc[2 * t + 1][2], sc[2 * t + 1][3])};
-            const int row = t * 16 + (lane & 15);
+            for (int t = 0; t < NT / 2; ++t) {
+                const uint32_t pa[4] = {pack_bf2(sc[2 * t][0], sc[2 * t][1]), pack_bf2(sc[2 * t][2], sc[2 * t][3]),
+                                        pack_bf2(sc[2 * t + 1][0], sc[2 * t + 1][1]),
+                                        pack_bf2(sc[2 * t + 1][2], sc[2 * t + 1][3])};
 #pragma unroll
-            for (int d = 0; d < DP / 16; ++d) {
-                if (d * 16 < D) {
-                    uint32_t b[4];
-                    ldmatrix4_t(b, vs + swz(GK, row, d * 2 + (lane >> 4)));
-                    if (!whole) {  // 0 * v must be 0 for the rows that do not see v
+                for (int d = 0; d < DP / 16; ++d) {
+                    if (d < 12 || slabs == 4) {
+                        uint32_t b[4];
+                        ldmatrix4_t(b, vs + (d >> 2) * (GK * 128) + t * 2048 + (v_lane ^ ((d & 3) << 5)));
+                        if constexpr (decltype(clean)::value) {  // 0 * v must be 0 for the rows that do not see v
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) b[x] = finite2(b[x], bad);
+                            for (int x = 0; x < 4; ++x) b[x] = finite2(b[x], bad);
+                        }
+                        mma16816(o[2 * d], pa, b[0], b[1]);
+                        mma16816(o[2 * d + 1], pa, b[2], b[3]);
                     }
-                    mma16816(o[2 * d], pa, b[0], b[1]);
-                    mma16816(o[2 * d + 1], pa, b[2], b[3]);
                 }
             }
-        }
+        };
+        if (whole) values(std::false_type{});
+        else values(std::true_type{});
         if (!whole && __any_sync(0xffffffffu, bad)) {
             // what finite2 took out, given back to the rows that see it
             for (int key = 0; key < GK; ++key) {
@@ -649,10 +684,6 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
 }
 
 // --- plan and launch ----------------------------------------------------------------------------
-#ifndef SPLITW
-#define SPLITW 16
-#define SPLITT 2
-#endif
 enum Kind { kSimt, kMma, kTc };
 
 // The tcgen05 kernel's 128-row tiles take over from the mma.sync kernel's 64-row ones above this
@@ -699,9 +730,11 @@ Args plan(const PagedAttention& p, Kind kind, int num_sms) {
     const int tiles = ceil_div(span, a.BN) + (p.window > 0 ? (a.align > 1 ? 2 : 1) : 0);
     const long long base = static_cast<long long>(p.batch.S) * p.cache.kv_heads * a.row_tiles;
     // One sequence: one wave of equal blocks. Several: their lengths differ and only the longest is
-    // known here, so blocks of a few waves' size even them out.
-    const long long want = static_cast<long long>(num_sms) * resident * (p.batch.S == 1 || kind == kTc ? 1 : SPLITW);
-    const long long splits = std::max<long long>(1, std::min<long long>(want / std::max<long long>(base, 1), tiles / SPLITT));
+    // known here, so the blocks are cut to a sixteenth of a wave's share and even out (64 sequences
+    // of 100 to 16000 tokens: 4, 8, 16 and 32 waves 314, 299, 305 and 340 us). A split of fewer than
+    // eight tiles gains less than the join and its workspace cost a caller.
+    const long long want = static_cast<long long>(num_sms) * resident * (p.batch.S == 1 || kind == kTc ? 1 : 16);
+    const long long splits = std::max<long long>(1, std::min<long long>(want / std::max<long long>(base, 1), tiles / 8));
     a.split_tiles = std::max(1, ceil_div(tiles, splits));
     a.splits = ceil_div(tiles, a.split_tiles);
     return a;
@@ -759,6 +792,15 @@ void launch_simt(const Args& a, dim3 grid, cudaStream_t st) {
 
 }  // namespace
 
+// With l = ceil(log2 d): x / d = (mulhi(x, 2^(32+l) / d - 2^32 + 1) + x) >> l for x < 2^31 / 2 and any d >= 1, since the
+// magic number exceeds 2^32 (2^l / d - 1) by at most 1 and x / 2^32 < 1 / (2 d) of a step is left.
+PageDivisor page_divisor(int d) {
+    PageDivisor v{0, 0};
+    while ((1LL << v.shift) < d) ++v.shift;
+    v.magic = static_cast<uint32_t>(((1ULL << 32) * ((1ULL << v.shift) - static_cast<unsigned>(d))) / static_cast<unsigned>(d) + 1);
+    return v;
+}
+
 // Boxes are whole groups of eight rows, which the swizzle needs. A tensor map's strides end at 2^40 bytes; a stride of 0
 // (other than of a size 1) is not encoded.
 int copy_box(const PagedCache& c, int keys) {
@@ -795,7 +837,8 @@ size_t paged_attention_workspace(const PagedAttention& p, int num_sms) {
     return n;
 }
 
-void paged_attention(const PagedAttention& p, int num_sms, cudaStream_t st) {
+void paged_attention(PagedAttention p, int num_sms, cudaStream_t st) {
+    p.page_div = page_divisor(p.cache.page_size);
     if (p.batch.S == 0 || p.batch.rows == 0 || p.batch.max_new == 0) return;
     const bool mma = cache_fits_mma(p.cache) && (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 &&
                      (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.ldq % 8 == 0 && p.ldo % 8 == 0;

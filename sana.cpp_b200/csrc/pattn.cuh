@@ -98,17 +98,20 @@ __device__ __forceinline__ bool seen(int j, int pos, int window, int sinks) {
     return j <= pos && (window <= 0 || j > pos - window || j < sinks);
 }
 
+PageDivisor page_divisor(int page_size);
+__device__ __forceinline__ int page_slot(const PagedAttention& p, int j) {  // j / page_size, 0 <= j < 2^30
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(j), p.page_div.magic) + static_cast<uint32_t>(j)) >> p.page_div.shift);
+}
+
 // Element offset of key j of sequence s in the cache (head 0), -1 if its page is not in the pool.
 __device__ __forceinline__ long long key_offset(const PagedAttention& p, int s, int j) {
-    const unsigned slot = static_cast<unsigned>(j) / static_cast<unsigned>(p.cache.page_size);
-    const int page = slot < static_cast<unsigned>(p.batch.table_width)
-                         ? p.batch.table[s * p.batch.table_stride + slot]
-                         : -1;
+    const int slot = page_slot(p, j);
+    const int page = slot < p.batch.table_width ? p.batch.table[s * p.batch.table_stride + slot] : -1;
     if (page < 0 || page >= p.cache.pages) {
         record_bad(p.bad, kBadPage);
         return -1;
     }
-    return page * p.cache.page_stride + static_cast<long long>(j - static_cast<int>(slot) * p.cache.page_size) * p.cache.token_stride;
+    return page * p.cache.page_stride + static_cast<long long>(j - slot * p.cache.page_size) * p.cache.token_stride;
 }
 
 // Whether the page of any of the keys [lo, hi) is not in the pool; the block's threads share out the pages.

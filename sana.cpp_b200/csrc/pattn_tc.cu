@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 const int key = start + pt * box;
                 int page = -1, at = 0;
                 if (pt < boxes && key < end) {
-                    const int slot = key / p.cache.page_size;
+                    const int slot = page_slot(p, key);
                     page = slot < p.batch.table_width ? p.batch.table[s * p.batch.table_stride + slot] : -1;
                     if (page >= p.cache.pages) page = -1;
                     at = key - slot * p.cache.page_size;
