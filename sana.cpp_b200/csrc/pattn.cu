@@ -713,7 +713,7 @@ Args plan(const PagedAttention& p, Kind kind, int num_sms) {
         resident = 2;
     } else if (kind == kTc) {
         a.BM = tc_rows(p.cache.D);
-        a.BN = tc_keys(p.cache.D);
+        a.BN = tc_keys();
         a.align = std::max(1, copy_box(p.cache, a.BN));
         resident = 1;
     } else {
@@ -813,9 +813,21 @@ int copy_box(const PagedCache& c, int keys) {
     return c.page_size % 8 == 0 && keys % c.page_size == 0 ? c.page_size : 0;
 }
 
+namespace {
+cuuint64_t map_stride(long long elements) { return static_cast<cuuint64_t>(elements > 8 ? elements * 2 : 16); }
+}  // namespace
+CUtensorMap pool_map_slabs(const PagedCache& c, const void* base, int box) {
+    CUtensorMap m;
+    const cuuint64_t dims[5] = {64, static_cast<cuuint64_t>(c.page_size), static_cast<cuuint64_t>(c.D / 64),
+                                static_cast<cuuint64_t>(c.kv_heads), static_cast<cuuint64_t>(c.pages)};
+    const cuuint64_t strides[4] = {map_stride(c.token_stride), 128, map_stride(c.head_stride), map_stride(c.page_stride)};
+    const cuuint32_t b[5] = {64, static_cast<cuuint32_t>(box), static_cast<cuuint32_t>(c.D / 64), 1, 1};
+    tma_encode_tiled(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, base, dims, strides, b, CU_TENSOR_MAP_SWIZZLE_128B);
+    return m;
+}
 CUtensorMap pool_map(const PagedCache& c, const void* base, int box) {
     CUtensorMap m;
-    auto stride = [](long long elements) { return static_cast<cuuint64_t>(elements > 8 ? elements * 2 : 16); };
+    auto stride = map_stride;
     const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.D), static_cast<cuuint64_t>(c.page_size),
                                 static_cast<cuuint64_t>(c.kv_heads), static_cast<cuuint64_t>(c.pages)};
     const cuuint64_t strides[3] = {stride(c.token_stride), stride(c.head_stride), stride(c.page_stride)};

@@ -146,9 +146,13 @@ int copy_box(const PagedCache& c, int keys);
 // the 128-byte swizzle.
 CUtensorMap pool_map(const PagedCache& c, const void* base, int box);
 
-// pattn_tc.cu: packed rows and keys of a block's tile for a head size, and the launch.
+// The same of all channels at once, [pages][kv_heads][slabs][page_size][64] (head sizes that are multiples
+// of 64).
+CUtensorMap pool_map_slabs(const PagedCache& c, const void* base, int box);
+
+// pattn_tc.cu: packed rows and keys of a block's tile, and the launch.
 int tc_rows(int D);
-int tc_keys(int D);
+int tc_keys();
 void launch_tc(const Args& a, dim3 grid, cudaStream_t st);
 
 }  // namespace pattn

@@ -3,13 +3,14 @@
 // ranges and splits, pattn.cu the other kernels and the choice between them.
 //
 // One block holds 256 packed rows as two tiles of 128 (one tile for head sizes above 128, whose
-// output fills the tensor memory, and where fewer rows are left) and walks the key tiles:
+// output fills the tensor memory, and where fewer rows are left) and walks the key tiles of 128:
 //   S = Q K^T into tensor memory; a thread per row reads its scores, masks them where the tile is
 //   not seen whole, and writes P = 2^(s - m) as bf16 over S; O += P V with P from tensor memory.
-// The unit of work is one S tile: unit u uses slot u & 1 of two. With two row tiles, u is row tile
-// u & 1 at key tile u >> 1; with one, key tile u. The issuing thread runs S(0), S(1), then PV(u),
-// S(u + 2) for every u, so that the tensor cores have the other slot's products while the softmax
-// of one is under way, and S(u + 2) may overwrite P(u) since products run in order.
+// S has two slots. With two row tiles each has its own; with one, key tiles take them in turn. The
+// issuing warp runs S(0), S(1), then PV(u), S(u + 2) for every S tile u, so that the tensor cores
+// have the other slot's products while the softmax of one is under way, and S(u + 2) may overwrite
+// P(u) since products run in order. (Two threads per row, or an issuing warp per slot, let both
+// slots fall into step, all products waiting for all softmaxes: 277 us where this took 186.)
 //
 // The running maximum is a reference that moves only when a row's maximum passes it by 8 (a
 // factor of 256): the output is rescaled in tensor memory then, by the row's own threads, and
@@ -18,10 +19,12 @@
 //
 // Keys and values come into the 128-byte-swizzled layout of the matrix descriptors: slabs of 64
 // channels, 128-byte rows, chunk c of row r at c ^ (r & 7); K and Q are K-major operands, V is
-// MN-major (its channels contiguous). Where pages divide a tile or tiles divide a page, one tensor
-// copy (TMA) per page and slab brings them; other page sizes end anywhere inside a tile and come by
-// 16-byte cp.async. Both by 64 producer threads. Measured on 2048 tokens after 8192 (16 heads of 128
-// over 4): 281 us with cp.async alone, whose issue bound the kernel.
+// MN-major (its channels contiguous). K and V have a ring each, filled by warps of their own, of
+// whole tiles, or for head sizes above 128, where a tile has 64 KB, of quarters (64 channels of K,
+// 32 keys of V). Where pages divide a tile or tiles divide a page, tensor copies (TMA) bring them:
+// K one per page and slab; V one per page, all slabs, where the head size is a multiple of 64. V's
+// keys stand in blocks of what one copy brings, [block][slab][key], which its descriptors follow.
+// Other page sizes end anywhere inside a tile and come by 16-byte cp.async.
 #include <type_traits>
 
 #include "pattn.cuh"
@@ -35,26 +38,31 @@ namespace {
 using namespace tc;
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kSoftmaxWarps = 8, kProducerWarps = 2;
-constexpr int kThreads = (kSoftmaxWarps + kProducerWarps + 1) * 32;
-constexpr int kMmaWarp = kSoftmaxWarps + kProducerWarps;
-constexpr int kProducers = kProducerWarps * 32;
+constexpr int kSoftmaxWarps = 8, kKeyWarp = 8, kValueWarp = 9, kMmaWarp = 11;  // (two value warps)
+constexpr int kThreads = 12 * 32;
+constexpr int kValueThreads = 64;
+constexpr int kKeys = 128;  // per key tile
 
 template <int DP>
 struct TcShape {
     static constexpr int kTiles = DP <= 128 ? 2 : 1;     // row tiles of 128
     static constexpr int kRows = 128 * kTiles;
-    static constexpr int kKeys = DP <= 128 ? 128 : 64;   // per key tile
     static constexpr int kSlabs = DP / 64;
-    static constexpr int kStages = DP == 64 ? 4 : 2;
+    static constexpr int kPieces = DP <= 128 ? 1 : 4;    // of a tile of K or V
+    static constexpr int kPieceSlabs = kSlabs / kPieces; // of K
+    static constexpr int kPieceKeys = kKeys / kPieces;   // of V
+    static constexpr int kPieceBytes = kKeys * DP * 2 / kPieces;
+    static constexpr int kKRing = DP == 64 ? 4 : DP == 128 ? 2 : 5, kVRing = DP == 64 ? 4 : DP == 128 ? 2 : 4;  // pieces
     static constexpr int kQBytes = kTiles * 128 * DP * 2;
-    static constexpr int kTileBytes = kKeys * DP * 2;    // of K or of V
-    static constexpr int kBarriers = 4 * kStages + 8 + 2;
-    static constexpr int kSmem = 1024 + kQBytes + kStages * 2 * kTileBytes + 2 * kKeys * 8 + kBarriers * 8 + 64;
+    static constexpr int kBarriers = 2 * (kKRing + kVRing) + 8 + 2;
+    // behind Q and the rings: keys' offsets [2 for K, 2 for V][kKeys] (cp.async), barriers, three words
+    static constexpr int kVRingAt = kQBytes + kKRing * kPieceBytes;
+    static constexpr int kOffs = kVRingAt + kVRing * kPieceBytes;
+    static constexpr int kBars = kOffs + 4 * kKeys * 8;
+    static constexpr int kSmem = 1024 + kBars + kBarriers * 8 + 16;
     // tensor memory columns: S slots at 0 and kKeys, O behind them
     static constexpr int kO = 2 * kKeys;
-    static constexpr int kCols = kO + kTiles * DP;
-    static_assert(kCols <= 512, "tensor memory");
+    static_assert(kO + kTiles * DP <= 512, "tensor memory");
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in) {
@@ -97,13 +105,13 @@ __device__ __forceinline__ void umma_bf16_ta(uint32_t d_tmem, uint32_t a_tmem, u
         : "memory");
 }
 // Descriptor of an MN-major operand in the 128-byte swizzle: 64 channels of a row contiguous, groups
-// of eight rows 1024 bytes apart (the stride offset), slabs of 64 channels `slab` bytes apart (the
+// of eight rows `group` bytes apart (the stride offset), slabs of 64 channels `slab` bytes apart (the
 // leading offset).
-__device__ __forceinline__ uint64_t mnmajor_sw128_desc(uint32_t smem_addr, uint32_t slab) {
+__device__ __forceinline__ uint64_t mnmajor_sw128_desc(uint32_t smem_addr, uint32_t slab, uint32_t group) {
     uint64_t d = 0;
     d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
     d |= static_cast<uint64_t>((slab >> 4) & 0x3FFFu) << 16;
-    d |= static_cast<uint64_t>(1024u >> 4) << 32;
+    d |= static_cast<uint64_t>((group >> 4) & 0x3FFFu) << 32;
     d |= static_cast<uint64_t>(1u) << 46;
     d |= static_cast<uint64_t>(2u) << 61;
     return d;
@@ -132,17 +140,17 @@ __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* err) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, kTimeout));
 }
-// Barrier of the producer warps, with the conjunction of what they bring.
-__device__ __forceinline__ bool producers_all(bool ok) {
+// Barrier `id` of `threads` threads, with the conjunction of what they bring.
+__device__ __forceinline__ bool meet_all(int id, int threads, bool ok) {
     int all;
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.and.pred q, 1, %2, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.and.pred q, %2, %3, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
         : "=r"(all)
-        : "r"(ok ? 1 : 0), "n"(kProducers)
+        : "r"(ok ? 1 : 0), "r"(id), "r"(threads)
         : "memory");
     return all != 0;
 }
-
+__device__ __forceinline__ bool value_warps(bool ok) { return meet_all(1, kValueThreads, ok); }
 // Bit i: the row at position pos sees key j0 + i, below `end`.
 __device__ __forceinline__ uint32_t low_bits(int n) {  // the n lowest bits, n of any sign and size
     return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
@@ -153,18 +161,51 @@ __device__ __forceinline__ uint32_t seen_bits(int j0, int end, int pos, int wind
     return bits & low_bits(end - j0);
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
+// Tensor copies: the page of box `b` of `boxes` of a key tile, -1 for none (behind the range, or a bad page).
+__device__ __forceinline__ int box_page(const PagedAttention& p, int s, const KeyTiles& kt, int tile, int b, int boxes, int box) {
+    int start, end;
+    key_range(kt, tile, kKeys, start, end);
+    const int key = start + b * box;
+    if (b >= boxes || key >= end) return -1;
+    const int slot = page_slot(p, key);
+    const int page = slot < p.batch.table_width ? p.batch.table[s * p.batch.table_stride + slot] : -1;
+    return page < p.cache.pages ? page : -1;
 }
+// cp.async: offsets of the keys t, t + THREADS, .. of a key tile, and the copy of `keys` keys and `count` slabs from
+// `slab` into [slab][key] at dst.
+template <int THREADS>
+__device__ __forceinline__ void tile_offsets(const PagedAttention& p, int s, const KeyTiles& kt, int tile, int t,
+                                             long long (&o)[kKeys / THREADS]) {
+    int start, end;
+    key_range(kt, tile, kKeys, start, end);
+#pragma unroll
+    for (int x = 0; x < kKeys / THREADS; ++x) {
+        const int key = start + t + x * THREADS;
+        o[x] = key < end ? key_offset(p, s, key) : -1;
+    }
+}
+template <int THREADS>
+__device__ __forceinline__ void copy_rows(uint32_t dst, const bf16* src, const long long* of, int keys, int slab, int count, int D,
+                                          int t) {
+    for (int x = 0; x < count; ++x) {
+        const int d = (slab + x) * 64 + (t & 7) * 8;
+#pragma unroll 4
+        for (int key = t >> 3; key < keys; key += THREADS / 8) {
+            const long long off = of[key];
+            const bool in = off >= 0 && d < D;
+            cp_async16(dst + x * (keys * 128) + key * 128 + (((t & 7) ^ (key & 7)) << 4), in ? src + off + d : src, in);
+        }
+    }
+}
+
 template <int DP, bool CAP>
 __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_constant__ Args a,
                                                                const __grid_constant__ CUtensorMap k_map,
-                                                               const __grid_constant__ CUtensorMap v_map, const int box) {
+                                                               const __grid_constant__ CUtensorMap v_map, const int k_box,
+                                                               const int v_box) {
     using Sh = TcShape<DP>;
-    constexpr int BN = Sh::kKeys, ST = Sh::kStages;
-    constexpr int kEarly = BN == 128 ? 3 : 1;  // quarters (halves) of a tile's P handed over before the rest
+    constexpr int BN = kKeys, NK = Sh::kKRing, NV = Sh::kVRing, kPieces = Sh::kPieces, kSlabs = Sh::kSlabs;
+    constexpr int kEarly = 3;  // quarters of a tile's P handed over before the rest
     extern __shared__ unsigned char smem_raw[];
     const PagedAttention& p = a.p;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = p.cache.D;
@@ -179,45 +220,45 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     if (n <= 0) return;
     const bool partial = kt.n > a.split_tiles;
     const bool pair = Sh::kTiles == 2 && rr0 + 128 < n_rows;
-    const int units = pair ? 2 * n : n;
+    const bool tma = k_box > 0;
 
     // shared memory, 1024-byte aligned for the swizzle
-    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    unsigned char* sm = smem_raw + (base - smem_u32(smem_raw));
-    const uint32_t q_s = base, kv_s = base + Sh::kQBytes;
-    constexpr int kOffs = Sh::kQBytes + ST * 2 * Sh::kTileBytes;
-    long long* offs = reinterpret_cast<long long*>(sm + kOffs);  // [2][BN]
-    const uint32_t bars = base + kOffs + 2 * BN * 8;
+    const uint32_t q_s = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    unsigned char* sm = smem_raw + (q_s - smem_u32(smem_raw));
+    const uint32_t k_ring = q_s + Sh::kQBytes, v_ring = q_s + Sh::kVRingAt;
+    const uint32_t bars = q_s + Sh::kBars;
     auto k_full = [&](int i) { return bars + 8u * i; };
-    auto v_full = [&](int i) { return bars + 8u * (ST + i); };
-    auto k_empty = [&](int i) { return bars + 8u * (2 * ST + i); };
-    auto v_empty = [&](int i) { return bars + 8u * (3 * ST + i); };
-    auto s_full = [&](int i) { return bars + 8u * (4 * ST + i); };
-    auto p_full = [&](int i) { return bars + 8u * (4 * ST + 2 + i); };
-    auto pv_done = [&](int i) { return bars + 8u * (4 * ST + 4 + i); };
-    auto p_half = [&](int i) { return bars + 8u * (4 * ST + 6 + i); };
-    const uint32_t drained = bars + 8u * (4 * ST + 8), v_raw = drained + 8u;
-    int* words = reinterpret_cast<int*>(sm + kOffs + 2 * BN * 8 + Sh::kBarriers * 8);  // [0] tensor memory, [1] bad page, [2] not finite
+    auto k_empty = [&](int i) { return bars + 8u * (NK + i); };
+    auto v_full = [&](int i) { return bars + 8u * (2 * NK + i); };
+    auto v_empty = [&](int i) { return bars + 8u * (2 * NK + NV + i); };
+    auto s_full = [&](int i) { return bars + 8u * (2 * NK + 2 * NV + i); };
+    auto p_early = [&](int i) { return bars + 8u * (2 * NK + 2 * NV + 2 + i); };
+    auto p_full = [&](int i) { return bars + 8u * (2 * NK + 2 * NV + 4 + i); };
+    auto pv_done = [&](int i) { return bars + 8u * (2 * NK + 2 * NV + 6 + i); };
+    const uint32_t drained = bars + 8u * (2 * NK + 2 * NV + 8), v_raw = drained + 8u;
+    int* words = reinterpret_cast<int*>(sm + Sh::kBars + Sh::kBarriers * 8);  // [0] tensor memory, [1] bad page, [2] not finite
 
     if (warp == kMmaWarp) {
         tmem_alloc(smem_u32(words), 512);
         tmem_relinquish();
     }
     if (tid == 0) {
-        for (int i = 0; i < ST; ++i) {
-            mbar_init(k_full(i), kProducers);
-            mbar_init(v_full(i), kProducers);
+        for (int i = 0; i < NK; ++i) {
+            mbar_init(k_full(i), tma ? 1 : 32);
             mbar_init(k_empty(i), 1);
+        }
+        for (int i = 0; i < NV; ++i) {
+            mbar_init(v_full(i), tma ? 1 : kValueThreads);
             mbar_init(v_empty(i), 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(s_full(i), 1);
+            mbar_init(p_early(i), 4);
             mbar_init(p_full(i), 4);
-            mbar_init(p_half(i), 4);
             mbar_init(pv_done(i), 1);
         }
         mbar_init(drained, 1);
-        mbar_init(v_raw, kProducers);
+        mbar_init(v_raw, 1);
         fence_barrier_init();
         words[1] = 0;
         words[2] = 0;
@@ -246,32 +287,30 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(words);
     const bool bad_page = *reinterpret_cast<volatile int*>(words + 1) != 0;
 
-    float m = -INFINITY, l = 0.f;  // of a softmax thread's row
-    const int wg = warp >> 2;      // softmax: row tile; tensor memory lanes 32 (warp & 3) ..
-    const int my_rr = rr0 + wg * 128 + (tid & 127);
-    const int my_pos = warp < kSoftmaxWarps && my_rr < n_rows ? sq.past + my_rr / a.G : -1;
+    // a softmax thread's row tile and row; tensor memory lanes 32 (warp & 3) ..
+    const int rt = warp >> 2, my_rr = rr0 + rt * 128 + (tid & 127);
+    const int my_pos = my_rr < n_rows ? sq.past + my_rr / a.G : -1;
     const uint32_t my_lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);
-    const bool softmax_on = warp < kSoftmaxWarps && (wg == 0 || pair);
+    const bool softmax_on = warp < kSoftmaxWarps && (rt == 0 || pair);
+    float m = -INFINITY, l = 0.f;
 
     if (warp < kSoftmaxWarps) {
         if (softmax_on) {
             const float scale_log2 = p.scale * kLog2e;
             const float cap_in = CAP ? 2.f * scale_log2 / p.softcap : 0.f, cap_out = p.softcap * kLog2e;
             // positions of this row tile
-            const int last = min(n_rows, rr0 + wg * 128 + 128) - 1;
             KeyTiles mine = kt;
-            mine.pmin = sq.past + (rr0 + wg * 128) / a.G;
-            mine.pmax = sq.past + last / a.G;
-            const uint32_t o_t = my_lanes + Sh::kO + wg * DP;
-            const int step = pair ? 2 : 1;
-            for (int u = pair ? wg : 0; u < units; u += step) {
-                const int slot = u & 1, kv = pair ? u >> 1 : u;
+            mine.pmin = sq.past + (rr0 + rt * 128) / a.G;
+            mine.pmax = sq.past + (min(n_rows, rr0 + rt * 128 + 128) - 1) / a.G;
+            const uint32_t o_t = my_lanes + Sh::kO + rt * DP;
+            for (int j = 0; j < n; ++j) {
+                const int slot = pair ? rt : j & 1, turn = pair ? j : j >> 1;
                 int start, end;
-                key_range(kt, t0 + kv, BN, start, end);
+                key_range(kt, t0 + j, BN, start, end);
                 const bool whole = end - start == BN && !bad_page && all_seen(mine, start, end, p.window, p.sinks);
-                if (!warp_wait(s_full(slot), (u >> 1) & 1, p.err)) break;
-                tc_fence_after();
                 const uint32_t s_t = my_lanes + slot * BN;
+                if (!warp_wait(s_full(slot), turn & 1, p.err)) break;
+                tc_fence_after();
                 // the whole row in registers: the loads are in flight together
                 uint32_t x[BN];
 #pragma unroll
@@ -280,10 +319,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 if (!whole) {
 #pragma unroll
                     for (int c = 0; c < BN / 32; ++c) {
-                        uint32_t bits = seen_bits(start + c * 32, end, my_pos, p.window, p.sinks);
+                        const int j0 = start + c * 32;
+                        uint32_t bits = seen_bits(j0, end, my_pos, p.window, p.sinks);
                         if (bad_page) {
                             for (int i = 0; i < 32; ++i)
-                                if ((bits >> i & 1u) && key_offset(p, s, start + c * 32 + i) < 0) bits &= ~(1u << i);
+                                if ((bits >> i & 1u) && key_offset(p, s, j0 + i) < 0) bits &= ~(1u << i);
                         }
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
@@ -292,67 +332,61 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 }
                 float mx4[4];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) mx4[c] = __uint_as_float(x[c]);
+                for (int c = 0; c < 4; ++c) mx4[c] = fmaxf(__uint_as_float(x[c]), __uint_as_float(x[4 + c]));
 #pragma unroll
-                for (int i = 4; i + 8 <= BN; i += 8)
+                for (int i = 8; i < BN; i += 4)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        mx4[c] = max3(mx4[c], __uint_as_float(x[i + c]), __uint_as_float(x[i + 4 + c]));
-                float mx = max3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3]));
-                mx = max3(mx, fmaxf(__uint_as_float(x[BN - 1]), __uint_as_float(x[BN - 2])),
-                          fmaxf(__uint_as_float(x[BN - 3]), __uint_as_float(x[BN - 4])));
+                    for (int c = 0; c < 4; ++c) mx4[c] = fmaxf(mx4[c], __uint_as_float(x[i + c]));
+                float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
                 // both maps rise with the score (scale > 0), so the maximum is mapped alone
                 if (mx != -INFINITY) mx = CAP ? soft_cap_log2(mx, cap_in, cap_out) : mx * scale_log2;
-                const bool move = mx > m + 8.f || (m == -INFINITY && mx > -INFINITY);
-                float alpha = 1.f;
-                if (move) {
-                    alpha = ex2_approx(m - mx);
-                    m = mx;
+                const bool move = mx > m + 8.f;  // (-inf + 8 is passed by any score)
+                if (__any_sync(0xffffffffu, move)) {
+                    const float alpha = move ? ex2_approx(m - mx) : 1.f;
+                    m = move ? mx : m;
                     l *= alpha;
-                }
-                if (kv > 0 && __any_sync(0xffffffffu, move)) {  // O holds sums against the old reference
-                    const int before = u - step;
-                    if (!warp_wait(pv_done(before & 1), (before >> 1) & 1, p.err)) break;
-                    tc_fence_after();
-                    for (int c = 0; c < D; c += 16) {
-                        uint32_t r[16];
-                        tmem_ld16(o_t + c, r);
-                        tmem_wait_ld();
+                    if (j > 0) {  // O holds sums against the old reference
+                        const int slot0 = pair ? rt : (j - 1) & 1, turn0 = pair ? j - 1 : (j - 1) >> 1;
+                        if (!warp_wait(pv_done(slot0), turn0 & 1, p.err)) break;
+                        tc_fence_after();
+                        for (int c = 0; c < D; c += 16) {
+                            uint32_t r[16];
+                            tmem_ld16(o_t + c, r);
+                            tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
-                        tmem_st16(o_t + c, r);
+                            for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+                            tmem_st16(o_t + c, r);
+                        }
                     }
                 }
                 const float ref = m == -INFINITY ? 0.f : m;
+                const uint64_t k2 = f2_make(scale_log2, scale_log2), r2 = f2_make(-ref, -ref);
                 uint64_t sum[2] = {0, 0};
-                {
-                    const uint64_t k2 = f2_make(scale_log2, scale_log2), r2 = f2_make(-ref, -ref);
 #pragma unroll
-                    for (int c = 0; c < BN / 32; ++c) {
-                        uint32_t pk[16];
+                for (int c = 0; c < BN / 32; ++c) {
+                    uint32_t pk[16];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float x0 = __uint_as_float(x[c * 32 + 2 * i]), x1 = __uint_as_float(x[c * 32 + 2 * i + 1]);
-                            uint64_t e;
-                            if constexpr (CAP) {
-                                e = add2(f2_make(soft_cap_log2(x0, cap_in, cap_out), soft_cap_log2(x1, cap_in, cap_out)), r2);
-                                const float2 v = f2_split(e);  // the cap maps what is masked to a number: it stays masked
-                                if (!whole) e = f2_make(x0 == -INFINITY ? x0 : v.x, x1 == -INFINITY ? x1 : v.y);
-                            } else {
-                                e = fma2(f2_make(x0, x1), k2, r2);
-                            }
-                            const float2 v = f2_split(e);
-                            const float e0 = ex2_approx(v.x), e1 = ex2_approx(v.y);
-                            sum[i & 1] = add2(sum[i & 1], f2_make(e0, e1));
-                            pk[i] = pack_bf2(e0, e1);
+                    for (int i = 0; i < 16; ++i) {
+                        const float x0 = __uint_as_float(x[c * 32 + 2 * i]), x1 = __uint_as_float(x[c * 32 + 2 * i + 1]);
+                        uint64_t e;
+                        if constexpr (CAP) {
+                            e = add2(f2_make(soft_cap_log2(x0, cap_in, cap_out), soft_cap_log2(x1, cap_in, cap_out)), r2);
+                            const float2 v = f2_split(e);  // the cap maps what is masked to a number: it stays masked
+                            if (!whole) e = f2_make(x0 == -INFINITY ? x0 : v.x, x1 == -INFINITY ? x1 : v.y);
+                        } else {
+                            e = fma2(f2_make(x0, x1), k2, r2);
                         }
-                        tmem_st16(s_t + c * 16, pk);  // over the scores, which this row has read
-                        if (c == kEarly - 1) {        // the products over these keys may start
-                            tmem_wait_st();
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(p_half(slot));
-                        }
+                        const float2 v = f2_split(e);
+                        const float e0 = ex2_approx(v.x), e1 = ex2_approx(v.y);
+                        sum[i & 1] = add2(sum[i & 1], f2_make(e0, e1));
+                        pk[i] = pack_bf2(e0, e1);
+                    }
+                    tmem_st16(s_t + c * 16, pk);  // over the scores, which this row has read
+                    if (c == kEarly - 1) {        // the products over these keys may start
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(p_early(slot));
                     }
                 }
                 const float2 total = f2_split(add2(sum[0], sum[1]));
@@ -363,47 +397,77 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 if (lane == 0) mbar_arrive(p_full(slot));
             }
         }
-    } else if (warp < kMmaWarp) {
-        const int pt = tid - kSoftmaxWarps * 32;
-        const bf16* kc = static_cast<const bf16*>(p.cache.k) + kvh * p.cache.head_stride;
-        const bf16* vc = static_cast<const bf16*>(p.cache.v) + kvh * p.cache.head_stride;
+    } else if (warp == kKeyWarp) {
         const int slabs = (D + 63) / 64;
-        // this thread's keys of tile i: pt, pt + 64
-        constexpr int kOwn = BN / kProducers;
-        static_assert(BN % kProducers == 0, "keys per producer");
-        auto offsets = [&](int i, long long (&o)[kOwn]) {
-            int start, end;
-            key_range(kt, t0 + i, BN, start, end);
-#pragma unroll
-            for (int x = 0; x < kOwn; ++x) {
-                const int j = start + pt + x * kProducers;
-                o[x] = j < end ? key_offset(p, s, j) : -1;
-            }
-        };
-        constexpr int kRowsPerPass = kProducers / 8;
-        auto chunk_at = [&](int slab, int key) { return slab * (BN * 128) + key * 128 + (((pt & 7) ^ (key & 7)) << 4); };
-        auto load = [&](uint32_t dst, const bf16* src, const long long* of) {
-            for (int slab = 0; slab < slabs; ++slab) {
-                const int d = slab * 64 + (pt & 7) * 8;
-#pragma unroll
-                for (int x = 0; x < BN / kRowsPerPass; ++x) {
-                    const int key = x * kRowsPerPass + (pt >> 3);
-                    const long long off = of[key];
-                    const bool in = off >= 0 && d < D;
-                    cp_async16(dst + chunk_at(slab, key), in ? src + off + d : src, in);
+        auto piece_slabs = [&](int pc) { return min(Sh::kPieceSlabs, max(0, slabs - pc * Sh::kPieceSlabs)); };
+        bool ok = true;
+        if (tma) {
+            // lane b < BN / k_box holds the page of box b, `k_box` keys of one page; one elected thread copies
+            const int boxes = BN / k_box;
+            auto page_of = [&](int j) { return box_page(p, s, kt, t0 + j, lane, boxes, k_box); };
+            const bool leader = elect_one();
+            int next = page_of(0), issued = 0;
+            for (int j = 0; j < n && ok; ++j) {
+                const int page = next;
+                if (j + 1 < n) next = page_of(j + 1);
+                int start, end;
+                key_range(kt, t0 + j, BN, start, end);
+                const int at = start + lane * k_box - page_slot(p, start + lane * k_box) * p.cache.page_size;
+                const uint32_t box_bytes = static_cast<uint32_t>(__popc(__ballot_sync(0xffffffffu, page >= 0))) * k_box * 128;
+                for (int pc = 0; pc < kPieces && ok; ++pc) {
+                    const int g = j * kPieces + pc, slot = g % NK, count = piece_slabs(pc);
+                    ok = warp_wait(k_empty(slot), ((g / NK) & 1) ^ 1, p.err);
+                    if (!ok) continue;
+                    if (leader) mbar_arrive_expect_tx(k_full(slot), box_bytes * count);
+                    __syncwarp();
+                    const uint32_t dst = k_ring + slot * Sh::kPieceBytes;
+                    for (int b = 0; b < boxes; ++b) {
+                        const int pg = __shfl_sync(0xffffffffu, page, b), row = __shfl_sync(0xffffffffu, at, b);
+                        if (leader && pg >= 0)
+                            for (int x = 0; x < count; ++x)
+                                tma_load_4d(&k_map, dst + x * (BN * 128) + b * k_box * 128, k_full(slot),
+                                            (pc * Sh::kPieceSlabs + x) * 64, row, kvh, pg);
+                    }
+                    issued = g + 1;
                 }
             }
-        };
+            if (!ok)  // what is on its way lands (or is waited for as long as a wait may last) before the block ends
+                for (int g = issued > NK ? issued - NK : 0; g < issued; ++g) mbar_wait_quiet(k_full(g % NK), (g / NK) & 1);
+        } else {
+            const bf16* kc = static_cast<const bf16*>(p.cache.k) + kvh * p.cache.head_stride;
+            long long* offs = reinterpret_cast<long long*>(sm + Sh::kOffs);
+            long long next[4];
+            tile_offsets<32>(p, s, kt, t0, lane, next);
+            for (int j = 0; j < n && ok; ++j) {
+                long long* of = offs + (j & 1) * BN;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) of[lane + x * 32] = next[x];
+                __syncwarp();
+                if (j + 1 < n) tile_offsets<32>(p, s, kt, t0 + j + 1, lane, next);
+                for (int pc = 0; pc < kPieces && ok; ++pc) {
+                    const int g = j * kPieces + pc, slot = g % NK;
+                    ok = warp_wait(k_empty(slot), ((g / NK) & 1) ^ 1, p.err);
+                    if (!ok) continue;
+                    copy_rows<32>(k_ring + slot * Sh::kPieceBytes, kc, of, BN, pc * Sh::kPieceSlabs, piece_slabs(pc), D, lane);
+                    cp_async_arrive(k_full(slot));
+                }
+            }
+            cp_async_commit();
+            cp_async_wait<0>();
+        }
+    } else if (warp < kMmaWarp) {
+        const int pt = tid - kValueWarp * 32, slabs = (D + 63) / 64;
+        const int block = tma ? v_box : Sh::kPieceKeys;  // keys of a block
         // Values that are not finite, in a tile that not every row sees whole, would reach the rows that do
         // not see them as 0 * v: zeros take their place, and the rows that see them get them at the end.
         // Keys from `keys` on, and those of bad pages, are zeros outright (a tensor copy brought what lies there).
-        auto clean = [&](unsigned char* v, int start, int keys) {
+        auto clean = [&](unsigned char* v, int key0, int start, int keys) {
             for (int slab = 0; slab < slabs; ++slab) {
-#pragma unroll 4
-                for (int x = 0; x < BN / kRowsPerPass; ++x) {
-                    const int key = x * kRowsPerPass + (pt >> 3);
-                    uint4* w = reinterpret_cast<uint4*>(v + chunk_at(slab, key));
-                    if (key >= keys || (bad_page && key_offset(p, s, start + key) < 0)) {
+                for (int key = pt >> 3; key < Sh::kPieceKeys; key += kValueThreads / 8) {
+                    const int row = key & (block - 1);
+                    uint4* w = reinterpret_cast<uint4*>(v + (key - row) * (kSlabs * 128) + slab * (block * 128) + row * 128 +
+                                                        (((pt & 7) ^ (row & 7)) << 4));
+                    if (key0 + key >= keys || (bad_page && key_offset(p, s, start + key0 + key) < 0)) {
                         *w = make_uint4(0, 0, 0, 0);
                         continue;
                     }
@@ -422,160 +486,191 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 }
             }
         };
+        auto at_piece = [&](int g) { return sm + Sh::kVRingAt + (g % NV) * Sh::kPieceBytes; };
         bool ok = true;
-        if (box > 0) {
-            // Producer thread b < BN / box copies box b of a tile, `box` keys of one page. Every producer arrives once
-            // on a tile's barrier, those that copy with the bytes to come.
-            const int boxes = BN / box;
-            const uint32_t bytes = static_cast<uint32_t>(box) * 128 * slabs;
-            int issued = 0, raw = 0;
+        if (tma) {
+            // as for K, by the first value warp; the second helps to clean and keeps step, waiting for no place
+            const int boxes = BN / v_box, boxes_piece = Sh::kPieceKeys / v_box;
+            auto page_of = [&](int j) { return box_page(p, s, kt, t0 + j, lane, boxes, v_box); };
+            const bool leader = elect_one(), all_slabs = D % 64 == 0;
+            int next = page_of(0), issued = 0, raw = 0;
             bool in_flight = false;  // on v_raw
-            for (int i = 0; i < n; ++i) {
-                const int st = i % ST, use = i / ST;
+            for (int j = 0; j < n; ++j) {
+                const int page = next;
+                if (j + 1 < n) next = page_of(j + 1);
                 int start, end;
-                key_range(kt, t0 + i, BN, start, end);
-                const int key = start + pt * box;
-                int page = -1, at = 0;
-                if (pt < boxes && key < end) {
-                    const int slot = page_slot(p, key);
-                    page = slot < p.batch.table_width ? p.batch.table[s * p.batch.table_stride + slot] : -1;
-                    if (page >= p.cache.pages) page = -1;
-                    at = key - slot * p.cache.page_size;
-                }
-                auto copy = [&](const CUtensorMap* map, uint32_t dst, uint32_t bar) {
-                    if (page < 0) {
-                        mbar_arrive(bar);
-                        return;
+                key_range(kt, t0 + j, BN, start, end);
+                const int at = start + lane * v_box - page_slot(p, start + lane * v_box) * p.cache.page_size;
+                const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
+                const uint32_t box_bytes = static_cast<uint32_t>(v_box) * 128 * slabs;
+                const bool edge = end - start < BN || bad_page || !all_seen(kt, start, end, p.window, p.sinks);
+                if (warp == kValueWarp) {
+                    if (edge && leader) mbar_arrive_expect_tx(v_raw, __popc(there) * box_bytes);
+                    for (int pc = 0; pc < kPieces && ok; ++pc) {
+                        const int g = j * kPieces + pc, slot = g % NV;
+                        ok = warp_wait(v_empty(slot), ((g / NV) & 1) ^ 1, p.err);
+                        if (!ok) continue;
+                        const uint32_t bar = edge ? v_raw : v_full(slot);
+                        if (!edge && leader) {
+                            const unsigned mine = there >> (pc * boxes_piece) & ((1u << boxes_piece) - 1u);
+                            mbar_arrive_expect_tx(bar, __popc(mine) * box_bytes);
+                        }
+                        __syncwarp();
+                        uint32_t dst = v_ring + slot * Sh::kPieceBytes;
+                        for (int b = pc * boxes_piece; b < (pc + 1) * boxes_piece; ++b, dst += v_box * kSlabs * 128) {
+                            const int pg = __shfl_sync(0xffffffffu, page, b), row = __shfl_sync(0xffffffffu, at, b);
+                            if (leader && pg >= 0) {
+                                if (all_slabs) {
+                                    tma_load_5d(&v_map, dst, bar, 0, row, 0, kvh, pg);
+                                } else {
+                                    for (int x = 0; x < slabs; ++x) tma_load_4d(&v_map, dst + x * (v_box * 128), bar, x * 64, row, kvh, pg);
+                                }
+                            }
+                        }
+                        if (!edge) issued = g + 1;
                     }
-                    mbar_arrive_expect_tx(bar, bytes);
-                    for (int slab = 0; slab < slabs; ++slab)
-                        tma_load_4d(map, dst + slab * (BN * 128) + pt * box * 128, bar, slab * 64, at, kvh, page);
-                };
-                const uint32_t ks = kv_s + st * (2 * Sh::kTileBytes);
-                ok = warp_wait(k_empty(st), (use & 1) ^ 1, p.err);
-                if (!ok) break;
-                copy(&k_map, ks, k_full(st));
-                issued = i + 1;
-                ok = warp_wait(v_empty(st), (use & 1) ^ 1, p.err);
-                if (!ok) break;
-                if (end - start == BN && !bad_page && all_seen(kt, start, end, p.window, p.sinks)) {
-                    copy(&v_map, ks + Sh::kTileBytes, v_full(st));
-                    continue;
+                    in_flight = edge;
                 }
-                copy(&v_map, ks + Sh::kTileBytes, v_raw);
-                in_flight = true;
-                ok = warp_wait(v_raw, raw & 1, p.err);
+                ok = value_warps(ok);
+                if (!ok) break;
+                if (!edge) continue;
+                ok = value_warps(warp_wait(v_raw, raw & 1, p.err));
                 if (!ok) break;
                 in_flight = false;
                 ++raw;
-                clean(sm + Sh::kQBytes + st * (2 * Sh::kTileBytes) + Sh::kTileBytes, start, end - start);
+                for (int pc = 0; pc < kPieces; ++pc) clean(at_piece(j * kPieces + pc), pc * Sh::kPieceKeys, start, end - start);
                 fence_proxy_async_smem();
-                mbar_arrive(v_full(st));
+                value_warps(true);
+                if (pt == 0)
+                    for (int pc = 0; pc < kPieces; ++pc) mbar_arrive(v_full((j * kPieces + pc) % NV));
+                issued = (j + 1) * kPieces;
             }
-            if (!ok) {  // what is on its way lands (or is waited for as long as a wait may last) before the block ends
+            if (!ok && warp == kValueWarp) {
                 if (in_flight) mbar_wait_quiet(v_raw, raw & 1);
-                for (int i = issued > ST ? issued - ST : 0; i < issued; ++i) {
-                    mbar_wait_quiet(k_full(i % ST), (i / ST) & 1);
-                    if (i + 1 < issued) mbar_wait_quiet(v_full(i % ST), (i / ST) & 1);
-                }
+                for (int g = issued > NV ? issued - NV : 0; g < issued; ++g) mbar_wait_quiet(v_full(g % NV), (g / NV) & 1);
             }
         } else {
-            long long next[kOwn];
-            offsets(0, next);
-            for (int i = 0; i < n; ++i) {
-                const int st = i % ST, use = i / ST;
-                long long* of = offs + (i & 1) * BN;
-    #pragma unroll
-                for (int x = 0; x < kOwn; ++x) of[pt + x * kProducers] = next[x];
-                ok = producers_all(ok);  // after a failed wait the warps leave together
+            const bf16* vc = static_cast<const bf16*>(p.cache.v) + kvh * p.cache.head_stride;
+            long long* offs = reinterpret_cast<long long*>(sm + Sh::kOffs) + 2 * BN;
+            long long next[2];
+            tile_offsets<kValueThreads>(p, s, kt, t0, pt, next);
+            for (int j = 0; j < n; ++j) {
+                long long* of = offs + (j & 1) * BN;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) of[pt + x * kValueThreads] = next[x];
+                ok = value_warps(ok);  // after a failed wait the warps leave together
                 if (!ok) break;
-                if (i + 1 < n) offsets(i + 1, next);
-                const uint32_t ks = kv_s + st * (2 * Sh::kTileBytes);
-                ok = warp_wait(k_empty(st), (use & 1) ^ 1, p.err);
-                if (!ok) continue;
-                load(ks, kc, of);
-                cp_async_arrive(k_full(st));
-                ok = warp_wait(v_empty(st), (use & 1) ^ 1, p.err);
-                if (!ok) continue;
-                load(ks + Sh::kTileBytes, vc, of);
+                if (j + 1 < n) tile_offsets<kValueThreads>(p, s, kt, t0 + j + 1, pt, next);
                 int start, end;
-                key_range(kt, t0 + i, BN, start, end);
-                if (all_seen(kt, start, end, p.window, p.sinks)) {
-                    cp_async_arrive(v_full(st));
-                } else {
-                    cp_async_commit();
-                    cp_async_wait<0>();
-                    clean(sm + Sh::kQBytes + st * (2 * Sh::kTileBytes) + Sh::kTileBytes, start, end - start);
-                    mbar_arrive(v_full(st));
+                key_range(kt, t0 + j, BN, start, end);
+                const bool edge = !all_seen(kt, start, end, p.window, p.sinks);
+                for (int pc = 0; pc < kPieces && ok; ++pc) {
+                    const int g = j * kPieces + pc, slot = g % NV;
+                    ok = warp_wait(v_empty(slot), ((g / NV) & 1) ^ 1, p.err);
+                    if (!ok) continue;
+                    copy_rows<kValueThreads>(v_ring + slot * Sh::kPieceBytes, vc, of + pc * Sh::kPieceKeys, Sh::kPieceKeys, 0, slabs, D, pt);
+                    if (!edge) cp_async_arrive(v_full(slot));
+                }
+                if (!edge || !ok) continue;
+                cp_async_commit();
+                cp_async_wait<0>();
+                for (int pc = 0; pc < kPieces; ++pc) {  // each thread what it has copied itself
+                    clean(at_piece(j * kPieces + pc), pc * Sh::kPieceKeys, start, end - start);
+                    mbar_arrive(v_full((j * kPieces + pc) % NV));
                 }
             }
             cp_async_commit();
             cp_async_wait<0>();
         }
     } else {
-        // The whole warp walks the units, so that all it computes is uniform; one elected thread issues.
+        // The whole warp walks the tiles, so that all it computes is uniform; one elected thread issues.
         const int d16 = (D + 15) & ~15, k_steps = d16 / 16;
+        const int block = tma ? v_box : Sh::kPieceKeys;
         const uint32_t t_mem = __shfl_sync(0xffffffffu, tmem, 0);
         const uint32_t idesc_s = idesc_bf16_f32(128, BN);
         const uint32_t idesc_o = idesc_bf16_f32(128, d16) | kBTransposed;
         // descriptors of the first operands; the others differ in the address field alone (16-byte units)
-        const uint64_t q_desc = kmajor_sw128_desc(q_s), k_desc = kmajor_sw128_desc(kv_s);
-        const uint64_t v_desc = mnmajor_sw128_desc(kv_s + Sh::kTileBytes, BN * 128);
+        const uint64_t q_desc = kmajor_sw128_desc(q_s), k_desc = kmajor_sw128_desc(k_ring);
+        const uint64_t v_desc = mnmajor_sw128_desc(v_ring, block * 128, block == 8 ? kSlabs * 1024 : 1024);
         const bool leader = elect_one();
+        auto piece_there = [&](uint32_t bar, int turn) -> bool {
+            if (!warp_wait(bar, turn & 1, p.err)) return false;
+            // cp.async writes through the generic proxy, the products read through the async one: ordered here, by
+            // the threads that have seen the copies land
+            if (!tma) fence_proxy_async_smem();
+            tc_fence_after();
+            return true;
+        };
+        // unit u: key tile j of row tile t, in slot u & 1; the second row tile reads what the first has waited for
         auto walk = [&](auto two) {
             constexpr bool kPair = decltype(two)::value;
             auto scores = [&](int u, int slot) -> bool {
-                const int kv = kPair ? u >> 1 : u, t = kPair ? slot : 0, st = kv % ST;
-                if (!warp_wait(k_full(st), (kv / ST) & 1, p.err)) return false;
-                // cp.async writes through the generic proxy, the products read through the async one: ordered here, by
-                // the threads that have seen the copies land
-                if (box == 0) fence_proxy_async_smem();
-                tc_fence_after();
-                const uint64_t qd = q_desc + static_cast<uint64_t>(t * (128 * DP * 2) >> 4);
-                const uint64_t kd = k_desc + static_cast<uint64_t>(st * (2 * Sh::kTileBytes) >> 4);
-                if (leader) {
-                    auto step = [&](int k) {
-                        umma_bf16(t_mem + slot * BN, qd + (((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4),
-                                  kd + (((k >> 2) * (BN * 128) + (k & 3) * 32) >> 4), idesc_s, k > 0);
-                    };
-                    if (k_steps == DP / 16) {
+                const int j = kPair ? u >> 1 : u, t = kPair ? slot : 0;
+                for (int pc = 0; pc < kPieces; ++pc) {
+                    const int g = j * kPieces + pc, at = g % NK;
+                    if ((!kPair || t == 0) && !piece_there(k_full(at), g / NK)) return false;
+                    const uint64_t kd = k_desc + static_cast<uint64_t>(at * Sh::kPieceBytes >> 4);
+                    const uint64_t qd = q_desc + static_cast<uint64_t>((t * (128 * DP * 2) + pc * Sh::kPieceSlabs * (128 * 128)) >> 4);
+                    if (leader) {
+                        const int steps = min(4 * Sh::kPieceSlabs, k_steps - pc * 4 * Sh::kPieceSlabs);
+                        auto step = [&](int k) {
+                            umma_bf16(t_mem + slot * BN, qd + (((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4),
+                                      kd + (((k >> 2) * (BN * 128) + (k & 3) * 32) >> 4), idesc_s, k > 0 || pc > 0);
+                        };
+                        if (steps == 4 * Sh::kPieceSlabs) {
 #pragma unroll
-                        for (int k = 0; k < DP / 16; ++k) step(k);
-                    } else {
-                        for (int k = 0; k < k_steps; ++k) step(k);
+                            for (int k = 0; k < 4 * Sh::kPieceSlabs; ++k) step(k);
+                        } else {
+                            for (int k = 0; k < steps; ++k) step(k);
+                        }
+                        if (pc == kPieces - 1) umma_commit(s_full(slot));
+                        if (!kPair || t == 1) umma_commit(k_empty(at));
                     }
-                    umma_commit(s_full(slot));
-                    if (!kPair || t == 1) umma_commit(k_empty(st));
+                    __syncwarp();
                 }
-                __syncwarp();
                 return true;
             };
             auto values = [&](int u, int slot) -> bool {
-                const int kv = kPair ? u >> 1 : u, t = kPair ? slot : 0, st = kv % ST;
-                const uint64_t vd = v_desc + static_cast<uint64_t>(st * (2 * Sh::kTileBytes) >> 4);
+                const int j = kPair ? u >> 1 : u, t = kPair ? slot : 0;
                 const uint32_t o = t_mem + Sh::kO + t * DP, pa = t_mem + slot * BN;
-                if (!kPair || t == 0) {  // the second row tile's products read what the first one's have waited for
-                    if (!warp_wait(v_full(st), (kv / ST) & 1, p.err)) return false;
-                    if (box == 0) fence_proxy_async_smem();
-                }
-                if (!warp_wait(p_half(slot), (u >> 1) & 1, p.err)) return false;
-                tc_fence_after();
-                if (leader) {
+                constexpr int kSteps = BN / 16 / kPieces;
+                for (int pc = 0; pc < kPieces; ++pc) {
+                    const int g = j * kPieces + pc, at = g % NV;
+                    if ((!kPair || t == 0) && !piece_there(v_full(at), g / NV)) return false;
+                    const uint64_t vd = v_desc + static_cast<uint64_t>(at * Sh::kPieceBytes >> 4);
+                    auto step = [&](int k) {  // 16 keys
+                        const int key = k * 16, in = key & (block - 1);
+                        umma_bf16_ta(o, pa + (pc * kSteps + k) * 8, vd + (((key - in) * (kSlabs * 128) + in * 128) >> 4), idesc_o,
+                                     k > 0 || pc > 0 || j > 0);
+                    };
+                    // quarters of P that are handed over early, and the rest
+                    constexpr int kQuarters = 4 / kPieces;  // of a piece
+                    if (pc == 0) {
+                        if (!warp_wait(p_early(slot), (u >> 1) & 1, p.err)) return false;
+                        tc_fence_after();
+                    }
+                    if (kPieces == 1) {
+                        if (leader) {
 #pragma unroll
-                    for (int k = 0; k < 2 * kEarly; ++k) umma_bf16_ta(o, pa + k * 8, vd + (k * 2048 >> 4), idesc_o, k > 0 || kv > 0);
-                }
-                __syncwarp();
-                if (!warp_wait(p_full(slot), (u >> 1) & 1, p.err)) return false;
-                tc_fence_after();
-                if (leader) {
+                            for (int k = 0; k < 2 * kEarly; ++k) step(k);
+                        }
+                        __syncwarp();
+                    }
+                    if (pc * kQuarters >= kEarly || kPieces == 1) {
+                        if (!warp_wait(p_full(slot), (u >> 1) & 1, p.err)) return false;
+                        tc_fence_after();
+                    }
+                    if (leader) {
 #pragma unroll
-                    for (int k = 2 * kEarly; k < BN / 16; ++k) umma_bf16_ta(o, pa + k * 8, vd + (k * 2048 >> 4), idesc_o, 1);
-                    umma_commit(pv_done(slot));
-                    if (!kPair || t == 1) umma_commit(v_empty(st));
+                        for (int k = kPieces == 1 ? 2 * kEarly : 0; k < kSteps; ++k) step(k);
+                        if (pc == kPieces - 1) umma_commit(pv_done(slot));
+                        if (!kPair || t == 1) umma_commit(v_empty(at));
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
                 return true;
             };
+            const int units = kPair ? 2 * n : n;
             bool ok = scores(0, 0) && (units < 2 || scores(1, 1));
             for (int u = 0; u < units && ok; u += 2) {
                 ok = values(u, 0) && (u + 2 >= units || scores(u + 2, 0));
@@ -594,9 +689,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     tc_fence_after();
 
     if (softmax_on) {
-        const int h_in = my_rr % a.G;
         const long long row = sq.row0 + my_rr / a.G;
-        const int h = kvh * a.G + h_in;
+        const int h = kvh * a.G + my_rr % a.G;
         const bool live = my_rr < n_rows;
         const long long at = (static_cast<long long>(split) * p.batch.rows + row) * p.q_heads + h;
         const float inv = partial ? 1.f : (l == 0.f ? 0.f : 1.f / l);
@@ -605,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         bf16* out = static_cast<bf16*>(p.out) + row * p.ldo + static_cast<long long>(h) * D;
         for (int c = 0; c < D; c += 16) {
             uint32_t r[16];
-            tmem_ld16(my_lanes + Sh::kO + wg * DP + c, r);
+            tmem_ld16(my_lanes + Sh::kO + rt * DP + c, r);
             tmem_wait_ld();
             float o[16];
 #pragma unroll
@@ -659,19 +753,19 @@ void launch(const Args& a, dim3 grid, cudaStream_t st) {
         SANA_CUDA(cudaFuncSetAttribute(paged_tc_kernel<DP, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem));
         once.mark();
     }
-    const int box = copy_box(a.p.cache, Sh::kKeys);
+    const int k_box = copy_box(a.p.cache, kKeys), v_box = k_box > 0 ? copy_box(a.p.cache, Sh::kPieceKeys) : 0;
     CUtensorMap k{}, v{};
-    if (box > 0) {
-        k = pool_map(a.p.cache, a.p.cache.k, box);
-        v = pool_map(a.p.cache, a.p.cache.v, box);
+    if (k_box > 0) {
+        k = pool_map(a.p.cache, a.p.cache.k, k_box);
+        v = a.p.cache.D % 64 == 0 ? pool_map_slabs(a.p.cache, a.p.cache.v, v_box) : pool_map(a.p.cache, a.p.cache.v, v_box);
     }
-    paged_tc_kernel<DP, CAP><<<grid, kThreads, Sh::kSmem, st>>>(a, k, v, box);
+    paged_tc_kernel<DP, CAP><<<grid, kThreads, Sh::kSmem, st>>>(a, k, v, k_box, v_box);
 }
 
 }  // namespace
 
 int tc_rows(int D) { return D <= 128 ? 256 : 128; }
-int tc_keys(int D) { return D <= 128 ? 128 : 64; }
+int tc_keys() { return kKeys; }
 void launch_tc(const Args& a, dim3 grid, cudaStream_t st) {
     const bool cap = a.p.softcap > 0.f;
     if (a.p.cache.D <= 64) cap ? launch<64, true>(a, grid, st) : launch<64, false>(a, grid, st);
