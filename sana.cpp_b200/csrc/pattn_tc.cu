@@ -22,8 +22,8 @@
 // MN-major (its channels contiguous). K and V have a ring each, filled by warps of their own, of
 // whole tiles, or for head sizes above 128, where a tile has 64 KB, of quarters (64 channels of K,
 // 32 keys of V). Where pages divide a tile or tiles divide a page, tensor copies (TMA) bring them:
-// K one per page and slab; V one per page, all slabs, where the head size is a multiple of 64. V's
-// keys stand in blocks of what one copy brings, [block][slab][key], which its descriptors follow.
+// K one per page and slab; V one per 16 keys, all slabs, where the head size is a multiple of 64. V's
+// keys stand in blocks of a product's 16, [block][slab][key], which makes a copy of all slabs one box.
 // Other page sizes end anywhere inside a tile and come by 16-byte cp.async.
 #include <type_traits>
 
@@ -47,18 +47,22 @@ template <int DP>
 struct TcShape {
     static constexpr int kTiles = DP <= 128 ? 2 : 1;     // row tiles of 128
     static constexpr int kRows = 128 * kTiles;
+    static constexpr int kParts = kTiles == 2 ? 1 : 2;   // threads of a row
+    static constexpr int kCols = kKeys / kParts;         // scores of a thread
     static constexpr int kSlabs = DP / 64;
     static constexpr int kPieces = DP <= 128 ? 1 : 4;    // of a tile of K or V
     static constexpr int kPieceSlabs = kSlabs / kPieces; // of K
     static constexpr int kPieceKeys = kKeys / kPieces;   // of V
+    static constexpr int kBlock = DP <= 128 ? kKeys : 16;  // keys of a block of V (8 of them where pages are of 8)
     static constexpr int kPieceBytes = kKeys * DP * 2 / kPieces;
     static constexpr int kKRing = DP == 64 ? 4 : DP == 128 ? 2 : 5, kVRing = DP == 64 ? 4 : DP == 128 ? 2 : 4;  // pieces
     static constexpr int kQBytes = kTiles * 128 * DP * 2;
     static constexpr int kBarriers = 2 * (kKRing + kVRing) + 8 + 2;
-    // behind Q and the rings: keys' offsets [2 for K, 2 for V][kKeys] (cp.async), barriers, three words
+    // behind Q and the rings: keys' offsets [2 for K, 2 for V][kKeys] (cp.async), maxima [2][kParts][128], barriers, three words
     static constexpr int kVRingAt = kQBytes + kKRing * kPieceBytes;
     static constexpr int kOffs = kVRingAt + kVRing * kPieceBytes;
-    static constexpr int kBars = kOffs + 4 * kKeys * 8;
+    static constexpr int kMax = kOffs + 4 * kKeys * 8;
+    static constexpr int kBars = kMax + (kParts > 1 ? 2 * kParts * 128 * 4 : 0);
     static constexpr int kSmem = 1024 + kBars + kBarriers * 8 + 16;
     // tensor memory columns: S slots at 0 and kKeys, O behind them
     static constexpr int kO = 2 * kKeys;
@@ -94,14 +98,30 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
         : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// D += A B with A (bf16 pairs) in tensor memory
-__device__ __forceinline__ void umma_bf16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                             uint32_t accumulate) {
+// The products and commits of the issuing warp, by the lane whose `on` is not 0: predicated, not branched around, so that
+// the descriptors' arithmetic stays uniform. D += A B with A in shared memory, or (bf16 pairs) in tensor memory.
+__device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate,
+                                        uint32_t on) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(on)
+        : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate,
+                                        uint32_t on) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(on)
+        : "memory");
+}
+__device__ __forceinline__ void umma_commit_on(uint32_t bar, uint32_t on) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(on)
         : "memory");
 }
 // Descriptor of an MN-major operand in the 128-byte swizzle: 64 channels of a row contiguous, groups
@@ -127,10 +147,10 @@ __device__ __forceinline__ float soft_cap_log2(float x, float in, float out) {
     return fmaf(-2.f * out, rcp_approx(1.f + ex2_approx(x * in)), out);
 }
 
-__device__ __forceinline__ bool elect_one() {
+__device__ __forceinline__ uint32_t elect_one() {
     uint32_t on;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(on));
-    return on != 0;
+    return on;
 }
 // One arrival of this thread on `bar` once all its copies so far have landed.
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
@@ -151,6 +171,31 @@ __device__ __forceinline__ bool meet_all(int id, int threads, bool ok) {
     return all != 0;
 }
 __device__ __forceinline__ bool value_warps(bool ok) { return meet_all(1, kValueThreads, ok); }
+// 2^x of a pair on the FMA pipe, |x| <= 125: x = n + f with n the nearest whole number, 2^f on [-1/2, 1/2] by the
+// degree-4 polynomial of least largest relative error (2.7e-6; fitted by linear programming over Chebyshev nodes), 2^n as
+// exponent bits: n + 127 is left in the low bits of x + 1.5 2^23 + 127.
+__device__ __forceinline__ uint64_t exp2_poly2(uint64_t x) {
+    constexpr float kMagic = 12582912.0f + 127.0f;
+    const uint64_t t = add2(x, f2_make(kMagic, kMagic));
+    const uint64_t f = sub2(x, sub2(t, f2_make(kMagic, kMagic)));
+    uint64_t q = fma2(f, f2_make(9.567709878e-03f, 9.567709878e-03f), f2_make(5.591749132e-02f, 5.591749132e-02f));
+    q = fma2(q, f, f2_make(2.402481151e-01f, 2.402481151e-01f));
+    q = fma2(q, f, f2_make(6.931219409e-01f, 6.931219409e-01f));
+    q = fma2(q, f, f2_make(9.999992499e-01f, 9.999992499e-01f));
+    const float2 n = f2_split(t);
+    return mul2(q, f2_make(__uint_as_float(__float_as_uint(n.x) << 23), __uint_as_float(__float_as_uint(n.y) << 23)));
+}
+// The cap of a pair. Of its two special functions and the probability's one, which bound the softmax of capped scores
+// (16 a clock and SM), the first exponential is taken on the FMA pipe: e^2z (1 + 3e-6) changes tanh z by at most 1.4e-6.
+// Beyond |2z log2 e| = 40 tanh z is 1 in fp32 either way; NaN stays NaN.
+__device__ __forceinline__ uint64_t soft_cap_log2_2(uint64_t x, float in, float out) {
+    float2 z = f2_split(mul2(x, f2_make(in, in)));
+    asm("{\n\t.reg .f32 t;\n\tmax.NaN.f32 t, %0, 0fC2200000;\n\tmin.NaN.f32 %0, t, 0f42200000;\n\t}" : "+f"(z.x));
+    asm("{\n\t.reg .f32 t;\n\tmax.NaN.f32 t, %0, 0fC2200000;\n\tmin.NaN.f32 %0, t, 0f42200000;\n\t}" : "+f"(z.y));
+    const float2 d = f2_split(add2(exp2_poly2(f2_make(z.x, z.y)), f2_make(1.f, 1.f)));
+    return fma2(f2_make(-2.f * out, -2.f * out), f2_make(rcp_approx(d.x), rcp_approx(d.y)), f2_make(out, out));
+}
+
 // Bit i: the row at position pos sees key j0 + i, below `end`.
 __device__ __forceinline__ uint32_t low_bits(int n) {  // the n lowest bits, n of any sign and size
     return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
@@ -172,7 +217,7 @@ __device__ __forceinline__ int box_page(const PagedAttention& p, int s, const Ke
     return page < p.cache.pages ? page : -1;
 }
 // cp.async: offsets of the keys t, t + THREADS, .. of a key tile, and the copy of `keys` keys and `count` slabs from
-// `slab` into [slab][key] at dst.
+// `slab` into [block of keys][slab][key] at dst.
 template <int THREADS>
 __device__ __forceinline__ void tile_offsets(const PagedAttention& p, int s, const KeyTiles& kt, int tile, int t,
                                              long long (&o)[kKeys / THREADS]) {
@@ -185,15 +230,17 @@ __device__ __forceinline__ void tile_offsets(const PagedAttention& p, int s, con
     }
 }
 template <int THREADS>
-__device__ __forceinline__ void copy_rows(uint32_t dst, const bf16* src, const long long* of, int keys, int slab, int count, int D,
-                                          int t) {
+__device__ __forceinline__ void copy_rows(uint32_t dst, const bf16* src, const long long* of, int keys, int block, int block_slabs,
+                                          int slab, int count, int D, int t) {
     for (int x = 0; x < count; ++x) {
         const int d = (slab + x) * 64 + (t & 7) * 8;
 #pragma unroll 4
         for (int key = t >> 3; key < keys; key += THREADS / 8) {
             const long long off = of[key];
             const bool in = off >= 0 && d < D;
-            cp_async16(dst + x * (keys * 128) + key * 128 + (((t & 7) ^ (key & 7)) << 4), in ? src + off + d : src, in);
+            const int row = key & (block - 1);
+            cp_async16(dst + (key - row) * (block_slabs * 128) + x * (block * 128) + row * 128 + (((t & 7) ^ (row & 7)) << 4),
+                       in ? src + off + d : src, in);
         }
     }
 }
@@ -205,7 +252,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                                                                const int v_box) {
     using Sh = TcShape<DP>;
     constexpr int BN = kKeys, NK = Sh::kKRing, NV = Sh::kVRing, kPieces = Sh::kPieces, kSlabs = Sh::kSlabs;
-    constexpr int kEarly = 3;  // quarters of a tile's P handed over before the rest
+    constexpr int kParts = Sh::kParts, kCols = Sh::kCols;
+    constexpr int kEarly = kParts == 1 ? 3 : 2;  // quarters of a tile's P handed over before the rest
     extern __shared__ unsigned char smem_raw[];
     const PagedAttention& p = a.p;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = p.cache.D;
@@ -287,11 +335,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(words);
     const bool bad_page = *reinterpret_cast<volatile int*>(words + 1) != 0;
 
-    // a softmax thread's row tile and row; tensor memory lanes 32 (warp & 3) ..
-    const int rt = warp >> 2, my_rr = rr0 + rt * 128 + (tid & 127);
+    float* maxima = reinterpret_cast<float*>(sm + Sh::kMax);
+    // a softmax thread's row tile, part of the row, and row; tensor memory lanes 32 (warp & 3) ..
+    const int rt = kParts == 1 ? warp >> 2 : 0, part = kParts == 1 ? 0 : warp >> 2, my_rr = rr0 + rt * 128 + (tid & 127);
     const int my_pos = my_rr < n_rows ? sq.past + my_rr / a.G : -1;
     const uint32_t my_lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);
-    const bool softmax_on = warp < kSoftmaxWarps && (rt == 0 || pair);
+    const bool softmax_on = warp < kSoftmaxWarps && (kParts > 1 || rt == 0 || pair);
     float m = -INFINITY, l = 0.f;
 
     if (warp < kSoftmaxWarps) {
@@ -303,41 +352,55 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             mine.pmin = sq.past + (rr0 + rt * 128) / a.G;
             mine.pmax = sq.past + (min(n_rows, rr0 + rt * 128 + 128) - 1) / a.G;
             const uint32_t o_t = my_lanes + Sh::kO + rt * DP;
+            bool ok = true;
             for (int j = 0; j < n; ++j) {
                 const int slot = pair ? rt : j & 1, turn = pair ? j : j >> 1;
                 int start, end;
                 key_range(kt, t0 + j, BN, start, end);
                 const bool whole = end - start == BN && !bad_page && all_seen(mine, start, end, p.window, p.sinks);
+                start += part * kCols;
                 const uint32_t s_t = my_lanes + slot * BN;
-                if (!warp_wait(s_full(slot), turn & 1, p.err)) break;
-                tc_fence_after();
-                // the whole row in registers: the loads are in flight together
-                uint32_t x[BN];
+                ok = ok && warp_wait(s_full(slot), turn & 1, p.err);
+                if (kParts == 1 && !ok) break;
+                // this thread's scores in registers: the loads are in flight together
+                uint32_t x[kCols];
+                float mx = -INFINITY;
+                if (ok) {
+                    tc_fence_after();
 #pragma unroll
-                for (int c = 0; c < BN / 32; ++c) tmem_ld32(s_t + c * 32, &x[c * 32]);
-                tmem_wait_ld();
-                if (!whole) {
+                    for (int c = 0; c < kCols / 32; ++c) tmem_ld32(s_t + part * kCols + c * 32, &x[c * 32]);
+                    tmem_wait_ld();
+                    if (!whole) {
 #pragma unroll
-                    for (int c = 0; c < BN / 32; ++c) {
-                        const int j0 = start + c * 32;
-                        uint32_t bits = seen_bits(j0, end, my_pos, p.window, p.sinks);
-                        if (bad_page) {
+                        for (int c = 0; c < kCols / 32; ++c) {
+                            uint32_t bits = seen_bits(start + c * 32, end, my_pos, p.window, p.sinks);
+                            if (bad_page) {
+                                for (int i = 0; i < 32; ++i)
+                                    if ((bits >> i & 1u) && key_offset(p, s, start + c * 32 + i) < 0) bits &= ~(1u << i);
+                            }
+#pragma unroll
                             for (int i = 0; i < 32; ++i)
-                                if ((bits >> i & 1u) && key_offset(p, s, j0 + i) < 0) bits &= ~(1u << i);
+                                if (!(bits & (1u << i))) x[c * 32 + i] = 0xff800000u;
                         }
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (!(bits & (1u << i))) x[c * 32 + i] = 0xff800000u;
                     }
+                    float mx4[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) mx4[c] = fmaxf(__uint_as_float(x[c]), __uint_as_float(x[4 + c]));
+#pragma unroll
+                    for (int i = 8; i < kCols; i += 4)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) mx4[c] = fmaxf(mx4[c], __uint_as_float(x[i + c]));
+                    mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
                 }
-                float mx4[4];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) mx4[c] = fmaxf(__uint_as_float(x[c]), __uint_as_float(x[4 + c]));
-#pragma unroll
-                for (int i = 8; i < BN; i += 4)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) mx4[c] = fmaxf(mx4[c], __uint_as_float(x[i + c]));
-                float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+                if constexpr (kParts > 1) {
+                    // The row's threads agree on its maximum; they have read their scores by then, so that P may be
+                    // written over them. After a failed wait they leave together.
+                    float* const my_max = maxima + (j & 1) * (kParts * 128) + (tid & 127);
+                    my_max[part * 128] = mx;
+                    ok = meet_all(2 + (warp & 3), kParts * 32, ok);
+                    if (!ok) break;
+                    mx = fmaxf(my_max[0], my_max[128]);
+                }
                 // both maps rise with the score (scale > 0), so the maximum is mapped alone
                 if (mx != -INFINITY) mx = CAP ? soft_cap_log2(mx, cap_in, cap_out) : mx * scale_log2;
                 const bool move = mx > m + 8.f;  // (-inf + 8 is passed by any score)
@@ -345,11 +408,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     const float alpha = move ? ex2_approx(m - mx) : 1.f;
                     m = move ? mx : m;
                     l *= alpha;
-                    if (j > 0) {  // O holds sums against the old reference
+                    if (j > 0) {  // O holds sums against the old reference; each part rescales some of its channels
                         const int slot0 = pair ? rt : (j - 1) & 1, turn0 = pair ? j - 1 : (j - 1) >> 1;
-                        if (!warp_wait(pv_done(slot0), turn0 & 1, p.err)) break;
+                        ok = warp_wait(pv_done(slot0), turn0 & 1, p.err);
+                        if (!ok) continue;  // (to tell the row's other threads)
                         tc_fence_after();
-                        for (int c = 0; c < D; c += 16) {
+                        for (int c = part * 16; c < D; c += kParts * 16) {
                             uint32_t r[16];
                             tmem_ld16(o_t + c, r);
                             tmem_wait_ld();
@@ -363,14 +427,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 const uint64_t k2 = f2_make(scale_log2, scale_log2), r2 = f2_make(-ref, -ref);
                 uint64_t sum[2] = {0, 0};
 #pragma unroll
-                for (int c = 0; c < BN / 32; ++c) {
+                for (int c = 0; c < kCols / 32; ++c) {
                     uint32_t pk[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const float x0 = __uint_as_float(x[c * 32 + 2 * i]), x1 = __uint_as_float(x[c * 32 + 2 * i + 1]);
                         uint64_t e;
                         if constexpr (CAP) {
-                            e = add2(f2_make(soft_cap_log2(x0, cap_in, cap_out), soft_cap_log2(x1, cap_in, cap_out)), r2);
+                            e = add2(soft_cap_log2_2(f2_make(x0, x1), cap_in, cap_out), r2);
                             const float2 v = f2_split(e);  // the cap maps what is masked to a number: it stays masked
                             if (!whole) e = f2_make(x0 == -INFINITY ? x0 : v.x, x1 == -INFINITY ? x1 : v.y);
                         } else {
@@ -381,8 +445,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         sum[i & 1] = add2(sum[i & 1], f2_make(e0, e1));
                         pk[i] = pack_bf2(e0, e1);
                     }
-                    tmem_st16(s_t + c * 16, pk);  // over the scores, which this row has read
-                    if (c == kEarly - 1) {        // the products over these keys may start
+                    tmem_st16(s_t + part * (kCols / 2) + c * 16, pk);  // over the scores, which this row has read
+                    if (kParts == 1 && c == kEarly - 1) {              // the products over these keys may start
                         tmem_wait_st();
                         tc_fence_before();
                         __syncwarp();
@@ -394,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(p_full(slot));
+                if (lane == 0) mbar_arrive(kParts == 1 || part == 1 ? p_full(slot) : p_early(slot));
             }
         }
     } else if (warp == kKeyWarp) {
@@ -405,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             // lane b < BN / k_box holds the page of box b, `k_box` keys of one page; one elected thread copies
             const int boxes = BN / k_box;
             auto page_of = [&](int j) { return box_page(p, s, kt, t0 + j, lane, boxes, k_box); };
-            const bool leader = elect_one();
+            const bool leader = elect_one() != 0;
             int next = page_of(0), issued = 0;
             for (int j = 0; j < n && ok; ++j) {
                 const int page = next;
@@ -448,7 +512,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     const int g = j * kPieces + pc, slot = g % NK;
                     ok = warp_wait(k_empty(slot), ((g / NK) & 1) ^ 1, p.err);
                     if (!ok) continue;
-                    copy_rows<32>(k_ring + slot * Sh::kPieceBytes, kc, of, BN, pc * Sh::kPieceSlabs, piece_slabs(pc), D, lane);
+                    copy_rows<32>(k_ring + slot * Sh::kPieceBytes, kc, of, BN, BN, Sh::kPieceSlabs, pc * Sh::kPieceSlabs,
+                                  piece_slabs(pc), D, lane);
                     cp_async_arrive(k_full(slot));
                 }
             }
@@ -457,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         }
     } else if (warp < kMmaWarp) {
         const int pt = tid - kValueWarp * 32, slabs = (D + 63) / 64;
-        const int block = tma ? v_box : Sh::kPieceKeys;  // keys of a block
+        const int block = Sh::kPieces > 1 && tma ? v_box : Sh::kBlock;  // keys of a block
         // Values that are not finite, in a tile that not every row sees whole, would reach the rows that do
         // not see them as 0 * v: zeros take their place, and the rows that see them get them at the end.
         // Keys from `keys` on, and those of bad pages, are zeros outright (a tensor copy brought what lies there).
@@ -492,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             // as for K, by the first value warp; the second helps to clean and keeps step, waiting for no place
             const int boxes = BN / v_box, boxes_piece = Sh::kPieceKeys / v_box;
             auto page_of = [&](int j) { return box_page(p, s, kt, t0 + j, lane, boxes, v_box); };
-            const bool leader = elect_one(), all_slabs = D % 64 == 0;
+            const bool leader = elect_one() != 0, all_slabs = kPieces > 1 && D % 64 == 0;
             int next = page_of(0), issued = 0, raw = 0;
             bool in_flight = false;  // on v_raw
             for (int j = 0; j < n; ++j) {
@@ -517,13 +582,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         }
                         __syncwarp();
                         uint32_t dst = v_ring + slot * Sh::kPieceBytes;
-                        for (int b = pc * boxes_piece; b < (pc + 1) * boxes_piece; ++b, dst += v_box * kSlabs * 128) {
+                        for (int b = pc * boxes_piece; b < (pc + 1) * boxes_piece; ++b, dst += v_box * (kPieces > 1 ? kSlabs * 128 : 128)) {
                             const int pg = __shfl_sync(0xffffffffu, page, b), row = __shfl_sync(0xffffffffu, at, b);
                             if (leader && pg >= 0) {
                                 if (all_slabs) {
                                     tma_load_5d(&v_map, dst, bar, 0, row, 0, kvh, pg);
                                 } else {
-                                    for (int x = 0; x < slabs; ++x) tma_load_4d(&v_map, dst + x * (v_box * 128), bar, x * 64, row, kvh, pg);
+                                    for (int x = 0; x < slabs; ++x) tma_load_4d(&v_map, dst + x * (block * 128), bar, x * 64, row, kvh, pg);
                                 }
                             }
                         }
@@ -568,7 +633,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     const int g = j * kPieces + pc, slot = g % NV;
                     ok = warp_wait(v_empty(slot), ((g / NV) & 1) ^ 1, p.err);
                     if (!ok) continue;
-                    copy_rows<kValueThreads>(v_ring + slot * Sh::kPieceBytes, vc, of + pc * Sh::kPieceKeys, Sh::kPieceKeys, 0, slabs, D, pt);
+                    copy_rows<kValueThreads>(v_ring + slot * Sh::kPieceBytes, vc, of + pc * Sh::kPieceKeys, Sh::kPieceKeys, Sh::kBlock, kSlabs, 0,
+                                             slabs, D, pt);
                     if (!edge) cp_async_arrive(v_full(slot));
                 }
                 if (!edge || !ok) continue;
@@ -585,14 +651,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     } else {
         // The whole warp walks the tiles, so that all it computes is uniform; one elected thread issues.
         const int d16 = (D + 15) & ~15, k_steps = d16 / 16;
-        const int block = tma ? v_box : Sh::kPieceKeys;
+        const int block = Sh::kPieces > 1 && tma ? v_box : Sh::kBlock;
         const uint32_t t_mem = __shfl_sync(0xffffffffu, tmem, 0);
         const uint32_t idesc_s = idesc_bf16_f32(128, BN);
         const uint32_t idesc_o = idesc_bf16_f32(128, d16) | kBTransposed;
         // descriptors of the first operands; the others differ in the address field alone (16-byte units)
         const uint64_t q_desc = kmajor_sw128_desc(q_s), k_desc = kmajor_sw128_desc(k_ring);
         const uint64_t v_desc = mnmajor_sw128_desc(v_ring, block * 128, block == 8 ? kSlabs * 1024 : 1024);
-        const bool leader = elect_one();
+        const uint32_t leader = elect_one();
         auto piece_there = [&](uint32_t bar, int turn) -> bool {
             if (!warp_wait(bar, turn & 1, p.err)) return false;
             // cp.async writes through the generic proxy, the products read through the async one: ordered here, by
@@ -601,6 +667,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             tc_fence_after();
             return true;
         };
+        // The products of a tile in one piece are branched around by the other lanes, those of smaller pieces predicated:
+        // 170 and 183 us, but 370 and 350 us (2048 tokens after 8192, head sizes 128 and 256).
+        constexpr bool kBranch = kPieces == 1;
+        const uint32_t on = kBranch ? 1u : leader;
         // unit u: key tile j of row tile t, in slot u & 1; the second row tile reads what the first has waited for
         auto walk = [&](auto two) {
             constexpr bool kPair = decltype(two)::value;
@@ -611,22 +681,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     if ((!kPair || t == 0) && !piece_there(k_full(at), g / NK)) return false;
                     const uint64_t kd = k_desc + static_cast<uint64_t>(at * Sh::kPieceBytes >> 4);
                     const uint64_t qd = q_desc + static_cast<uint64_t>((t * (128 * DP * 2) + pc * Sh::kPieceSlabs * (128 * 128)) >> 4);
-                    if (leader) {
-                        const int steps = min(4 * Sh::kPieceSlabs, k_steps - pc * 4 * Sh::kPieceSlabs);
-                        auto step = [&](int k) {
-                            umma_bf16(t_mem + slot * BN, qd + (((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4),
-                                      kd + (((k >> 2) * (BN * 128) + (k & 3) * 32) >> 4), idesc_s, k > 0 || pc > 0);
-                        };
+                    auto step = [&](int k) {
+                        umma_ss(t_mem + slot * BN, qd + (((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4),
+                                kd + (((k >> 2) * (BN * 128) + (k & 3) * 32) >> 4), idesc_s, k > 0 || pc > 0, on);
+                    };
+                    const int steps = min(4 * Sh::kPieceSlabs, k_steps - pc * 4 * Sh::kPieceSlabs);
+                    if (!kBranch || leader) {
                         if (steps == 4 * Sh::kPieceSlabs) {
 #pragma unroll
                             for (int k = 0; k < 4 * Sh::kPieceSlabs; ++k) step(k);
                         } else {
                             for (int k = 0; k < steps; ++k) step(k);
                         }
-                        if (pc == kPieces - 1) umma_commit(s_full(slot));
-                        if (!kPair || t == 1) umma_commit(k_empty(at));
                     }
                     __syncwarp();
+                    if (pc == kPieces - 1) umma_commit_on(s_full(slot), leader);
+                    if (!kPair || t == 1) umma_commit_on(k_empty(at), leader);
                 }
                 return true;
             };
@@ -639,9 +709,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     if ((!kPair || t == 0) && !piece_there(v_full(at), g / NV)) return false;
                     const uint64_t vd = v_desc + static_cast<uint64_t>(at * Sh::kPieceBytes >> 4);
                     auto step = [&](int k) {  // 16 keys
-                        const int key = k * 16, in = key & (block - 1);
-                        umma_bf16_ta(o, pa + (pc * kSteps + k) * 8, vd + (((key - in) * (kSlabs * 128) + in * 128) >> 4), idesc_o,
-                                     k > 0 || pc > 0 || j > 0);
+                        umma_ts(o, pa + (pc * kSteps + k) * 8, vd + (k * (kPieces > 1 ? 2048 * kSlabs : 2048) >> 4), idesc_o,
+                                k > 0 || pc > 0 || j > 0, on);
                     };
                     // quarters of P that are handed over early, and the rest
                     constexpr int kQuarters = 4 / kPieces;  // of a piece
@@ -650,23 +719,23 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         tc_fence_after();
                     }
                     if (kPieces == 1) {
-                        if (leader) {
+                        if (!kBranch || leader) {
 #pragma unroll
                             for (int k = 0; k < 2 * kEarly; ++k) step(k);
                         }
                         __syncwarp();
                     }
-                    if (pc * kQuarters >= kEarly || kPieces == 1) {
+                    if (pc * kQuarters == kEarly || kPieces == 1) {
                         if (!warp_wait(p_full(slot), (u >> 1) & 1, p.err)) return false;
                         tc_fence_after();
                     }
-                    if (leader) {
+                    if (!kBranch || leader) {
 #pragma unroll
                         for (int k = kPieces == 1 ? 2 * kEarly : 0; k < kSteps; ++k) step(k);
-                        if (pc == kPieces - 1) umma_commit(pv_done(slot));
-                        if (!kPair || t == 1) umma_commit(v_empty(at));
                     }
                     __syncwarp();
+                    if (pc == kPieces - 1) umma_commit_on(pv_done(slot), leader);
+                    if (!kPair || t == 1) umma_commit_on(v_empty(at), leader);
                 }
                 return true;
             };
@@ -679,8 +748,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         };
         if (Sh::kTiles == 2 && pair) walk(std::true_type{});
         else walk(std::false_type{});
-        if (leader) umma_commit(drained);  // whatever was issued has run before the tensor memory is given back
-        __syncwarp();
+        umma_commit_on(drained, leader);  // whatever was issued has run before the tensor memory is given back
         mbar_wait_quiet(drained, 0);
     }
     __syncwarp();
@@ -688,16 +756,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     __syncthreads();
     tc_fence_after();
 
+    if (kParts > 1) {  // the sums of a row's threads meet where the maxima were
+        if (softmax_on) maxima[part * 128 + (tid & 127)] = l;
+        __syncthreads();
+        if (softmax_on) l = maxima[tid & 127] + maxima[128 + (tid & 127)];
+    }
     if (softmax_on) {
         const long long row = sq.row0 + my_rr / a.G;
         const int h = kvh * a.G + my_rr % a.G;
         const bool live = my_rr < n_rows;
         const long long at = (static_cast<long long>(split) * p.batch.rows + row) * p.q_heads + h;
         const float inv = partial ? 1.f : (l == 0.f ? 0.f : 1.f / l);
-        if (partial && live) a.ml[at] = make_float2(m, l);
+        if (partial && live && part == 0) a.ml[at] = make_float2(m, l);
         const bool repair = *reinterpret_cast<volatile int*>(words + 2) != 0;
         bf16* out = static_cast<bf16*>(p.out) + row * p.ldo + static_cast<long long>(h) * D;
-        for (int c = 0; c < D; c += 16) {
+        for (int c = part * 16; c < D; c += kParts * 16) {
             uint32_t r[16];
             tmem_ld16(my_lanes + Sh::kO + rt * DP + c, r);
             tmem_wait_ld();
@@ -753,11 +826,11 @@ void launch(const Args& a, dim3 grid, cudaStream_t st) {
         SANA_CUDA(cudaFuncSetAttribute(paged_tc_kernel<DP, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem));
         once.mark();
     }
-    const int k_box = copy_box(a.p.cache, kKeys), v_box = k_box > 0 ? copy_box(a.p.cache, Sh::kPieceKeys) : 0;
+    const int k_box = copy_box(a.p.cache, kKeys), v_box = k_box > 0 ? copy_box(a.p.cache, Sh::kBlock) : 0;
     CUtensorMap k{}, v{};
     if (k_box > 0) {
         k = pool_map(a.p.cache, a.p.cache.k, k_box);
-        v = a.p.cache.D % 64 == 0 ? pool_map_slabs(a.p.cache, a.p.cache.v, v_box) : pool_map(a.p.cache, a.p.cache.v, v_box);
+        v = Sh::kPieces > 1 && a.p.cache.D % 64 == 0 ? pool_map_slabs(a.p.cache, a.p.cache.v, v_box) : pool_map(a.p.cache, a.p.cache.v, v_box);
     }
     paged_tc_kernel<DP, CAP><<<grid, kThreads, Sh::kSmem, st>>>(a, k, v, k_box, v_box);
 }
