@@ -74,7 +74,7 @@ struct RotaryRows {
 };
 void rotary_rows(const RotaryRows& p, bool append, cudaStream_t st);
 
-struct PageDivisor {  // division by the page size as a product (pattn.cu)
+struct PageDivisor {  // division by the page size (or another number) as a product (pattn.cu)
     uint32_t magic;
     int shift;
 };

@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
     for (int i = tid; i < BM * (DP / 8); i += 128) {
         const int r = i / (DP / 8), c = i % (DP / 8), rr = rr0 + r;
         const bool in = rr < n_rows && c * 8 < D;
-        const int t = rr / a.G;
+        const int t = head_group(a, rr);
         const bf16* src = in ? q + (sq.row0 + t) * p.ldq + static_cast<long long>(kvh * a.G + rr - t * a.G) * D + c * 8 : q;
         cp_async16(q_s + swz(BM, r, c), src, in);
     }
@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int rr = rr0 + wm * 16 + (lane >> 2) + 8 * i;
-        pos[i] = rr < n_rows ? sq.past + rr / a.G : -1;
+        pos[i] = rr < n_rows ? sq.past + head_group(a, rr) : -1;
     }
     const float scale_log2 = p.scale * kLog2e;
     const float cap_in = p.softcap > 0.f ? 2.f * scale_log2 / p.softcap : 0.f, cap_out = p.softcap * kLog2e;
@@ -593,7 +593,7 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = fmaf(src[e], f, v[e]);
         }
-        const int t = rr / a.G, h = kvh * a.G + rr - t * a.G;
+        const int t = head_group(a, rr), h = kvh * a.G + rr - t * a.G;
         const long long row = sq.row0 + t;
         if (partial) {
             const long long at = (static_cast<long long>(split) * p.batch.rows + row) * p.q_heads + h;
@@ -704,6 +704,7 @@ Args plan(const PagedAttention& p, Kind kind, int num_sms) {
     Args a{};
     a.p = p;
     a.G = p.q_heads / p.cache.kv_heads;
+    a.g_div = page_divisor(a.G);
     const long long packed = static_cast<long long>(p.batch.max_new) * a.G;
     a.align = 1;
     int resident;  // blocks per SM

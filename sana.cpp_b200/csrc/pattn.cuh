@@ -25,6 +25,7 @@ namespace pattn {
 struct Args {
     PagedAttention p;
     int G;            // query heads per cache head
+    PageDivisor g_div;  // division by it
     int row_tiles;    // of BM packed rows, per sequence
     int BM, BN;
     int splits, split_tiles;
@@ -98,7 +99,10 @@ __device__ __forceinline__ bool seen(int j, int pos, int window, int sinks) {
     return j <= pos && (window <= 0 || j > pos - window || j < sinks);
 }
 
-PageDivisor page_divisor(int page_size);
+PageDivisor page_divisor(int d);
+__device__ __forceinline__ int head_group(const Args& a, int rr) {  // the token of packed row rr: rr / G
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(rr), a.g_div.magic) + static_cast<uint32_t>(rr)) >> a.g_div.shift);
+}
 __device__ __forceinline__ int page_slot(const PagedAttention& p, int j) {  // j / page_size, 0 <= j < 2^30
     return static_cast<int>((__umulhi(static_cast<uint32_t>(j), p.page_div.magic) + static_cast<uint32_t>(j)) >> p.page_div.shift);
 }
@@ -117,7 +121,7 @@ __device__ __forceinline__ long long key_offset(const PagedAttention& p, int s, 
 // Whether the page of any of the keys [lo, hi) is not in the pool; the block's threads share out the pages.
 __device__ __forceinline__ bool any_bad_page(const PagedAttention& p, int s, int lo, int hi) {
     bool bad = false;
-    for (int j = lo / p.cache.page_size + static_cast<int>(threadIdx.x); j <= (hi - 1) / p.cache.page_size;
+    for (int j = page_slot(p, lo) + static_cast<int>(threadIdx.x), last = page_slot(p, hi - 1); j <= last;
          j += static_cast<int>(blockDim.x))
         bad = key_offset(p, s, min(max(j * p.cache.page_size, lo), hi - 1)) < 0 || bad;
     return bad;

@@ -57,7 +57,7 @@ struct TcShape {
     static constexpr int kPieceBytes = kKeys * DP * 2 / kPieces;
     static constexpr int kKRing = DP == 64 ? 4 : DP == 128 ? 2 : 5, kVRing = DP == 64 ? 4 : DP == 128 ? 2 : 4;  // pieces
     static constexpr int kQBytes = kTiles * 128 * DP * 2;
-    static constexpr int kBarriers = 2 * (kKRing + kVRing) + 8 + 2;
+    static constexpr int kBarriers = 2 * (kKRing + kVRing) + 8 + 3;
     // behind Q and the rings: keys' offsets [2 for K, 2 for V][kKeys] (cp.async), maxima [2][kParts][128], barriers, three words
     static constexpr int kVRingAt = kQBytes + kKRing * kPieceBytes;
     static constexpr int kOffs = kVRingAt + kVRing * kPieceBytes;
@@ -283,8 +283,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     auto p_early = [&](int i) { return bars + 8u * (2 * NK + 2 * NV + 2 + i); };
     auto p_full = [&](int i) { return bars + 8u * (2 * NK + 2 * NV + 4 + i); };
     auto pv_done = [&](int i) { return bars + 8u * (2 * NK + 2 * NV + 6 + i); };
-    const uint32_t drained = bars + 8u * (2 * NK + 2 * NV + 8), v_raw = drained + 8u;
-    int* words = reinterpret_cast<int*>(sm + Sh::kBars + Sh::kBarriers * 8);  // [0] tensor memory, [1] bad page, [2] not finite
+    const uint32_t drained = bars + 8u * (2 * NK + 2 * NV + 8), v_raw = drained + 8u, q_full = v_raw + 8u;
+    int* words = reinterpret_cast<int*>(sm + Sh::kBars + Sh::kBarriers * 8);  // [0] tensor memory, [1] not finite
 
     if (warp == kMmaWarp) {
         tmem_alloc(smem_u32(words), 512);
@@ -307,43 +307,41 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         }
         mbar_init(drained, 1);
         mbar_init(v_raw, 1);
+        mbar_init(q_full, kSoftmaxWarps * 32);
         fence_barrier_init();
         words[1] = 0;
-        words[2] = 0;
     }
-    // Q: every thread helps
-    {
-        const bf16* q = static_cast<const bf16*>(p.q);
-        const int rows = pair ? 256 : 128;
-        for (int i = tid; i < rows * (DP / 8); i += kThreads) {
-            const int r = i / (DP / 8), c = i % (DP / 8), rr = rr0 + r;
-            const bool in = rr < n_rows && c * 8 < D;
-            const int t = rr / a.G;
-            const bf16* src = in ? q + (sq.row0 + t) * p.ldq + static_cast<long long>(kvh * a.G + rr - t * a.G) * D + c * 8 : q;
-            const int rt = r & 127;
-            cp_async16(q_s + (r >> 7) * (128 * DP * 2) + (c >> 3) * (128 * 128) + rt * 128 + (((c & 7) ^ (rt & 7)) << 4), src, in);
-        }
-        cp_async_commit();
-    }
-    __syncthreads();  // words[] are set; the pages of this block's keys are checked while Q is on its way
-    if (any_bad_page(p, s, kt, t0, n, BN)) words[1] = 1;
-    cp_async_wait<0>();
-    fence_proxy_async_smem();
+    const bool bad_here = any_bad_page(p, s, kt, t0, n, BN);
     tc_fence_before();
-    __syncthreads();
+    const bool bad_page = __syncthreads_or(bad_here);  // (and the barriers and words[] are set)
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(words);
-    const bool bad_page = *reinterpret_cast<volatile int*>(words + 1) != 0;
-
     float* maxima = reinterpret_cast<float*>(sm + Sh::kMax);
     // a softmax thread's row tile, part of the row, and row; tensor memory lanes 32 (warp & 3) ..
     const int rt = kParts == 1 ? warp >> 2 : 0, part = kParts == 1 ? 0 : warp >> 2, my_rr = rr0 + rt * 128 + (tid & 127);
-    const int my_pos = my_rr < n_rows ? sq.past + my_rr / a.G : -1;
+    const int my_pos = my_rr < n_rows ? sq.past + head_group(a, my_rr) : -1;
     const uint32_t my_lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);
     const bool softmax_on = warp < kSoftmaxWarps && (kParts > 1 || rt == 0 || pair);
     float m = -INFINITY, l = 0.f;
 
     if (warp < kSoftmaxWarps) {
+        // Q, by the softmax warps, which have nothing else to do yet; only the issuing warp waits for it
+        {
+            constexpr int kChunks = DP / 8, kRowsPerPass = kSoftmaxWarps * 32 / kChunks;
+            const bf16* q = static_cast<const bf16*>(p.q);
+            const int rows = pair ? 256 : 128, c = tid % kChunks;
+#pragma unroll 4
+            for (int r = tid / kChunks; r < rows; r += kRowsPerPass) {
+                const int rr = rr0 + r, t = head_group(a, rr), lr = r & 127;
+                const bool in = rr < n_rows && c * 8 < D;
+                const bf16* src = in ? q + (sq.row0 + t) * p.ldq + static_cast<long long>(kvh * a.G + rr - t * a.G) * D + c * 8 : q;
+                cp_async16(q_s + (r >> 7) * (128 * DP * 2) + (c >> 3) * (128 * 128) + lr * 128 + (((c & 7) ^ (lr & 7)) << 4), src, in);
+            }
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        fence_proxy_async_smem();
+        mbar_arrive(q_full);
         if (softmax_on) {
             const float scale_log2 = p.scale * kLog2e;
             const float cap_in = CAP ? 2.f * scale_log2 / p.softcap : 0.f, cap_out = p.softcap * kLog2e;
@@ -525,29 +523,35 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         const int block = Sh::kPieces > 1 && tma ? v_box : Sh::kBlock;  // keys of a block
         // Values that are not finite, in a tile that not every row sees whole, would reach the rows that do
         // not see them as 0 * v: zeros take their place, and the rows that see them get them at the end.
-        // Keys from `keys` on, and those of bad pages, are zeros outright (a tensor copy brought what lies there).
+        // Keys from `keys` on, and those of bad pages, are zeros outright (a tensor copy brought what lies there). Keys that
+        // every row sees are left alone.
         auto clean = [&](unsigned char* v, int key0, int start, int keys) {
-            for (int slab = 0; slab < slabs; ++slab) {
-                for (int key = pt >> 3; key < Sh::kPieceKeys; key += kValueThreads / 8) {
-                    const int row = key & (block - 1);
-                    uint4* w = reinterpret_cast<uint4*>(v + (key - row) * (kSlabs * 128) + slab * (block * 128) + row * 128 +
-                                                        (((pt & 7) ^ (row & 7)) << 4));
-                    if (key0 + key >= keys || (bad_page && key_offset(p, s, start + key0 + key) < 0)) {
-                        *w = make_uint4(0, 0, 0, 0);
-                        continue;
-                    }
-                    const uint4 c = *w;
-                    uint32_t e[4] = {c.x, c.y, c.z, c.w};
-                    bool bad = false;
+#pragma unroll 2
+            for (int key = pt >> 3; key < Sh::kPieceKeys; key += kValueThreads / 8) {
+                const int at = start + key0 + key, row = key & (block - 1);
+                const bool absent = key0 + key >= keys || (bad_page && key_offset(p, s, at) < 0);
+                if (!absent && at <= kt.pmin && (p.window <= 0 || at < p.sinks || at > kt.pmax - p.window)) continue;
+                uint4* w = reinterpret_cast<uint4*>(v + (key - row) * (kSlabs * 128) + row * 128 + (((pt & 7) ^ (row & 7)) << 4));
+                const int step = block * (128 / 16);  // from slab to slab
+                uint4 c[kSlabs];
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                        if ((e[y] & 0x7f80u) == 0x7f80u) e[y] &= 0xffff0000u, bad = true;
-                        if ((e[y] & 0x7f800000u) == 0x7f800000u) e[y] &= 0x0000ffffu, bad = true;
-                    }
+                for (int x = 0; x < kSlabs; ++x) c[x] = x < slabs && !absent ? w[x * step] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int x = 0; x < kSlabs; ++x) {
+                    uint32_t e[4] = {c[x].x, c[x].y, c[x].z, c[x].w}, top = 0;
+                    // an exponent of all ones carries into the bit above it
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) top |= (e[y] & 0x7f807f80u) + 0x00800080u;
+                    const bool bad = (top & 0x80008000u) != 0;
                     if (bad) {
-                        *w = make_uint4(e[0], e[1], e[2], e[3]);
-                        words[2] = 1;
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            if ((e[y] & 0x7f80u) == 0x7f80u) e[y] &= 0xffff0000u;
+                            if ((e[y] & 0x7f800000u) == 0x7f800000u) e[y] &= 0x0000ffffu;
+                        }
+                        words[1] = 1;
                     }
+                    if (x < slabs && (bad || absent)) w[x * step] = make_uint4(e[0], e[1], e[2], e[3]);
                 }
             }
         };
@@ -740,7 +744,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 return true;
             };
             const int units = kPair ? 2 * n : n;
-            bool ok = scores(0, 0) && (units < 2 || scores(1, 1));
+            bool ok = warp_wait(q_full, 0, p.err) && scores(0, 0) && (units < 2 || scores(1, 1));
             for (int u = 0; u < units && ok; u += 2) {
                 ok = values(u, 0) && (u + 2 >= units || scores(u + 2, 0));
                 if (ok && u + 1 < units) ok = values(u + 1, 1) && (u + 3 >= units || scores(u + 3, 1));
@@ -768,15 +772,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         const long long at = (static_cast<long long>(split) * p.batch.rows + row) * p.q_heads + h;
         const float inv = partial ? 1.f : (l == 0.f ? 0.f : 1.f / l);
         if (partial && live && part == 0) a.ml[at] = make_float2(m, l);
-        const bool repair = *reinterpret_cast<volatile int*>(words + 2) != 0;
+        const bool repair = *reinterpret_cast<volatile int*>(words + 1) != 0;
         bf16* out = static_cast<bf16*>(p.out) + row * p.ldo + static_cast<long long>(h) * D;
-        for (int c = part * 16; c < D; c += kParts * 16) {
-            uint32_t r[16];
-            tmem_ld16(my_lanes + Sh::kO + rt * DP + c, r);
+        for (int c = part * 32; c < D; c += kParts * 32) {
+            uint32_t r[32];
+            tmem_ld32(my_lanes + Sh::kO + rt * DP + c, r);
             tmem_wait_ld();
-            float o[16];
+            float o[32];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __uint_as_float(r[i]) * inv;
+            for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(r[i]) * inv;
             if (repair && live) {
                 const bf16* vc = static_cast<const bf16*>(p.cache.v) + kvh * p.cache.head_stride;
                 for (int t = 0; t < n; ++t) {
@@ -788,7 +792,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         const long long off = key_offset(p, s, j);
                         if (off < 0) continue;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
+                        for (int i = 0; i < 32; ++i) {
                             if (c + i >= D) continue;
                             const float v = __bfloat162float(vc[off + c + i]);
                             if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) o[i] += v;
@@ -798,7 +802,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             }
             if (!live) continue;
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
+            for (int b = 0; b < 4; ++b) {
                 if (c + 8 * b >= D) continue;
                 const float* x = o + 8 * b;
                 if (partial) {
