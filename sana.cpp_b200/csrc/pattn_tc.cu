@@ -55,7 +55,7 @@ struct TcShape {
     static constexpr int kPieceKeys = kKeys / kPieces;   // of V
     static constexpr int kBlock = DP <= 128 ? kKeys : 16;  // keys of a block of V (8 of them where pages are of 8)
     static constexpr int kPieceBytes = kKeys * DP * 2 / kPieces;
-    static constexpr int kKRing = DP == 64 ? 4 : DP == 128 ? 2 : 5, kVRing = DP == 64 ? 4 : DP == 128 ? 2 : 4;  // pieces
+    static constexpr int kKRing = DP == 64 ? 4 : DP == 128 ? 2 : 4, kVRing = DP == 64 ? 4 : DP == 128 ? 2 : 5;  // pieces
     static constexpr int kQBytes = kTiles * 128 * DP * 2;
     static constexpr int kBarriers = 2 * (kKRing + kVRing) + 8 + 3;
     // behind Q and the rings: keys' offsets [2 for K, 2 for V][kKeys] (cp.async), maxima [2][kParts][128], barriers, three words
@@ -171,31 +171,6 @@ __device__ __forceinline__ bool meet_all(int id, int threads, bool ok) {
     return all != 0;
 }
 __device__ __forceinline__ bool value_warps(bool ok) { return meet_all(1, kValueThreads, ok); }
-// 2^x of a pair on the FMA pipe, |x| <= 125: x = n + f with n the nearest whole number, 2^f on [-1/2, 1/2] by the
-// degree-4 polynomial of least largest relative error (2.7e-6; fitted by linear programming over Chebyshev nodes), 2^n as
-// exponent bits: n + 127 is left in the low bits of x + 1.5 2^23 + 127.
-__device__ __forceinline__ uint64_t exp2_poly2(uint64_t x) {
-    constexpr float kMagic = 12582912.0f + 127.0f;
-    const uint64_t t = add2(x, f2_make(kMagic, kMagic));
-    const uint64_t f = sub2(x, sub2(t, f2_make(kMagic, kMagic)));
-    uint64_t q = fma2(f, f2_make(9.567709878e-03f, 9.567709878e-03f), f2_make(5.591749132e-02f, 5.591749132e-02f));
-    q = fma2(q, f, f2_make(2.402481151e-01f, 2.402481151e-01f));
-    q = fma2(q, f, f2_make(6.931219409e-01f, 6.931219409e-01f));
-    q = fma2(q, f, f2_make(9.999992499e-01f, 9.999992499e-01f));
-    const float2 n = f2_split(t);
-    return mul2(q, f2_make(__uint_as_float(__float_as_uint(n.x) << 23), __uint_as_float(__float_as_uint(n.y) << 23)));
-}
-// The cap of a pair. Of its two special functions and the probability's one, which bound the softmax of capped scores
-// (16 a clock and SM), the first exponential is taken on the FMA pipe: e^2z (1 + 3e-6) changes tanh z by at most 1.4e-6.
-// Beyond |2z log2 e| = 40 tanh z is 1 in fp32 either way; NaN stays NaN.
-__device__ __forceinline__ uint64_t soft_cap_log2_2(uint64_t x, float in, float out) {
-    float2 z = f2_split(mul2(x, f2_make(in, in)));
-    asm("{\n\t.reg .f32 t;\n\tmax.NaN.f32 t, %0, 0fC2200000;\n\tmin.NaN.f32 %0, t, 0f42200000;\n\t}" : "+f"(z.x));
-    asm("{\n\t.reg .f32 t;\n\tmax.NaN.f32 t, %0, 0fC2200000;\n\tmin.NaN.f32 %0, t, 0f42200000;\n\t}" : "+f"(z.y));
-    const float2 d = f2_split(add2(exp2_poly2(f2_make(z.x, z.y)), f2_make(1.f, 1.f)));
-    return fma2(f2_make(-2.f * out, -2.f * out), f2_make(rcp_approx(d.x), rcp_approx(d.y)), f2_make(out, out));
-}
-
 // Bit i: the row at position pos sees key j0 + i, below `end`.
 __device__ __forceinline__ uint32_t low_bits(int n) {  // the n lowest bits, n of any sign and size
     return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
@@ -245,6 +220,49 @@ __device__ __forceinline__ void copy_rows(uint32_t dst, const bf16* src, const l
     }
 }
 
+// Values that are not finite, in a tile that not every row sees whole, would reach the rows that do not see them as 0 * v:
+// zeros take their place in `count` keys from `first` of tile j, before the products read them, and the rows that see them
+// get them at the end (*found is set). Keys from `end` on, and those of bad pages, are zeros outright (a tensor copy brought
+// what lies there). Keys that every row of kt sees are left alone. By THREADS threads: with two threads per row by those,
+// each the keys of its own scores, before they hand P over; with one by the value warps, since the registers are missing
+// in the softmax (2048 tokens after 8192, head size 128: 202 us there, 175 here; head size 256: 310 there, 339 here).
+template <int DP, int THREADS>
+__device__ __forceinline__ void clean_values(const PagedAttention& p, int s, const KeyTiles& kt, unsigned char* ring, int* found,
+                                             int j, int start, int end, int first, int count, int block, bool bad_page) {
+    using Sh = TcShape<DP>;
+    constexpr int kSlabs = Sh::kSlabs;
+    const int t = threadIdx.x % THREADS, slabs = (p.cache.D + 63) / 64;
+#pragma unroll 1
+    for (int key = first + (t >> 3); key < first + count; key += THREADS / 8) {
+        const int at = start + key, in = key % Sh::kPieceKeys, row = in & (block - 1);
+        const bool absent = at >= end || (bad_page && key_offset(p, s, at) < 0);
+        if (!absent && at <= kt.pmin && (p.window <= 0 || at < p.sinks || at > kt.pmax - p.window)) continue;
+        uint4* w = reinterpret_cast<uint4*>(ring + ((j * Sh::kPieces + key / Sh::kPieceKeys) % Sh::kVRing) * Sh::kPieceBytes +
+                                            (in - row) * (kSlabs * 128) + row * 128 + (((t & 7) ^ (row & 7)) << 4));
+        const int step = block * (128 / 16);  // from slab to slab
+        uint4 c[kSlabs];
+#pragma unroll
+        for (int x = 0; x < kSlabs; ++x) c[x] = x < slabs && !absent ? w[x * step] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int x = 0; x < kSlabs; ++x) {
+            uint32_t e[4] = {c[x].x, c[x].y, c[x].z, c[x].w}, top = 0;
+            // an exponent of all ones carries into the bit above it
+#pragma unroll
+            for (int y = 0; y < 4; ++y) top |= (e[y] & 0x7f807f80u) + 0x00800080u;
+            const bool bad = (top & 0x80008000u) != 0;
+            if (bad) {
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    if ((e[y] & 0x7f80u) == 0x7f80u) e[y] &= 0xffff0000u;
+                    if ((e[y] & 0x7f800000u) == 0x7f800000u) e[y] &= 0x0000ffffu;
+                }
+                *found = 1;
+            }
+            if (x < slabs && (bad || absent)) w[x * step] = make_uint4(e[0], e[1], e[2], e[3]);
+        }
+    }
+}
+
 template <int DP, bool CAP>
 __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_constant__ Args a,
                                                                const __grid_constant__ CUtensorMap k_map,
@@ -283,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     auto p_early = [&](int i) { return bars + 8u * (2 * NK + 2 * NV + 2 + i); };
     auto p_full = [&](int i) { return bars + 8u * (2 * NK + 2 * NV + 4 + i); };
     auto pv_done = [&](int i) { return bars + 8u * (2 * NK + 2 * NV + 6 + i); };
-    const uint32_t drained = bars + 8u * (2 * NK + 2 * NV + 8), v_raw = drained + 8u, q_full = v_raw + 8u;
+    const uint32_t drained = bars + 8u * (2 * NK + 2 * NV + 8), q_full = drained + 8u, v_raw = q_full + 8u;
     int* words = reinterpret_cast<int*>(sm + Sh::kBars + Sh::kBarriers * 8);  // [0] tensor memory, [1] not finite
 
     if (warp == kMmaWarp) {
@@ -323,6 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     const uint32_t my_lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);
     const bool softmax_on = warp < kSoftmaxWarps && (kParts > 1 || rt == 0 || pair);
     float m = -INFINITY, l = 0.f;
+    const int v_block = kPieces > 1 && tma ? v_box : Sh::kBlock;  // keys of a block of V
 
     if (warp < kSoftmaxWarps) {
         // Q, by the softmax warps, which have nothing else to do yet; only the issuing warp waits for it
@@ -356,7 +375,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 int start, end;
                 key_range(kt, t0 + j, BN, start, end);
                 const bool whole = end - start == BN && !bad_page && all_seen(mine, start, end, p.window, p.sinks);
-                start += part * kCols;
                 const uint32_t s_t = my_lanes + slot * BN;
                 ok = ok && warp_wait(s_full(slot), turn & 1, p.err);
                 if (kParts == 1 && !ok) break;
@@ -371,10 +389,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     if (!whole) {
 #pragma unroll
                         for (int c = 0; c < kCols / 32; ++c) {
-                            uint32_t bits = seen_bits(start + c * 32, end, my_pos, p.window, p.sinks);
+                            const int j0 = start + part * kCols + c * 32;
+                            uint32_t bits = seen_bits(j0, end, my_pos, p.window, p.sinks);
                             if (bad_page) {
                                 for (int i = 0; i < 32; ++i)
-                                    if ((bits >> i & 1u) && key_offset(p, s, start + c * 32 + i) < 0) bits &= ~(1u << i);
+                                    if ((bits >> i & 1u) && key_offset(p, s, j0 + i) < 0) bits &= ~(1u << i);
                             }
 #pragma unroll
                             for (int i = 0; i < 32; ++i)
@@ -409,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                     if (j > 0) {  // O holds sums against the old reference; each part rescales some of its channels
                         const int slot0 = pair ? rt : (j - 1) & 1, turn0 = pair ? j - 1 : (j - 1) >> 1;
                         ok = warp_wait(pv_done(slot0), turn0 & 1, p.err);
-                        if (!ok) continue;  // (to tell the row's other threads)
+                        if (!ok) continue;  // (to tell the row's other threads, or to leave)
                         tc_fence_after();
                         for (int c = part * 16; c < D; c += kParts * 16) {
                             uint32_t r[16];
@@ -432,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         const float x0 = __uint_as_float(x[c * 32 + 2 * i]), x1 = __uint_as_float(x[c * 32 + 2 * i + 1]);
                         uint64_t e;
                         if constexpr (CAP) {
-                            e = add2(soft_cap_log2_2(f2_make(x0, x1), cap_in, cap_out), r2);
+                            e = add2(f2_make(soft_cap_log2(x0, cap_in, cap_out), soft_cap_log2(x1, cap_in, cap_out)), r2);
                             const float2 v = f2_split(e);  // the cap maps what is masked to a number: it stays masked
                             if (!whole) e = f2_make(x0 == -INFINITY ? x0 : v.x, x1 == -INFINITY ? x1 : v.y);
                         } else {
@@ -453,6 +472,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 }
                 const float2 total = f2_split(add2(sum[0], sum[1]));
                 l += total.x + total.y;
+                if (kParts > 1 && !whole) {  // the values of this part's keys
+                    for (int pc = part * (kPieces / kParts); pc < (part + 1) * kPieces / kParts && ok; ++pc) {
+                        const int g = j * kPieces + pc;
+                        ok = warp_wait(v_full(g % NV), (g / NV) & 1, p.err);
+                    }
+                    if (!ok) continue;  // (as above)
+                    clean_values<DP, 128>(p, s, mine, sm + Sh::kVRingAt, words + 1, j, start, end, part * kCols, kCols,
+                                          v_block, bad_page);
+                    fence_proxy_async_smem();
+                }
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -519,43 +548,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
             cp_async_wait<0>();
         }
     } else if (warp < kMmaWarp) {
+        constexpr bool kClean = kParts == 1;
         const int pt = tid - kValueWarp * 32, slabs = (D + 63) / 64;
-        const int block = Sh::kPieces > 1 && tma ? v_box : Sh::kBlock;  // keys of a block
-        // Values that are not finite, in a tile that not every row sees whole, would reach the rows that do
-        // not see them as 0 * v: zeros take their place, and the rows that see them get them at the end.
-        // Keys from `keys` on, and those of bad pages, are zeros outright (a tensor copy brought what lies there). Keys that
-        // every row sees are left alone.
-        auto clean = [&](unsigned char* v, int key0, int start, int keys) {
-#pragma unroll 2
-            for (int key = pt >> 3; key < Sh::kPieceKeys; key += kValueThreads / 8) {
-                const int at = start + key0 + key, row = key & (block - 1);
-                const bool absent = key0 + key >= keys || (bad_page && key_offset(p, s, at) < 0);
-                if (!absent && at <= kt.pmin && (p.window <= 0 || at < p.sinks || at > kt.pmax - p.window)) continue;
-                uint4* w = reinterpret_cast<uint4*>(v + (key - row) * (kSlabs * 128) + row * 128 + (((pt & 7) ^ (row & 7)) << 4));
-                const int step = block * (128 / 16);  // from slab to slab
-                uint4 c[kSlabs];
-#pragma unroll
-                for (int x = 0; x < kSlabs; ++x) c[x] = x < slabs && !absent ? w[x * step] : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                for (int x = 0; x < kSlabs; ++x) {
-                    uint32_t e[4] = {c[x].x, c[x].y, c[x].z, c[x].w}, top = 0;
-                    // an exponent of all ones carries into the bit above it
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) top |= (e[y] & 0x7f807f80u) + 0x00800080u;
-                    const bool bad = (top & 0x80008000u) != 0;
-                    if (bad) {
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            if ((e[y] & 0x7f80u) == 0x7f80u) e[y] &= 0xffff0000u;
-                            if ((e[y] & 0x7f800000u) == 0x7f800000u) e[y] &= 0x0000ffffu;
-                        }
-                        words[1] = 1;
-                    }
-                    if (x < slabs && (bad || absent)) w[x * step] = make_uint4(e[0], e[1], e[2], e[3]);
-                }
-            }
+        auto is_edge = [&](int start, int end) {
+            return kClean && (end - start < BN || bad_page || !all_seen(kt, start, end, p.window, p.sinks));
         };
-        auto at_piece = [&](int g) { return sm + Sh::kVRingAt + (g % NV) * Sh::kPieceBytes; };
         bool ok = true;
         if (tma) {
             // as for K, by the first value warp; the second helps to clean and keeps step, waiting for no place
@@ -572,33 +569,32 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 const int at = start + lane * v_box - page_slot(p, start + lane * v_box) * p.cache.page_size;
                 const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
                 const uint32_t box_bytes = static_cast<uint32_t>(v_box) * 128 * slabs;
-                const bool edge = end - start < BN || bad_page || !all_seen(kt, start, end, p.window, p.sinks);
-                if (warp == kValueWarp) {
-                    if (edge && leader) mbar_arrive_expect_tx(v_raw, __popc(there) * box_bytes);
-                    for (int pc = 0; pc < kPieces && ok; ++pc) {
-                        const int g = j * kPieces + pc, slot = g % NV;
-                        ok = warp_wait(v_empty(slot), ((g / NV) & 1) ^ 1, p.err);
-                        if (!ok) continue;
-                        const uint32_t bar = edge ? v_raw : v_full(slot);
-                        if (!edge && leader) {
-                            const unsigned mine = there >> (pc * boxes_piece) & ((1u << boxes_piece) - 1u);
-                            mbar_arrive_expect_tx(bar, __popc(mine) * box_bytes);
-                        }
-                        __syncwarp();
-                        uint32_t dst = v_ring + slot * Sh::kPieceBytes;
-                        for (int b = pc * boxes_piece; b < (pc + 1) * boxes_piece; ++b, dst += v_box * (kPieces > 1 ? kSlabs * 128 : 128)) {
-                            const int pg = __shfl_sync(0xffffffffu, page, b), row = __shfl_sync(0xffffffffu, at, b);
-                            if (leader && pg >= 0) {
-                                if (all_slabs) {
-                                    tma_load_5d(&v_map, dst, bar, 0, row, 0, kvh, pg);
-                                } else {
-                                    for (int x = 0; x < slabs; ++x) tma_load_4d(&v_map, dst + x * (block * 128), bar, x * 64, row, kvh, pg);
-                                }
+                const bool edge = is_edge(start, end);
+                for (int pc = 0; pc < kPieces && ok && warp == kValueWarp; ++pc) {
+                    const int g = j * kPieces + pc, slot = g % NV;
+                    ok = warp_wait(v_empty(slot), ((g / NV) & 1) ^ 1, p.err);
+                    if (!ok) continue;
+                    const uint32_t bar = edge ? v_raw : v_full(slot);
+                    const unsigned mine = there >> (pc * boxes_piece) & ((1u << boxes_piece) - 1u);
+                    if (leader) mbar_arrive_expect_tx(bar, __popc(mine) * box_bytes);
+                    __syncwarp();
+                    uint32_t dst = v_ring + slot * Sh::kPieceBytes;
+                    for (int b = pc * boxes_piece; b < (pc + 1) * boxes_piece; ++b, dst += v_box * (kPieces > 1 ? kSlabs * 128 : 128)) {
+                        const int pg = __shfl_sync(0xffffffffu, page, b), row = __shfl_sync(0xffffffffu, at, b);
+                        if (leader && pg >= 0) {
+                            if (all_slabs) {
+                                tma_load_5d(&v_map, dst, bar, 0, row, 0, kvh, pg);
+                            } else {
+                                for (int x = 0; x < slabs; ++x) tma_load_4d(&v_map, dst + x * (v_block * 128), bar, x * 64, row, kvh, pg);
                             }
                         }
-                        if (!edge) issued = g + 1;
                     }
-                    in_flight = edge;
+                    if (edge) in_flight = true;
+                    else issued = g + 1;
+                }
+                if (!kClean) {
+                    if (!ok || warp != kValueWarp) break;
+                    continue;
                 }
                 ok = value_warps(ok);
                 if (!ok) break;
@@ -607,12 +603,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 if (!ok) break;
                 in_flight = false;
                 ++raw;
-                for (int pc = 0; pc < kPieces; ++pc) clean(at_piece(j * kPieces + pc), pc * Sh::kPieceKeys, start, end - start);
+                clean_values<DP, kValueThreads>(p, s, kt, sm + Sh::kVRingAt, words + 1, j, start, end, 0, BN, v_block, bad_page);
                 fence_proxy_async_smem();
                 value_warps(true);
-                if (pt == 0)
-                    for (int pc = 0; pc < kPieces; ++pc) mbar_arrive(v_full((j * kPieces + pc) % NV));
-                issued = (j + 1) * kPieces;
+                if (pt == 0) mbar_arrive(v_full(j % NV));
+                issued = j + 1;
             }
             if (!ok && warp == kValueWarp) {
                 if (in_flight) mbar_wait_quiet(v_raw, raw & 1);
@@ -632,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 if (j + 1 < n) tile_offsets<kValueThreads>(p, s, kt, t0 + j + 1, pt, next);
                 int start, end;
                 key_range(kt, t0 + j, BN, start, end);
-                const bool edge = !all_seen(kt, start, end, p.window, p.sinks);
+                const bool edge = is_edge(start, end);
                 for (int pc = 0; pc < kPieces && ok; ++pc) {
                     const int g = j * kPieces + pc, slot = g % NV;
                     ok = warp_wait(v_empty(slot), ((g / NV) & 1) ^ 1, p.err);
@@ -644,10 +639,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 if (!edge || !ok) continue;
                 cp_async_commit();
                 cp_async_wait<0>();
-                for (int pc = 0; pc < kPieces; ++pc) {  // each thread what it has copied itself
-                    clean(at_piece(j * kPieces + pc), pc * Sh::kPieceKeys, start, end - start);
-                    mbar_arrive(v_full((j * kPieces + pc) % NV));
-                }
+                ok = value_warps(true);  // both warps' copies are there (what a thread cleans, another may have copied)
+                clean_values<DP, kValueThreads>(p, s, kt, sm + Sh::kVRingAt, words + 1, j, start, end, 0, BN, v_block, bad_page);
+                mbar_arrive(v_full(j % NV));
             }
             cp_async_commit();
             cp_async_wait<0>();
@@ -655,13 +649,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     } else {
         // The whole warp walks the tiles, so that all it computes is uniform; one elected thread issues.
         const int d16 = (D + 15) & ~15, k_steps = d16 / 16;
-        const int block = Sh::kPieces > 1 && tma ? v_box : Sh::kBlock;
         const uint32_t t_mem = __shfl_sync(0xffffffffu, tmem, 0);
         const uint32_t idesc_s = idesc_bf16_f32(128, BN);
         const uint32_t idesc_o = idesc_bf16_f32(128, d16) | kBTransposed;
         // descriptors of the first operands; the others differ in the address field alone (16-byte units)
         const uint64_t q_desc = kmajor_sw128_desc(q_s), k_desc = kmajor_sw128_desc(k_ring);
-        const uint64_t v_desc = mnmajor_sw128_desc(v_ring, block * 128, block == 8 ? kSlabs * 1024 : 1024);
+        const uint64_t v_desc = mnmajor_sw128_desc(v_ring, v_block * 128, v_block == 8 ? kSlabs * 1024 : 1024);
         const uint32_t leader = elect_one();
         auto piece_there = [&](uint32_t bar, int turn) -> bool {
             if (!warp_wait(bar, turn & 1, p.err)) return false;
