@@ -21,65 +21,101 @@ constexpr float kNegInf = -INFINITY;
 
 // --- CUDA cores -------------------------------------------------------------------------------
 // 32 packed rows x 32 keys per step, four threads per row: thread c of a row takes keys c + 4 i of
-// the scores and channels 4 c + 16 i of the output. q, k and v sit in shared memory as fp32 rows
-// padded by four words, so that the eight rows (or four keys) a warp reads at once lie in
-// different banks.
+// the scores and channels 4 c + 16 i of the output; for the copies, thread c of key tid / 4 takes the
+// same channels of that key. q, k and v sit in shared memory as fp32 rows padded by four words, so
+// that the eight rows (or four keys) a warp reads at once lie in different banks. fp32 keys and
+// values come by cp.async a tile ahead (16 bytes each where rows are aligned, else 4); bf16 ones, of
+// odd sizes or alignment only, are converted on the way. DM: channels that registers hold.
 constexpr int kSRows = 32, kSKeys = 32, kSThreads = 128;
 
-template <class T>
-__global__ void __launch_bounds__(kSThreads) paged_simt_kernel(const __grid_constant__ Args a) {
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+template <class T, int DM>
+__global__ void __launch_bounds__(kSThreads) paged_simt_kernel(const __grid_constant__ Args a, const int vec) {
     extern __shared__ float sm[];
-    __shared__ long long offs[kSKeys];
+    __shared__ int there[2][kSKeys];
     const PagedAttention& p = a.p;
     const int tid = threadIdx.x, D = p.cache.D, D4 = (D + 3) & ~3, ld = D4 + 4;
     float* Qs = sm;
-    float* Ks = Qs + kSRows * ld;
-    float* Vs = Ks + kSKeys * ld;
+    float* kv = Qs + kSRows * ld;  // [2][k, v][kSKeys][ld]
     const int tile = a.row_tiles - 1 - static_cast<int>(blockIdx.x % a.row_tiles);
     const int rest = blockIdx.x / a.row_tiles, split = rest % a.splits, s = rest / a.splits, kvh = blockIdx.y;
     cudaTriggerProgrammaticLaunchCompletion();  // the join's blocks may take their places
     const Sequence sq = sequence(p, s, blockIdx.x % (a.row_tiles * a.splits) == 0 && kvh == 0 && tid == 0);
-    const int rr0 = tile * kSRows;
-    if (!sq.ok || rr0 >= sq.n_new * a.G) return;
-    const KeyTiles kt = key_tiles(sq.past, sq.n_new, a.G, rr0, rr0 + kSRows, p.window, p.sinks, kSKeys, 1);
+    const int rr0 = tile * kSRows, n_rows = sq.n_new * a.G;
+    if (!sq.ok || rr0 >= n_rows) return;
+    const KeyTiles kt = key_tiles(sq.past, sq.n_new, a.G, rr0, rr0 + kSRows, p.window, p.sinks, kSKeys, a.align);
     const int t0 = split * a.split_tiles, t1 = min(kt.n, t0 + a.split_tiles);
     if (t0 >= t1) return;
     const bool partial = kt.n > a.split_tiles;
 
-    const T* q = static_cast<const T*>(p.q);
-    for (int i = tid; i < kSRows * D4; i += kSThreads) {
-        const int r = i / D4, d = i - r * D4, rr = rr0 + r;
-        float v = 0.f;
-        if (rr < sq.n_new * a.G && d < D)
-            v = to_f(q[(sq.row0 + rr / a.G) * p.ldq + static_cast<long long>(kvh * a.G + rr % a.G) * D + d]);
-        Qs[r * ld + d] = v;
-    }
-    const int r = tid >> 2, c = tid & 3, rr = rr0 + r;
-    const bool live = rr < sq.n_new * a.G;
-    const int pos = live ? sq.past + rr / a.G : -1;
-    float4 o[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    float m = kNegInf, l = 0.f;
+    const int r = tid >> 2, c = tid & 3, rr = rr0 + r, tok = head_group(a, rr), h = kvh * a.G + rr - tok * a.G;
+    const bool live = rr < n_rows;
+    const long long row = sq.row0 + tok;
+    const int pos = live ? sq.past + tok : -1;
     const T* kc = static_cast<const T*>(p.cache.k) + kvh * p.cache.head_stride;
     const T* vc = static_cast<const T*>(p.cache.v) + kvh * p.cache.head_stride;
-
-    for (int t = t0; t < t1; ++t) {
+    auto load = [&](int t, int buf) {
         int start, end;
         key_range(kt, t, kSKeys, start, end);
-        __syncthreads();  // the previous step's readers are done
-        if (tid < kSKeys) offs[tid] = start + tid < end ? key_offset(p, s, start + tid) : -1;
-        __syncthreads();
-        for (int i = tid; i < kSKeys * D4; i += kSThreads) {
-            const int key = i / D4, d = i - key * D4;
-            const long long off = offs[key];
-            const bool in = off >= 0 && d < D;
-            Ks[key * ld + d] = in ? to_f(kc[off + d]) : 0.f;
-            Vs[key * ld + d] = in ? to_f(vc[off + d]) : 0.f;
+        const long long off = start + r < end ? key_offset(p, s, start + r) : -1;
+        if (c == 0) there[buf][r] = off >= 0;
+        if (off < 0) return;  // (left as it is: nothing of it is used)
+        float* kd = kv + (2 * buf * kSKeys + r) * ld;
+        float* vd = kd + kSKeys * ld;
+        if constexpr (sizeof(T) == 4) {
+            const uint32_t ks = smem_u32(kd), vs = smem_u32(vd);
+            if (vec) {
+                for (int d = 4 * c; d < D; d += 16) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ks + d * 4), "l"(kc + off + d) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(vs + d * 4), "l"(vc + off + d) : "memory");
+                }
+            } else {
+                for (int d = c; d < D; d += 4) {
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(ks + d * 4), "l"(kc + off + d) : "memory");
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(vs + d * 4), "l"(vc + off + d) : "memory");
+                }
+            }
+        } else {
+            for (int d = c; d < D; d += 4) {
+                kd[d] = to_f(kc[off + d]);
+                vd[d] = to_f(vc[off + d]);
+            }
         }
+    };
+    // the channels between D and D4 are zeros throughout
+    if (D4 != D) {
+        for (int i = tid; i < (kSRows + 4 * kSKeys) * 4; i += kSThreads)
+            if (D + (i & 3) < D4) sm[(i >> 2) * ld + D + (i & 3)] = 0.f;
+    }
+    load(t0, 0);
+    cp_async_commit();
+    {
+        const T* q = static_cast<const T*>(p.q) + row * p.ldq + static_cast<long long>(h) * D;
+        for (int d = c; d < D; d += 4) Qs[r * ld + d] = live ? to_f(q[d]) : 0.f;
+    }
+    float4 o[DM / 16];
+#pragma unroll
+    for (int i = 0; i < DM / 16; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    float m = kNegInf, l = 0.f;
+
+    for (int t = t0; t < t1; ++t) {
+        const int buf = (t - t0) & 1;
+        if (t + 1 < t1) load(t + 1, buf ^ 1);
+        cp_async_commit();
+        cp_async_wait<1>();
         __syncthreads();
+        int start, end;
+        key_range(kt, t, kSKeys, start, end);
+        const float* Ks = kv + 2 * buf * kSKeys * ld;
+        const float* Vs = Ks + kSKeys * ld;
         float sc[8] = {};
         const float4* qv = reinterpret_cast<const float4*>(Qs + r * ld);
+#pragma unroll 2
         for (int d = 0; d < D4 / 4; ++d) {
             const float4 x = qv[d];
 #pragma unroll
@@ -94,7 +130,7 @@ __global__ void __launch_bounds__(kSThreads) paged_simt_kernel(const __grid_cons
             const int key = c + 4 * i;
             float v = sc[i] * p.scale;
             if (p.softcap > 0.f) v = p.softcap * tanhf(v / p.softcap);
-            sc[i] = offs[key] >= 0 && seen(start + key, pos, p.window, p.sinks) ? v : kNegInf;
+            sc[i] = there[buf][key] && seen(start + key, pos, p.window, p.sinks) ? v : kNegInf;
             mx = fmaxf(mx, sc[i]);
         }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -109,11 +145,12 @@ __global__ void __launch_bounds__(kSThreads) paged_simt_kernel(const __grid_cons
             l += sc[i];
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+        for (int i = 0; i < DM / 16; ++i) {
             o[i].x *= alpha, o[i].y *= alpha, o[i].z *= alpha, o[i].w *= alpha;
         }
         // a key that a row does not see has p = 0, and 0 * v is left out where v may not be finite for it
-        const bool whole = all_seen(kt, start, end, p.window, p.sinks);
+        const bool whole = end - start == kSKeys && all_seen(kt, start, end, p.window, p.sinks) &&
+                           __all_sync(0xffffffffu, there[buf][tid & 31]);
         const int quad = tid & 28;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -123,7 +160,7 @@ __global__ void __launch_bounds__(kSThreads) paged_simt_kernel(const __grid_cons
                 if (!whole && pr == 0.f) continue;
                 const float* v = Vs + (cc + 4 * i) * ld + 4 * c;
 #pragma unroll
-                for (int d = 0; d < 16; ++d) {
+                for (int d = 0; d < DM / 16; ++d) {
                     if (4 * c + 16 * d < D4) {
                         const float4 y = *reinterpret_cast<const float4*>(v + 16 * d);
                         o[d].x = fmaf(pr, y.x, o[d].x);
@@ -134,18 +171,17 @@ __global__ void __launch_bounds__(kSThreads) paged_simt_kernel(const __grid_cons
                 }
             }
         }
+        __syncthreads();  // before this tile's place is filled again
     }
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     if (!live) return;
-    const long long row = sq.row0 + rr / a.G;
-    const int h = kvh * a.G + rr % a.G;
     const float inv = partial ? 1.f : (l > 0.f || l != l ? 1.f / l : 0.f);
     const long long at = (static_cast<long long>(split) * p.batch.rows + row) * p.q_heads + h;
-    if (partial && c == 0) a.ml[at] = make_float2(m * kLog2e, l);  // base-2 exponents, as the other kernel's
+    if (partial && c == 0) a.ml[at] = make_float2(m * kLog2e, l);  // base-2 exponents, as the other kernels'
     T* out = static_cast<T*>(p.out) + row * p.ldo + static_cast<long long>(h) * D;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < DM / 16; ++i) {
         const float v[4] = {o[i].x, o[i].y, o[i].z, o[i].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -160,11 +196,6 @@ __global__ void __launch_bounds__(kSThreads) paged_simt_kernel(const __grid_cons
 // --- tensor cores, mma.sync -------------------------------------------------------------------
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -733,9 +764,9 @@ Args plan(const PagedAttention& p, Kind kind, int num_sms) {
     // One sequence: one wave of equal blocks. Several: their lengths differ and only the longest is
     // known here, so the blocks are cut to a sixteenth of a wave's share and even out (64 sequences
     // of 100 to 16000 tokens: 4, 8, 16 and 32 waves 314, 299, 305 and 340 us). A split of fewer than
-    // eight tiles gains less than the join and its workspace cost a caller.
-    const long long want = static_cast<long long>(num_sms) * resident * (p.batch.S == 1 || kind == kTc ? 1 : 16);
-    const long long splits = std::max<long long>(1, std::min<long long>(want / std::max<long long>(base, 1), tiles / 8));
+    // eight tiles (CUDA cores: two) gains less than the join and its workspace cost a caller.
+    const long long want = static_cast<long long>(num_sms) * resident * (p.batch.S == 1 || kind == kTc ? 1 : kind == kSimt ? 4 : 16);
+    const long long splits = std::max<long long>(1, std::min<long long>(want / std::max<long long>(base, 1), tiles / (kind == kSimt ? 2 : 8)));
     a.split_tiles = std::max(1, ceil_div(tiles, splits));
     a.splits = ceil_div(tiles, a.split_tiles);
     return a;
@@ -782,13 +813,23 @@ void launch_mma_rows(const Args& a, dim3 grid, cudaStream_t st) {
     else launch_mma<DP, 4>(a, grid, st);
 }
 
-template <class T>
+template <class T, int DM>
 void launch_simt(const Args& a, dim3 grid, cudaStream_t st) {
     static PerDeviceOnce once;
-    constexpr int most = (kSRows + 2 * kSKeys) * (256 + 4) * 4;
-    raise_smem(reinterpret_cast<const void*>(&paged_simt_kernel<T>), most, once);
-    const int ld = ((a.p.cache.D + 3) & ~3) + 4;
-    paged_simt_kernel<T><<<grid, kSThreads, (kSRows + 2 * kSKeys) * ld * 4, st>>>(a);
+    constexpr int most = (kSRows + 4 * kSKeys) * (DM + 4) * 4;
+    static_assert(most <= 232448, "shared memory of one block");
+    raise_smem(reinterpret_cast<const void*>(&paged_simt_kernel<T, DM>), most, once);
+    const PagedCache& c = a.p.cache;
+    const int ld = ((c.D + 3) & ~3) + 4;
+    const bool vec = c.D % 4 == 0 && c.page_stride % 4 == 0 && c.token_stride % 4 == 0 && c.head_stride % 4 == 0 &&
+                     (reinterpret_cast<uintptr_t>(c.k) & 15) == 0 && (reinterpret_cast<uintptr_t>(c.v) & 15) == 0;
+    paged_simt_kernel<T, DM><<<grid, kSThreads, (kSRows + 4 * kSKeys) * ld * 4, st>>>(a, vec ? 1 : 0);
+}
+template <class T>
+void launch_simt(const Args& a, dim3 grid, cudaStream_t st) {
+    if (a.p.cache.D <= 64) launch_simt<T, 64>(a, grid, st);
+    else if (a.p.cache.D <= 128) launch_simt<T, 128>(a, grid, st);
+    else launch_simt<T, 256>(a, grid, st);
 }
 
 }  // namespace
