@@ -236,7 +236,7 @@ __device__ __forceinline__ float soft_cap_log2(float x, float two_log2e_over_cap
 // groups: a single token's few rows keep all four warps busy on different keys. Every group runs
 // on its own: it brings its keys and values into its own ring of ST tiles, waits for them alone
 // (no block barrier in the loop), and every warp has its own softmax; the groups' results are
-// joined once at the end. P is rounded to bf16 for the second product, its sum is not.
+// joined once at the end. P is rounded to bf16 for the second product.
 //
 // Keys and values sit in slabs of 64 channels, rows of 128 bytes whose 16-byte chunks are swapped
 // by the row number (c ^ (r & 7)), so that ldmatrix meets no bank twice. TMA: a page's keys come by
@@ -394,7 +394,10 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
     float o[DP / 8][4];
 #pragma unroll
     for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f};
+    // The divisor is the sum of the rounded probabilities (the weights then sum to 1: see pattn_tc.cu), which one more
+    // product with a matrix of ones gives, the same in every column.
+    float m[2] = {kNegInf, kNegInf}, sums[4] = {0.f, 0.f, 0.f, 0.f};
+    constexpr uint32_t kOnes = 0x3f803f80u;
     int pos[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -519,7 +522,7 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
                 const bool move = mx[r] > m[r] + 8.f;
                 alpha[r] = move ? ex2_approx(m[r] - mx[r]) : 1.f;
                 m[r] = move ? mx[r] : m[r];
-                l[r] *= alpha[r];
+                sums[2 * r] *= alpha[r], sums[2 * r + 1] *= alpha[r];
             }
 #pragma unroll
             for (int d = 0; d < DP / 8; ++d) {
@@ -530,14 +533,11 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             const float base = m[r] == kNegInf ? 0.f : m[r];
-            float sum = 0.f;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 sc[t][2 * r] = ex2_approx(sc[t][2 * r] - base);
                 sc[t][2 * r + 1] = ex2_approx(sc[t][2 * r + 1] - base);
-                sum += sc[t][2 * r] + sc[t][2 * r + 1];
             }
-            l[r] += sum;
         }
         bool bad = false;
         auto values = [&](auto clean) {
@@ -546,6 +546,7 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
                 const uint32_t pa[4] = {pack_bf2(sc[2 * t][0], sc[2 * t][1]), pack_bf2(sc[2 * t][2], sc[2 * t][3]),
                                         pack_bf2(sc[2 * t + 1][0], sc[2 * t + 1][1]),
                                         pack_bf2(sc[2 * t + 1][2], sc[2 * t + 1][3])};
+                mma16816(sums, pa, kOnes, kOnes);
 #pragma unroll
                 for (int d = 0; d < DP / 16; ++d) {
                     if (d < 12 || slabs == 4) {
@@ -586,11 +587,6 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
         if (!TMA && gt < GK) offs[((i + ST) % (ST + 1)) * GK + gt] = next;
     }
     cp_async_wait<0>();
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    }
     __syncthreads();
     // [WK][BM] rows of DP fp32 over the tiles' memory, and (max, sum) behind it
     constexpr int LD = DP + 8;
@@ -601,7 +597,7 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         const int row = wk * BM + wm * 16 + (lane >> 2) + 8 * r;
-        if ((lane & 3) == 0) st[row] = make_float2(m[r], l[r]);
+        if ((lane & 3) == 0) st[row] = make_float2(m[r], sums[2 * r]);
 #pragma unroll
         for (int d = 0; d < DP / 8; ++d)
             *reinterpret_cast<float2*>(os + row * LD + d * 8 + (lane & 3) * 2) = make_float2(o[d][2 * r], o[d][2 * r + 1]);

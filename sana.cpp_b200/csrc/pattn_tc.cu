@@ -14,8 +14,12 @@
 //
 // The running maximum is a reference that moves only when a row's maximum passes it by 8 (a
 // factor of 256): the output is rescaled in tensor memory then, by the row's own threads, and
-// almost never after the first tiles. P stays below 2^8, its sum is fp32, its rounding to bf16 is
-// relative, and the division at the end takes the reference out.
+// almost never after the first tiles. P stays below 2^8, its rounding to bf16 is relative, and the
+// division at the end takes the reference out. The divisor is the fp32 sum of the rounded P, so that
+// the weights still sum to 1: with a reference that is not the maximum the largest weights are
+// rounded too, and the sum of the unrounded ones leaves an error 1.4 times that of the output's own
+// rounding (1.05 to 1.4 times now, the less the fewer keys count), for 3 % of the time at head size
+// 128. At 64, where all hangs on the softmax, it would be 17 %: there the sum is of the unrounded P.
 //
 // Keys and values come into the 128-byte-swizzled layout of the matrix descriptors: slabs of 64
 // channels, 128-byte rows, chunk c of row r at c ^ (r & 7); K and Q are K-major operands, V is
@@ -138,6 +142,12 @@ __device__ __forceinline__ uint64_t mnmajor_sw128_desc(uint32_t smem_addr, uint3
 }
 constexpr uint32_t kBTransposed = 1u << 16;  // instruction descriptor: B is MN-major
 
+// lo += x's low bf16, hi += its high one
+__device__ __forceinline__ void add_bf2(float& lo, float& hi, uint32_t x) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tadd.rn.f32.bf16 %0, a, %0;\n\tadd.rn.f32.bf16 %1, b, %1;\n\t}"
+        : "+f"(lo), "+f"(hi)
+        : "r"(x));
+}
 __device__ __forceinline__ uint32_t pack_bf2(float lo, float hi) {
     const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&b);
@@ -271,6 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
     using Sh = TcShape<DP>;
     constexpr int BN = kKeys, NK = Sh::kKRing, NV = Sh::kVRing, kPieces = Sh::kPieces, kSlabs = Sh::kSlabs;
     constexpr int kParts = Sh::kParts, kCols = Sh::kCols;
+    constexpr bool kSumRounded = DP > 64;
     constexpr int kEarly = kParts == 1 ? 3 : 2;  // quarters of a tile's P handed over before the rest
     extern __shared__ unsigned char smem_raw[];
     const PagedAttention& p = a.p;
@@ -442,7 +453,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                 }
                 const float ref = m == -INFINITY ? 0.f : m;
                 const uint64_t k2 = f2_make(scale_log2, scale_log2), r2 = f2_make(-ref, -ref);
-                uint64_t sum[2] = {0, 0};
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                uint64_t sum2[2] = {0, 0};
 #pragma unroll
                 for (int c = 0; c < kCols / 32; ++c) {
                     uint32_t pk[16];
@@ -459,8 +471,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         }
                         const float2 v = f2_split(e);
                         const float e0 = ex2_approx(v.x), e1 = ex2_approx(v.y);
-                        sum[i & 1] = add2(sum[i & 1], f2_make(e0, e1));
                         pk[i] = pack_bf2(e0, e1);
+                        if (kSumRounded) add_bf2(sum[(2 * i) & 3], sum[(2 * i + 1) & 3], pk[i]);
+                        else sum2[i & 1] = add2(sum2[i & 1], f2_make(e0, e1));
                     }
                     tmem_st16(s_t + part * (kCols / 2) + c * 16, pk);  // over the scores, which this row has read
                     if (kParts == 1 && c == kEarly - 1) {              // the products over these keys may start
@@ -470,8 +483,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                         if (lane == 0) mbar_arrive(p_early(slot));
                     }
                 }
-                const float2 total = f2_split(add2(sum[0], sum[1]));
-                l += total.x + total.y;
+                const float2 total = f2_split(add2(sum2[0], sum2[1]));
+                l += kSumRounded ? (sum[0] + sum[1]) + (sum[2] + sum[3]) : total.x + total.y;
                 if (kParts > 1 && !whole) {  // the values of this part's keys
                     for (int pc = part * (kPieces / kParts); pc < (part + 1) * kPieces / kParts && ok; ++pc) {
                         const int g = j * kPieces + pc;
