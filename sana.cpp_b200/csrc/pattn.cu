@@ -713,11 +713,13 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
 // --- plan and launch ----------------------------------------------------------------------------
 enum Kind { kSimt, kMma, kTc };
 
-// The tcgen05 kernel's 128-row tiles take over from the mma.sync kernel's 64-row ones above this
-// many packed rows of the longest chunk.
-constexpr long long kTcRows = 64;
+// The tcgen05 kernel's 128-row tiles take over from the mma.sync kernel above so many packed rows of the longest chunk.
+// Measured on 1, 16 and 64 sequences behind 8000, 2000 and 300 tokens, us with mma.sync / with tcgen05: head size 64, 48 and
+// 128 rows, 29.5 / 30.9 and 57.7 / 43.5 (16 sequences); 128, 32 and 48 rows, 28.7 / 33.0 and 57.4 / 35.1; 256, 8 and 18 rows,
+// 41.2 / 40.6 and 53.5 / 37.9.
 bool wants_tc(const PagedAttention& p) {
-    return static_cast<long long>(p.batch.max_new) * (p.q_heads / p.cache.kv_heads) > kTcRows;
+    const int rows = p.cache.D <= 64 ? 64 : p.cache.D <= 128 ? 32 : 16;
+    return static_cast<long long>(p.batch.max_new) * (p.q_heads / p.cache.kv_heads) > rows;
 }
 
 bool cache_fits_mma(const PagedCache& c) {
@@ -757,12 +759,16 @@ Args plan(const PagedAttention& p, Kind kind, int num_sms) {
     // a window's sinks and its start, rounded down to `align`, may each take part of one tile more
     const int tiles = ceil_div(span, a.BN) + (p.window > 0 ? (a.align > 1 ? 2 : 1) : 0);
     const long long base = static_cast<long long>(p.batch.S) * p.cache.kv_heads * a.row_tiles;
-    // One sequence: one wave of equal blocks. Several: their lengths differ and only the longest is
-    // known here, so the blocks are cut to a sixteenth of a wave's share and even out (64 sequences
-    // of 100 to 16000 tokens: 4, 8, 16 and 32 waves 314, 299, 305 and 340 us). A split of fewer than
-    // eight tiles (CUDA cores: two) gains less than the join and its workspace cost a caller.
-    const long long want = static_cast<long long>(num_sms) * resident * (p.batch.S == 1 || kind == kTc ? 1 : kind == kSimt ? 4 : 16);
-    const long long splits = std::max<long long>(1, std::min<long long>(want / std::max<long long>(base, 1), tiles / (kind == kSimt ? 2 : 8)));
+    // Splits fill one wave, in shares of three tiles or more (one sequence of 2000 tokens, 8 heads of 128 over 4: 12.4 us;
+    // shares of eight tiles 16.5; of two no less, while a short cache then pays for the join). Beyond one wave, sequences
+    // of different lengths, of which only the longest is known here, even out in blocks of a sixteenth of a wave's share (64
+    // sequences of 100 to 16000 tokens: 4, 8, 16 and 32 waves 314, 299, 305 and 340 us), but in shares of eight tiles: 64
+    // sequences of 1500 tokens took 48 us so, and 56 in shares of three. The CUDA-core kernel's tiles take longer.
+    const long long slots = static_cast<long long>(num_sms) * resident, per = std::max<long long>(base, 1);
+    long long splits = slots / per;
+    if (kind == kMma && p.batch.S > 1) splits = std::max<long long>(splits, std::min<long long>(16 * slots / per, tiles / 8));
+    if (kind == kSimt && p.batch.S > 1) splits = 4 * slots / per;
+    splits = std::max<long long>(1, std::min<long long>(splits, tiles / (kind == kSimt ? 2 : 3)));
     a.split_tiles = std::max(1, ceil_div(tiles, splits));
     a.splits = ceil_div(tiles, a.split_tiles);
     return a;
