@@ -554,9 +554,9 @@ typedef struct sana_paged_cache {
  * [sequences + 1] ascending, kv_len [sequences], page_table [sequences, table_width]: int32,
  * device; entries behind a sequence's last page are not read, and neither are entries that no
  * new token sees. max_new and max_kv are upper bounds of the new and of the cached tokens of
- * any sequence (they size the launch; a larger kv_len is taken as max_kv's violation and
- * recorded). Rows behind the last sequence are left as they were. A sequence may have no new
- * token. */
+ * any sequence (they size the launch; a sequence beyond them is recorded and left out). Rows in
+ * front of the first sequence and behind the last are left as they were. A sequence may have no
+ * new token. */
 typedef struct sana_paged_batch {
     int sequences, rows, max_new, max_kv;
     const int *row_start;
@@ -583,9 +583,10 @@ int sana_op_rotary_append_device(sana_cuda_ctx *ctx, const sana_rotary *rotary, 
  * q); scores, softmax statistics and sums are fp32. What a token does not see does not reach
  * its output, be it NaN or infinite; a token that sees nothing gets zeros. head_dim <= 256.
  * BF16 with head_dim a multiple of 8 and 16-byte aligned pointers and strides runs on the
- * tensor cores, the rest on the CUDA cores. workspace: device, 16-byte aligned,
+ * tensor cores (pages whose size divides 128, or is a multiple of it, and is at least 8, are the
+ * fast ones there), the rest on the CUDA cores. workspace: device, 16-byte aligned,
  * sana_op_paged_attention_workspace() bytes of the same batch, cache, heads, window and sinks
- * (0 bytes: may be NULL); its contents need no preparation and nothing is kept in it, but two
+ * (0 bytes, which invalid arguments give too: may be NULL); its contents need no preparation and nothing is kept in it, but two
  * calls that may overlap (two streams, two graphs in flight) need one each. */
 int sana_op_paged_attention_device(sana_cuda_ctx *ctx, const sana_paged_batch *batch, const sana_paged_cache *cache,
                                    const void *q, long long ldq, int q_heads, float scale, int window, int sinks,

@@ -188,7 +188,7 @@ void launch(const AddRmsNorm& p, int num_sms, cudaStream_t st) {
     a.weight = p.weight;
     a.scale = p.scale;
     a.C = p.C;
-    a.group = p.group ? p.group : p.C;
+    a.group = p.group && p.group < p.C ? p.group : p.C;
     a.groups = (p.C + a.group - 1) / a.group;
     a.offset = p.offset;
     a.eps = p.eps;
@@ -208,18 +208,23 @@ void launch(const AddRmsNorm& p, int num_sms, cudaStream_t st) {
                      (!RES || (aligned(r, p.ldr, sizeof(TR)) && aligned(sum, p.ldr, sizeof(TR)))) &&
                      (reinterpret_cast<uintptr_t>(p.weight) & 15) == 0;
     const unsigned grid = static_cast<unsigned>(p.rows);
+    auto run = [&](auto* kernel, int block) {
+        if (smem > 40960)  // beyond what a launch gets unasked: single channels as groups of wide rows
+            SANA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+        kernel<<<grid, block, smem, st>>>(x, r, sum, out, a);
+    };
     auto threads = [&](int units, int per) { return (((units + per - 1) / per + 31) / 32) * 32; };
     if (vec) {
         const int units = p.C / 8;
         if (units <= 1024) {
-            add_rms_norm_kernel<TX, TR, TO, 8, 1, RES><<<grid, threads(units, 1), smem, st>>>(x, r, sum, out, a);
+            run(&add_rms_norm_kernel<TX, TR, TO, 8, 1, RES>, threads(units, 1));
         } else {
-            add_rms_norm_kernel<TX, TR, TO, 8, 2, RES><<<grid, threads(units, 2), smem, st>>>(x, r, sum, out, a);
+            run(&add_rms_norm_kernel<TX, TR, TO, 8, 2, RES>, threads(units, 2));
         }
     } else if (p.C <= 4096) {
-        add_rms_norm_kernel<TX, TR, TO, 1, 4, RES><<<grid, threads(p.C, 4), smem, st>>>(x, r, sum, out, a);
+        run(&add_rms_norm_kernel<TX, TR, TO, 1, 4, RES>, threads(p.C, 4));
     } else {
-        add_rms_norm_kernel<TX, TR, TO, 1, 16, RES><<<grid, threads(p.C, 16), smem, st>>>(x, r, sum, out, a);
+        run(&add_rms_norm_kernel<TX, TR, TO, 1, 16, RES>, threads(p.C, 16));
     }
     SANA_CUDA(cudaGetLastError());
 }

@@ -1875,6 +1875,7 @@ int sana_op_paged_attention_device(sana_cuda_ctx* ctx, const sana_paged_batch* b
         check_rows("out", out, p.batch.rows, ldo, width);
         SANA_REQUIRE(std::isfinite(scale), "scale must be finite");
         SANA_REQUIRE(softcap >= 0.f && std::isfinite(softcap), "softcap must be finite and not negative");
+        SANA_REQUIRE(softcap == 0.f || std::abs(scale) <= 1e30f * softcap, "softcap is too small for the scale");
         sana::Engine& eng = engine(ctx);
         const size_t need = sana::paged_attention_workspace(p, eng.num_sms());
         SANA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),

@@ -57,7 +57,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) rotary_kernel(const __
         const int s = sequence_of(p.batch.row_start, S, row);
         if (s >= S) return;  // behind the last sequence
         const int end = p.batch.row_start[s + 1], len = p.batch.kv_len[s];
-        if (p.batch.row_start[s] > row || end > p.rows) {
+        const bool before = p.batch.row_start[s] > row;
+        if (before && s == 0) return;  // in front of the first sequence
+        if (before || end > p.rows) {
             if (tid == 0) record_bad(p.bad, kBadRows);
             return;
         }

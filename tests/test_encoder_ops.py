@@ -121,7 +121,7 @@ def test_cache_refusals(handle, change, word):
 @pytest.mark.parametrize("change, word", [
     (dict(q=None), "q must"), (dict(out=None), "out must"), (dict(ldq=511), "row stride"), (dict(ldo=0), "row stride"),
     (dict(heads=7), "multiple"), (dict(heads=0), "multiple"), (dict(window=-1), "window"), (dict(sinks=-1), "window"),
-    (dict(scale=math.inf), "scale"), (dict(cap=-1.0), "softcap"), (dict(cap=math.nan), "softcap")])
+    (dict(scale=math.inf), "scale"), (dict(cap=-1.0), "softcap"), (dict(cap=math.nan), "softcap"), (dict(cap=1e-38), "softcap")])
 def test_attention_refusals(handle, change, word):
     lib, h, _ = handle
     assert attend(lib, h, **change) == INVALID and word in message(lib, h)

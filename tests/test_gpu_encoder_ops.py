@@ -70,7 +70,7 @@ def check_norm(g, x, r, w, offset, out, group, eps=1e-6):
         close(res[0], y, y.abs() * (U[out] + NORM_U) * 1.001 + 1e-37, "out")
         return res
     C = x.shape[1]
-    gs = group or C
+    gs = min(group or C, C)
     n = -(-C // gs)
     z = torch.nn.functional.pad(y, (0, n * gs - C)).view(-1, n, gs)
     scale = (z.abs().amax(-1) / 448.0).clamp(min=2.0 ** -100)
@@ -92,9 +92,10 @@ def test_norm_sizes_and_types(g, rows, C, xt, rt, out):
 
 
 @pytest.mark.parametrize("C, group", [(2304, 128), (2304, 64), (2304, 100), (1000, 128), (72, 8), (77, 10), (8200, 256), (64, 1),
-                                      (24, 4096), (12288, 16)])
+                                      (24, 4096), (12288, 16),
+                                      (16384, 1), (16384, 8), (64, 2 ** 31 - 1)])
 def test_norm_groups(g, C, group):
-    x, r = randn(9, C, seed=C, dtype=BF16), randn(9, C, seed=group, dtype=F32)
+    x, r = randn(9, C, seed=C, dtype=BF16), randn(9, C, seed=group % 1000, dtype=F32)
     x[:, :group] = 0
     r[:, :group] = 0  # a group of zeros has the smallest scale, and zeros
     res = check_norm(g, x, r, None, 0.0, E4M3, group)
@@ -469,6 +470,57 @@ def test_offsets_beyond_32_bits(g):
     check_attention(g, b, randn(1, 4, 64, seed=2, dtype=BF16))
     b.new, b.past, b.max_new, b.row_start = [18], [2], 18, torch.tensor([0, 18], dtype=torch.int32, device="cuda")
     check_attention(g, b, randn(18, 4, 64, seed=2, dtype=BF16))
+
+
+@pytest.mark.parametrize("D", [8, 16, 40, 56, 88, 120, 136, 192, 200, 248])
+@pytest.mark.parametrize("page", [8, 16, 32, 128, 256, 48, 4])
+def test_attention_head_and_page_sizes(g, D, page):
+    """Head sizes that end inside a slab, pages that divide a tile, that tiles divide, and others; few rows and many."""
+    for new, past in (([1, 2], [200, 40]), ([70, 5], [130, 300])):
+        b = Paged(new, past, 2, D, page, BF16, seed=D + page).fill(7)
+        check_attention(g, b, randn(b.rows, 6, D, seed=1, dtype=BF16), window=150 if page != 16 else 0, sinks=3)
+
+
+def test_rows_in_front_and_behind(g):
+    """Rows before the first sequence, as behind the last, are nobody's."""
+    b = Paged([3, 40], [20, 9], 1, 64, 16, BF16, seed=3, trailing=2).fill(5)
+    starts = b.row_start + 4
+    q = randn(b.rows + 4, 2, 64, seed=1, dtype=BF16)
+    out, plain = torch.full_like(q, 3.0), check_attention(g, b, q[4:])
+    g.paged_attention_device(q, b.k, b.v, starts, b.kv_len, b.table, b.max_new, b.max_kv, out=out)
+    g.synchronize()
+    assert torch.equal(out[4:47], plain[:43]) and (out[:4] == 3.0).all() and (out[47:] == 3.0).all()
+    k, v = randn(b.rows + 4, 1, 64, seed=2, dtype=BF16), randn(b.rows + 4, 1, 64, seed=3, dtype=BF16)
+    freq = torch.ones(32, dtype=torch.float64, device="cuda")
+    keep = q.clone()
+    got = g.rotary_append_device(q, k, v, freq, b.k, b.v, starts, b.kv_len, b.table, b.max_new, inplace=True)
+    g.synchronize()
+    assert torch.equal(got[:4], keep[:4]) and torch.equal(got[47:], keep[47:]) and not torch.equal(got[4:47], keep[4:47])
+    assert torch.equal(b.v[b.places(1, 9, 49)], v[7:47])
+
+
+def test_two_handles_at_once(g):
+    """Two handles on two streams, each with a workspace of its own: the results of one at a time."""
+    from sana_b200 import SanaCuda
+    other = SanaCuda(0)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    bs = [Paged([1, 1, 1, 1], [3000, 64, 900, 10 + i], 2, 128, 16, BF16, seed=i).fill(5 + i) for i in range(2)]
+    bs += [Paged([300], [700 + i], 2, 128, 16, BF16, seed=i).fill(9 + i) for i in range(2)]
+    qs = [randn(b.rows, 8, 128, seed=i, dtype=BF16) for i, b in enumerate(bs)]
+    want = [check_attention(g, b, q).clone() for b, q in zip(bs, qs)]
+    torch.cuda.synchronize()
+    got = [[], [], [], []]
+    for _ in range(10):
+        for h, st, pick in ((g, streams[0], (0, 2)), (other, streams[1], (1, 3))):
+            with torch.cuda.stream(st):
+                h.set_stream(st.cuda_stream)
+                for i in pick:
+                    got[i].append(h.paged_attention_device(qs[i], bs[i].k, bs[i].v, *bs[i].args(), bs[i].max_kv))
+    torch.cuda.synchronize()
+    g.set_stream(1)
+    for w, all_ in zip(want, got):
+        assert all(torch.equal(x, w) for x in all_)
+    other.close()
 
 
 def test_shared_prefix_pages(g):
