@@ -504,8 +504,8 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
                     if (!there(key) || !seen(start + key, pos[e >> 1], p.window, p.sinks)) sc[t][e] = kNegInf;
                 }
         }
-        // The maximum that the exponents are taken against moves only when a score passes it by 8 (a factor of 256):
-        // every lane looks at its own scores, and the rows' maxima are shared out among lanes when one has to.
+        // The rows' maxima are shared out among lanes only where a lane has a score above its row's, which is seldom after
+        // the first tiles (the largest probability is then exactly 1, and its rounding exact).
         float mx[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -513,13 +513,13 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
 #pragma unroll
             for (int t = 1; t < NT; ++t) mx[r] = fmaxf(mx[r], fmaxf(sc[t][2 * r], sc[t][2 * r + 1]));
         }
-        if (__any_sync(0xffffffffu, mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f)) {  // (-inf + 8 is passed by any score)
+        if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
             float alpha[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
                 mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-                const bool move = mx[r] > m[r] + 8.f;
+                const bool move = mx[r] > m[r];
                 alpha[r] = move ? ex2_approx(m[r] - mx[r]) : 1.f;
                 m[r] = move ? mx[r] : m[r];
                 sums[2 * r] *= alpha[r], sums[2 * r + 1] *= alpha[r];
