@@ -143,8 +143,9 @@ __device__ __forceinline__ float gelu_tanh(float x) {
 // unwinds. Waiters also give up early once any thread has recorded an error.
 //
 // A handle's device error word is 16 bytes: int [0] is the error code (0 = none), int [1] what
-// kernels found wrong in device data (it ends no wait), and the 64-bit value at byte 8 is the handle's wait limit in nanoseconds (sana_cuda_set_wait_limit;
-// kWaitLimitNs by default). Waiters read the limit once they have spun a while.
+// kernels found wrong in device data (it ends no wait), and the 64-bit value at byte 8 is the
+// handle's wait limit in nanoseconds (sana_cuda_set_wait_limit; kWaitLimitNs by default). Waiters
+// read the limit once they have spun a while.
 // ---------------------------------------------------------------------------------------
 constexpr uint64_t kWaitLimitNs = 2000000000ull;  // 2 s
 constexpr int kErrWordBytes = 16;

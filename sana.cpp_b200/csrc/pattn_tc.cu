@@ -26,8 +26,8 @@
 // MN-major (its channels contiguous). K and V have a ring each, filled by warps of their own, of
 // whole tiles, or for head sizes above 128, where a tile has 64 KB, of quarters (64 channels of K,
 // 32 keys of V). Where pages divide a tile or tiles divide a page, tensor copies (TMA) bring them:
-// K one per page and slab; V one per 16 keys, all slabs, where the head size is a multiple of 64. V's
-// keys stand in blocks of a product's 16, [block][slab][key], which makes a copy of all slabs one box.
+// one per page and slab. Above 128, V's keys stand in blocks of a product's 16 (8 where pages are of
+// 8), [block][slab][key], which makes a copy of all slabs one box where the head size is a multiple of 64.
 // Other page sizes end anywhere inside a tile and come by 16-byte cp.async.
 #include <type_traits>
 
