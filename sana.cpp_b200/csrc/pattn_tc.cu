@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(s_full(i), 1);
-            mbar_init(p_early(i), 4);
+            mbar_init(p_early(i), 4 * kParts);  // also the rescaling of the rows' other threads
             mbar_init(p_full(i), 4);
             mbar_init(pv_done(i), 1);
         }
@@ -450,6 +450,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const __grid_cons
                             tmem_st16(o_t + c, r);
                         }
                     }
+                }
+                if (kParts > 1 && part == 1) {
+                    // The products that start on p_early add to every channel of O: this part's channels are rescaled
+                    // by then too (its probabilities follow with p_full).
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_early(slot));
                 }
                 const float ref = m == -INFINITY ? 0.f : m;
                 const uint64_t k2 = f2_make(scale_log2, scale_log2), r2 = f2_make(-ref, -ref);
