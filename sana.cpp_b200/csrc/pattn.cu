@@ -289,7 +289,11 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
     long long* offs = reinterpret_cast<long long*>(smem + kOffs) + wk * (ST + 1) * GK;  // [ST + 1][GK], cp.async
     const uint32_t full = q_s + kOffs + 512 + wk * (ST * 8);                            // [ST] barriers, TMA
     auto group_all = [&](bool ok) -> bool {  // barrier of the group, with the conjunction of what its threads bring
-        if (WM == 1) return __all_sync(0xffffffffu, ok);
+        if (WM == 1) {
+            const bool all_ok = __all_sync(0xffffffffu, ok);
+            __syncwarp();  // a vote alone does not order the lanes' shared memory
+            return all_ok;
+        }
         int all;
         asm volatile(
             "{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.and.pred q, %2, %3, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"

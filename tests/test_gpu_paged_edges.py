@@ -49,3 +49,19 @@ def test_a_maximum_that_rises_from_tile_to_tile(g, D, page, new, past, window):
         close(got, want, tol + want.abs() * 2 * U[BF16], (D, window))
         assert first is None or torch.equal(got, first)
         first = got
+
+
+# --- few rows -------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("D, G", [(64, 4), (128, 8), (256, 2), (136, 1)])
+@pytest.mark.parametrize("page", [1, 5, 24, 16])
+def test_single_tokens_over_any_pages_repeat_themselves(g, D, G, page):
+    """One warp to a group of keys: what its lanes copy and look up for one another is there before it is read. The same
+    bits each time, beside other work, and the 64-bit result."""
+    b = Paged([1, 2, 1, 1], [3000, 130, 15, 700], 2, D, page, BF16, seed=D + page).fill(3)
+    q = randn(b.rows, 2 * G, D, seed=4, dtype=BF16, scale=2.0)
+    want, tol = attention_want(b, q, D ** -0.5, 0, 0, 0.0)
+    got = [g.paged_attention_device(q, b.k, b.v, *b.args(), b.max_kv) for _ in range(20)]
+    g.synchronize()
+    close(got[0], want, tol + want.abs() * 2 * U[BF16])
+    assert all(torch.equal(x, got[0]) for x in got[1:])
