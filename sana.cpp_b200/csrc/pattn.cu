@@ -227,13 +227,18 @@ __device__ __forceinline__ uint32_t finite2(uint32_t x, bool& bad) {
     if ((x & 0x7f800000u) == 0x7f800000u) x &= 0x0000ffffu, bad = true;
     return x;
 }
-// cap * tanh(x / cap) * log2(e) from the hardware exponential: tanh z = 1 - 2 / (1 + e^2z), absolute
-// error a few 2^-24 for any z, which times the cap stays far below a bf16 probability's rounding.
-__device__ __forceinline__ float soft_cap_log2(float x, float two_log2e_over_cap, float cap_log2e) {
-    return fmaf(-2.f * cap_log2e, rcp_approx(1.f + ex2_approx(x * two_log2e_over_cap)), cap_log2e);
+// cap tanh(z) log2(e) of a product x, z = x scale / cap, for caps beyond kCheapCap (pattn.cuh has the cheap form, which
+// cancels where |z| is small): below |z| = 1/4 the score itself times the Taylor series of tanh(z) / z up to z^8 (what
+// follows is below 2^-26), from there on the cheap form, whose error is then 2^-19 of the score.
+__device__ __forceinline__ float wide_cap_log2(float x, float to_z, float scale_log2, float cap_log2) {
+    constexpr float kTwoLog2e = 2.885390081777927f;
+    const float z = x * to_z, z2 = z * z;
+    const float series = fmaf(z2, fmaf(z2, fmaf(z2, fmaf(z2, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+    return fabsf(z) < 0.25f ? x * scale_log2 * series : soft_cap_log2(z, kTwoLog2e, cap_log2);
 }
 
-// DP: padded head size. Groups of WM warps (16 rows each) share out each step's 64 keys, 4 / WM
+// DP: padded head size. WIDE: soft caps beyond kCheapCap, a kernel of its own (as a branch, or for every cap, it cost single
+// tokens at head size 256 3 %: 428 us for 64 behind 100 to 16000 tokens, 414 without). Groups of WM warps (16 rows each) share out each step's 64 keys, 4 / WM
 // groups: a single token's few rows keep all four warps busy on different keys. Every group runs
 // on its own: it brings its keys and values into its own ring of ST tiles, waits for them alone
 // (no block barrier in the loop), and every warp has its own softmax; the groups' results are
@@ -258,7 +263,7 @@ struct MmaShape {
     }
 };
 
-template <int DP, int WM, bool TMA>
+template <int DP, int WM, bool TMA, bool WIDE>
 __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ Args a,
                                                         const __grid_constant__ CUtensorMap k_map,
                                                         const __grid_constant__ CUtensorMap v_map, const int box) {
@@ -410,7 +415,7 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
         pos[i] = rr < n_rows ? sq.past + head_group(a, rr) : -1;
     }
     const float scale_log2 = p.scale * kLog2e;
-    const float cap_in = p.softcap > 0.f ? 2.f * scale_log2 / p.softcap : 0.f, cap_out = p.softcap * kLog2e;
+    const float cap_in = p.softcap > 0.f ? (WIDE ? p.scale : 2.f * scale_log2) / p.softcap : 0.f, cap_out = p.softcap * kLog2e;
 
     // A lane's part of the ldmatrix addresses: its row, and its chunk of the first 16 channels of a slab, swapped by the
     // row; the other channels' chunks differ in bits 5 and 6 (^ 32 per 16 channels).
@@ -493,7 +498,8 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sc[t][e] = soft_cap_log2(sc[t][e], cap_in, cap_out);
+                for (int e = 0; e < 4; ++e)
+                    sc[t][e] = WIDE ? wide_cap_log2(sc[t][e], cap_in, scale_log2, cap_out) : soft_cap_log2(sc[t][e], cap_in, cap_out);
         } else {
 #pragma unroll
             for (int t = 0; t < NT; ++t)
@@ -792,25 +798,26 @@ void raise_smem(const void* f, int bytes, PerDeviceOnce& once) {
     once.mark();
 }
 
-template <int DP, int WM, bool TMA>
+template <int DP, int WM, bool TMA, bool WIDE>
 void launch_mma(const Args& a, int box, dim3 grid, cudaStream_t st) {
     static PerDeviceOnce once;
     constexpr int bytes = MmaShape<DP>::smem(16 * WM, TMA);
     static_assert(bytes <= 232448, "shared memory of one block");
-    raise_smem(reinterpret_cast<const void*>(&paged_mma_kernel<DP, WM, TMA>), bytes, once);
+    raise_smem(reinterpret_cast<const void*>(&paged_mma_kernel<DP, WM, TMA, WIDE>), bytes, once);
     CUtensorMap k{}, v{};
     if (TMA) {
         k = pool_map(a.p.cache, a.p.cache.k, box);
         v = pool_map(a.p.cache, a.p.cache.v, box);
     }
-    paged_mma_kernel<DP, WM, TMA><<<grid, 128, bytes, st>>>(a, k, v, box);
+    paged_mma_kernel<DP, WM, TMA, WIDE><<<grid, 128, bytes, st>>>(a, k, v, box);
 }
 
 template <int DP, int WM>
 void launch_mma(const Args& a, dim3 grid, cudaStream_t st) {
     const int box = copy_box(a.p.cache, 16 * WM);  // within a group's keys
-    if (box > 0) launch_mma<DP, WM, true>(a, box, grid, st);
-    else launch_mma<DP, WM, false>(a, 0, grid, st);
+    const bool wide = a.p.softcap > kCheapCap;
+    if (box > 0) wide ? launch_mma<DP, WM, true, true>(a, box, grid, st) : launch_mma<DP, WM, true, false>(a, box, grid, st);
+    else wide ? launch_mma<DP, WM, false, true>(a, 0, grid, st) : launch_mma<DP, WM, false, false>(a, 0, grid, st);
 }
 
 template <int DP>
@@ -903,8 +910,9 @@ void paged_attention(PagedAttention p, int num_sms, cudaStream_t st) {
     if (p.batch.S == 0 || p.batch.rows == 0 || p.batch.max_new == 0) return;
     const bool mma = cache_fits_mma(p.cache) && (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 &&
                      (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.ldq % 8 == 0 && p.ldo % 8 == 0;
-    // the tcgen05 kernel maps a tile's largest score alone, which takes a map that rises: scale > 0
-    const Kind kind = !mma ? kSimt : wants_tc(p) && p.scale > 0.f ? kTc : kMma;
+    // the tcgen05 kernel maps a tile's largest score alone, which takes a map that rises: scale > 0; and it has the cheap
+    // form of the soft cap only (2048 tokens after 8192, head size 128: 646 us there, 1992 with the other form here)
+    const Kind kind = !mma ? kSimt : wants_tc(p) && p.scale > 0.f && p.softcap <= kCheapCap ? kTc : kMma;
     Args a = plan(p, kind, num_sms);
     const size_t n = static_cast<size_t>(a.splits) * p.batch.rows * p.q_heads;
     a.ml = static_cast<float2*>(p.workspace);

@@ -99,6 +99,14 @@ __device__ __forceinline__ bool seen(int j, int pos, int window, int sinks) {
     return j <= pos && (window <= 0 || j > pos - window || j < sinks);
 }
 
+// The soft cap of the tensor-core kernels, cap tanh(x / cap) log2(e) of a product x, in = 2 scale log2(e) / cap: by tanh z =
+// 1 - 2 / (1 + e^2z) from the hardware exponential and reciprocal. Its error, whatever the score, moves a probability by at
+// most cap 2^-21 of itself: up to kCheapCap 2^-11, an eighth of the rounding to bf16. Larger caps take another form.
+constexpr float kCheapCap = 1024.f;
+__device__ __forceinline__ float soft_cap_log2(float x, float in, float cap_log2) {
+    return fmaf(-2.f * cap_log2, rcp_approx(1.f + ex2_approx(x * in)), cap_log2);
+}
+
 PageDivisor page_divisor(int d);
 __device__ __forceinline__ int head_group(const Args& a, int rr) {  // the token of packed row rr: rr / G
     return static_cast<int>((__umulhi(static_cast<uint32_t>(rr), a.g_div.magic) + static_cast<uint32_t>(rr)) >> a.g_div.shift);

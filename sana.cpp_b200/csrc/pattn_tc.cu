@@ -152,10 +152,6 @@ __device__ __forceinline__ uint32_t pack_bf2(float lo, float hi) {
     const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&b);
 }
-// cap tanh(x / cap) log2(e), as in pattn.cu
-__device__ __forceinline__ float soft_cap_log2(float x, float in, float out) {
-    return fmaf(-2.f * out, rcp_approx(1.f + ex2_approx(x * in)), out);
-}
 
 __device__ __forceinline__ uint32_t elect_one() {
     uint32_t on;

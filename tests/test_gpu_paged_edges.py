@@ -65,3 +65,42 @@ def test_single_tokens_over_any_pages_repeat_themselves(g, D, G, page):
     g.synchronize()
     close(got[0], want, tol + want.abs() * 2 * U[BF16])
     assert all(torch.equal(x, got[0]) for x in got[1:])
+
+
+# --- soft caps of any size ------------------------------------------------------------------------
+
+def capped_want(b, q, scale, cap):
+    """attention_want with an error of the cap that does not grow with it. The cheap form, used up to a cap of 1024, is off
+    by at most 3.5 2^-23 of the base-2 exponent's cap (the exponential's, the sum's and the quotient's roundings, twice, and the
+    last one's): 2^-21 of the cap in the score. Any other is off by that at a quarter of the cap or more, 2^-19 of the
+    score, or by a few roundings of the score (attention_want's eight)."""
+    heads, hk, D = q.shape[1], b.k.shape[2], q.shape[2]
+    want, tol = (torch.zeros(q.shape, dtype=torch.float64, device="cuda") for _ in range(2))
+    row = 0
+    for s, (n, p) in enumerate(zip(b.new, b.past)):
+        at = b.places(s, 0, n + p)
+        k, v = (t[at].double().repeat_interleave(heads // hk, 1).transpose(0, 1) for t in (b.k, b.v))
+        qq = q[row:row + n].double().transpose(0, 1)
+        t = cap * torch.tanh(qq @ k.transpose(1, 2) * scale / cap)
+        size = qq.abs() @ k.abs().transpose(1, 2) * scale
+        hidden = torch.arange(n + p, device="cuda") > torch.arange(p, p + n, device="cuda")[:, None]
+        prob = torch.softmax(t.masked_fill(hidden, -math.inf), -1)
+        e = (D / 8 + 16) * 2.0 ** -24 * size + (2.0 ** -21 * cap if cap <= 1024 else 2.0 ** -19 * t.abs()) + 2.0 ** -20
+        e = e.masked_fill(hidden, 0).amax(-1, keepdim=True)
+        p_round = U[BF16] if q.dtype == BF16 else 0.0
+        want[row:row + n] = (prob @ v).transpose(0, 1)
+        tol[row:row + n] = ((prob @ v.abs()) * (2 * e * 1.01 + p_round + (n + p) / 16 * 2.0 ** -24)).transpose(0, 1)
+        row += n
+    return want, tol + want.abs() * (2 if q.dtype == BF16 else 1) * U[q.dtype]
+
+
+@pytest.mark.parametrize("cap", [0.5, 50.0, 1000.0, 1025.0, 1e4, 1e5, 1e6, 1e7, 1e30])
+@pytest.mark.parametrize("dtype, D", [(BF16, 64), (BF16, 128), (BF16, 256), (F32, 64)])
+@pytest.mark.parametrize("new, past", [([1, 1], [40, 600]), ([150, 9], [70, 300])])
+def test_caps_large_against_the_scores(g, cap, dtype, D, new, past):
+    b = Paged(new, past, 2, D, 16, dtype, seed=D).fill(8)
+    q = randn(b.rows, 4, D, seed=9, dtype=dtype, scale=3.0)
+    want, tol = capped_want(b, q, D ** -0.5, cap)
+    got = g.paged_attention_device(q, b.k, b.v, *b.args(), b.max_kv, softcap=cap)
+    g.synchronize()
+    close(got, want, tol)
