@@ -45,6 +45,26 @@ struct PagedBatch {
     long long table_stride;
     int table_width;
 };
+// Sequence s of a batch. `ok`: its lengths are in order and it has new tokens; otherwise nothing of it is computed or
+// written. `report`: this thread records what is out of order.
+struct Sequence {
+    int row0, n_new, past;
+    bool ok;
+};
+__device__ __forceinline__ Sequence batch_sequence(const PagedBatch& b, int s, bool report, int* bad) {
+    Sequence q;
+    q.row0 = b.row_start[s];
+    const int end = b.row_start[s + 1], len = b.kv_len[s];
+    // 64-bit differences: the inputs are unchecked
+    const long long n = static_cast<long long>(end) - q.row0;
+    const bool rows_ok = q.row0 >= 0 && n >= 0 && end <= b.rows && n <= b.max_new;
+    const bool len_ok = len >= 0 && len <= b.max_kv && (n == 0 || len >= n);
+    if (report && !(rows_ok && len_ok)) record_bad(bad, rows_ok ? kBadLength : kBadRows);
+    q.ok = rows_ok && len_ok && n > 0;
+    q.n_new = static_cast<int>(n);
+    q.past = len - static_cast<int>(n);
+    return q;
+}
 struct PagedCache {
     void* k;
     void* v;

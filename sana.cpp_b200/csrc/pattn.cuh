@@ -34,24 +34,8 @@ struct Args {
     float2* ml;       // [splits][rows][q_heads]: (max, sum)
 };
 
-struct Sequence {
-    int row0, n_new, past;
-    bool ok;
-};
-// The checked lengths of sequence s; ok false: nothing of it is computed. `report`: this thread records why.
 __device__ __forceinline__ Sequence sequence(const PagedAttention& p, int s, bool report) {
-    Sequence q;
-    q.row0 = p.batch.row_start[s];
-    const int end = p.batch.row_start[s + 1], len = p.batch.kv_len[s];
-    // 64-bit differences: the inputs are unchecked
-    const long long n = static_cast<long long>(end) - q.row0;
-    const bool rows_ok = q.row0 >= 0 && n >= 0 && end <= p.batch.rows && n <= p.batch.max_new;
-    const bool len_ok = len >= 0 && len <= p.batch.max_kv && (n == 0 || len >= n);
-    if (report && !(rows_ok && len_ok)) record_bad(p.bad, rows_ok ? kBadLength : kBadRows);
-    q.ok = rows_ok && len_ok && n > 0;
-    q.n_new = static_cast<int>(n);
-    q.past = len - static_cast<int>(n);
-    return q;
+    return batch_sequence(p.batch, s, report, p.bad);
 }
 
 // The key tiles of packed rows [rr0, rr1) of a sequence.

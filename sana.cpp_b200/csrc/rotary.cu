@@ -54,20 +54,13 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) rotary_kernel(const __
     long long place = -1;  // element offset of the token's place in the cache
     if constexpr (APPEND) {
         const int S = p.batch.S;
+        // every sequence is checked by some block, its rows in the batch or not
+        for (long long i = row + tid * p.rows; i < S; i += kThreads * p.rows) batch_sequence(p.batch, static_cast<int>(i), true, p.bad);
         const int s = sequence_of(p.batch.row_start, S, row);
         if (s >= S) return;  // behind the last sequence
-        const int end = p.batch.row_start[s + 1], len = p.batch.kv_len[s];
-        const bool before = p.batch.row_start[s] > row;
-        if (before && s == 0) return;  // in front of the first sequence
-        if (before || end > p.rows) {
-            if (tid == 0) record_bad(p.bad, kBadRows);
-            return;
-        }
-        pos = len - (end - static_cast<int>(row));
-        if (len < 0 || len > p.batch.max_kv || pos < 0) {
-            if (tid == 0) record_bad(p.bad, kBadLength);
-            return;
-        }
+        const Sequence sq = batch_sequence(p.batch, s, false, p.bad);
+        if (!sq.ok || row < sq.row0) return;  // left out, or in front of the first sequence
+        pos = sq.past + static_cast<int>(row - sq.row0);
         const int slot = pos / p.cache.page_size;
         const int page = slot < p.batch.table_width ? p.batch.table[s * p.batch.table_stride + slot] : -1;
         if (page < 0 || page >= p.cache.pages) {

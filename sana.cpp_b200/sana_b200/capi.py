@@ -570,12 +570,15 @@ class SanaCuda:
                                 page_table.stride(0) if S > 1 else shape[1], shape[1])
 
     def rotary_append_device(self, q, k, v, frequencies, k_cache, v_cache, row_start, kv_len, page_table, max_new: int,
-                             interleaved: bool = False, magnitude: float = 1.0, inplace: bool = False):
+                             interleaved: bool = False, magnitude: float = 1.0, inplace: bool = False,
+                             max_kv: Optional[int] = None):
         """sana_op_rotary_append_device: turns q [rows, q_heads, D] (returned) and k, and writes k
         and v [rows, kv_heads, D] into their tokens' places in the caches [pages, page_size,
         kv_heads, D]. row_start [S + 1], kv_len [S] (the new tokens included) and page_table
         [S, pages of a sequence] are int32; frequencies None appends without turning (q is then
-        returned as it is)."""
+        returned as it is). A sequence of more than max_new new or max_kv cached tokens (None: only the
+        table bounds them) is left out and recorded. Without inplace, the returned q holds
+        anything in rows of no sequence or of one left out."""
         cache = self._cache(k_cache, v_cache)
         rows, heads = k.shape[0], 0
         kv, D, dt = cache.kv_heads, cache.head_dim, cache.dtype
@@ -589,8 +592,7 @@ class SanaCuda:
                 heads, qp = q.shape[1], q.data_ptr()
                 q_out = q if inplace else self._like_rows(q, ldq)
                 qo = q_out.data_ptr()
-        # the append reads each row's place from the lengths alone: any kv_len of the table is within bounds
-        batch = self._batch(rows, row_start, kv_len, page_table, max_new, 0x7fffffff)
+        batch = self._batch(rows, row_start, kv_len, page_table, max_new, 0x7fffffff if max_kv is None else max_kv)
         self._run("sana_op_rotary_append_device", rot, ctypes.byref(batch), ctypes.byref(cache), qp, ldq, heads, qo,
                   k.data_ptr(), ldk, v.data_ptr(), ldv)
         return q_out

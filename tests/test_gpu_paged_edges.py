@@ -104,3 +104,40 @@ def test_caps_large_against_the_scores(g, cap, dtype, D, new, past):
     got = g.paged_attention_device(q, b.k, b.v, *b.args(), b.max_kv, softcap=cap)
     g.synchronize()
     close(got, want, tol)
+
+
+# --- the append leaves out what attention leaves out ----------------------------------------------
+
+@pytest.mark.parametrize("starts, lens, max_new, max_kv, left_out", [
+    ([0, 2, 5], [8, 5], 2, 64, [1]),        # more new tokens than max_new
+    ([0, 2, 5], [8, 2], 3, 64, [1]),        # fewer tokens than new ones: none of them, not the first alone
+    ([0, 2, 5], [1, 5], 3, 64, [0]),
+    ([0, 2, 5], [8, 5], 3, 7, [0]),         # longer than max_kv
+    ([-1, 2, 5], [8, 5], 3, 64, [0]),       # begins in front of the rows
+    ([0, 2, 7], [8, 5], 9, 64, [1]),        # ends behind them
+    ([0, 2, 5, 8], [8, 5, 3], 3, 64, [2]),  # lies behind them
+    ([0, 2, 5, 5], [8, 5, -1], 3, 64, []),  # no new token, and a length that cannot be
+])
+@pytest.mark.parametrize("turned", [False, True])
+def test_append_leaves_out_whole_sequences(g, starts, lens, max_new, max_kv, left_out, turned):
+    """A sequence out of bounds is recorded, and none of its rows is written, as the header says."""
+    b = Paged([2, 3], [6, 2], 2, 64, 4, BF16, seed=1, fill=7.0)
+    table = torch.cat([b.table, b.table[:1]])[:len(lens)]
+    q, k, v = (randn(5, n, 64, seed=i, dtype=BF16) for i, n in enumerate((4, 2, 2)))
+    freq = torch.full((32,), 0.5, dtype=torch.float64, device="cuda") if turned else None
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    keep = q.clone()
+    out = g.rotary_append_device(q, k, v, freq, b.k, b.v, i32(starts), i32(lens), table, max_new, inplace=True, max_kv=max_kv)
+    with pytest.raises(ValueError, match="kv_len|row_start"):
+        g.synchronize()
+    g.synchronize()  # once
+    written = 0
+    for s, (n, p) in enumerate(zip(b.new, b.past)):
+        rows = slice(2 * s, 2 * s + n)
+        if s in left_out:
+            assert torch.equal(out[rows], keep[rows])
+            continue
+        assert torch.equal(b.v[b.places(s, p, p + n)], v[rows])
+        assert not turned or not torch.equal(out[rows], keep[rows])
+        written += n
+    assert (b.v != 7.0).any(-1).any(-1).sum().item() == written
