@@ -781,7 +781,7 @@ Args plan(const PagedAttention& p, Kind kind, int num_sms) {
     if (kind == kSimt && p.batch.S > 1) splits = 4 * slots / per;
     splits = std::max<long long>(1, std::min<long long>(splits, tiles / (kind == kSimt ? 2 : 3)));
     a.split_tiles = std::max(1, ceil_div(tiles, splits));
-    a.splits = ceil_div(tiles, a.split_tiles);
+    a.splits = std::max(1, ceil_div(tiles, a.split_tiles));  // (max_kv 0: the checks still run)
     return a;
 }
 

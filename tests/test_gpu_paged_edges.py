@@ -141,3 +141,19 @@ def test_append_leaves_out_whole_sequences(g, starts, lens, max_new, max_kv, lef
         assert not turned or not torch.equal(out[rows], keep[rows])
         written += n
     assert (b.v != 7.0).any(-1).any(-1).sum().item() == written
+
+
+@pytest.mark.parametrize("dtype, max_new", [(BF16, 1), (BF16, 200), (F32, 1)])
+def test_nothing_cached(g, dtype, max_new):
+    """A padded batch whose sequences are all empty, max_new its fixed bound: nothing is written or recorded. A token with
+    a length of 0 is recorded."""
+    b = Paged([0, 0, 0], [0, 0, 0], 2, 64, 16, dtype, seed=0)
+    q = randn(4, 4, 64, seed=1, dtype=dtype)
+    out = torch.full_like(q, 3.0)
+    g.paged_attention_device(q, b.k, b.v, b.row_start, b.kv_len, b.table, max_new, 0, out=out)
+    g.synchronize()
+    b.row_start[1:] = 1
+    g.paged_attention_device(q, b.k, b.v, b.row_start, b.kv_len, b.table, max_new, 0, out=out)
+    with pytest.raises(ValueError, match="kv_len"):
+        g.synchronize()
+    assert (out == 3.0).all()
