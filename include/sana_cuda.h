@@ -476,7 +476,8 @@ int sana_cuda_prompt_pairs_device(sana_cuda_ctx *ctx, int pairs, const float *ne
  * one batch, keys and values in a paged cache whose instruction prefix is computed once and
  * shared, and single tokens for prompt rewriting. No reference counterpart (llama.cpp's).
  *
- * All take device pointers of the handle's device (whatever device is current), queue their
+ * All take device pointers of the handle's device (whatever device is current), each aligned to its
+ * elements, queue their
  * work on the handle's stream, allocate nothing, never wait for the device and may be captured
  * into a CUDA graph. Argument errors that the host can see are SANA_ERR_INVALID and launch
  * nothing. What only the device sees (a page number outside the pool, a sequence longer than

@@ -1639,9 +1639,18 @@ namespace {
 
 bool act_dtype(int t) { return t == SANA_DTYPE_F32 || t == SANA_DTYPE_BF16; }
 
-// `rows` rows of `width` elements with stride ld
-void check_rows(const char* what, const void* ptr, long long rows, long long ld, long long width) {
+// A misaligned element would fault the device.
+void check_aligned(const char* what, const void* ptr, size_t bytes) {
+    if (reinterpret_cast<uintptr_t>(ptr) % bytes != 0)
+        throw sana::InvalidArg(std::string(what) + " must be aligned to its elements");
+}
+
+size_t dtype_bytes(int t) { return t == SANA_DTYPE_F32 ? 4 : t == SANA_DTYPE_BF16 ? 2 : 1; }
+
+// `rows` rows of `width` elements of a type with stride ld
+void check_rows(const char* what, const void* ptr, int dtype, long long rows, long long ld, long long width) {
     if (rows > 0 && !ptr) throw sana::InvalidArg(std::string(what) + " must not be NULL");
+    check_aligned(what, ptr, dtype_bytes(dtype));
     if (ld < width) throw sana::InvalidArg(std::string(what) + ": the row stride is below the row's width");
 }
 
@@ -1652,6 +1661,9 @@ sana::PagedBatch paged_batch_of(const sana_paged_batch* b) {
     SANA_REQUIRE(b->sequences == 0 || (b->row_start && b->kv_len && (b->page_table || b->table_width == 0)),
                  "row_start, kv_len and page_table must not be NULL");
     SANA_REQUIRE(b->table_stride >= b->table_width, "table_stride is below table_width");
+    check_aligned("row_start", b->row_start, sizeof(int));
+    check_aligned("kv_len", b->kv_len, sizeof(int));
+    check_aligned("page_table", b->page_table, sizeof(int));
     sana::PagedBatch o;
     o.S = b->sequences;
     o.rows = b->rows;
@@ -1671,6 +1683,8 @@ sana::PagedCache paged_cache_of(const sana_paged_cache* c) {
     SANA_REQUIRE(c->pages >= 0 && c->page_size >= 1 && c->kv_heads >= 1 && c->head_dim >= 1, "invalid cache sizes");
     SANA_REQUIRE(c->pages == 0 || (c->k && c->v), "k and v of the cache must not be NULL");
     SANA_REQUIRE(c->page_stride >= 0 && c->token_stride >= 0 && c->head_stride >= 0, "negative cache strides");
+    check_aligned("k of the cache", c->k, dtype_bytes(c->dtype));
+    check_aligned("v of the cache", c->v, dtype_bytes(c->dtype));
     sana::PagedCache o;
     o.k = c->k;
     o.v = c->v;
@@ -1690,6 +1704,7 @@ sana::Rotary rotary_of(const sana_rotary* r, int head_dim) {
     SANA_REQUIRE(r->rotated >= 0 && r->rotated % 2 == 0 && r->rotated <= head_dim && r->rotated <= 512,
                  "rotated must be even, at most head_dim and at most 512");
     SANA_REQUIRE(r->rotated == 0 || r->freq, "freq must not be NULL");
+    check_aligned("freq", r->freq, sizeof(double));
     sana::Rotary o;
     o.freq = r->freq;
     o.rotated = r->rotated;
@@ -1732,9 +1747,12 @@ int sana_op_add_rms_norm_device(sana_cuda_ctx* ctx, const void* x, int x_dtype, 
         SANA_REQUIRE(out_dtype == SANA_DTYPE_E4M3 || group == 0, "a group size goes with an E4M3 output only");
         SANA_REQUIRE(out_dtype != SANA_DTYPE_E4M3 || scale || rows == 0, "an E4M3 output needs scale");
         SANA_REQUIRE(residual || !sum, "sum needs a residual");
-        check_rows("x", x, rows, ldx, C);
-        check_rows("out", out, rows, ldo, C);
-        if (residual) check_rows("residual", residual, rows, ldr, C);
+        check_rows("x", x, x_dtype, rows, ldx, C);
+        check_rows("out", out, out_dtype, rows, ldo, C);
+        if (residual) check_rows("residual", residual, residual_dtype, rows, ldr, C);
+        check_aligned("sum", sum, residual ? dtype_bytes(residual_dtype) : 1);
+        check_aligned("weight", weight, sizeof(float));
+        check_aligned("scale", scale, sizeof(float));
         sana::AddRmsNorm p;
         p.x = x;
         p.residual = residual;
@@ -1792,14 +1810,15 @@ int sana_op_rotary_device(sana_cuda_ctx* ctx, const sana_rotary* rotary, int dty
         SANA_REQUIRE(static_cast<long long>(head_dim) * (static_cast<long long>(q_heads) + kv_heads) <= 0x3fffffffLL,
                      "a row is too wide");
         SANA_REQUIRE(positions || rows == 0, "positions must not be NULL");
+        check_aligned("positions", positions, sizeof(int));
         if (!k) kv_heads = 0;
         if (q_heads) {
-            check_rows("q", q, rows, ldq, static_cast<long long>(q_heads) * head_dim);
-            check_rows("q_out", q_out, rows, ldq, static_cast<long long>(q_heads) * head_dim);
+            check_rows("q", q, dtype, rows, ldq, static_cast<long long>(q_heads) * head_dim);
+            check_rows("q_out", q_out, dtype, rows, ldq, static_cast<long long>(q_heads) * head_dim);
         }
         if (kv_heads) {
-            check_rows("k", k, rows, ldk, static_cast<long long>(kv_heads) * head_dim);
-            check_rows("k_out", k_out, rows, ldk, static_cast<long long>(kv_heads) * head_dim);
+            check_rows("k", k, dtype, rows, ldk, static_cast<long long>(kv_heads) * head_dim);
+            check_rows("k_out", k_out, dtype, rows, ldk, static_cast<long long>(kv_heads) * head_dim);
         }
         sana::RotaryRows p{};
         p.rot = rotary_of(rotary, head_dim);
@@ -1840,11 +1859,11 @@ int sana_op_rotary_append_device(sana_cuda_ctx* ctx, const sana_rotary* rotary, 
             q_heads = 0;
         }
         const long long width = static_cast<long long>(p.cache.kv_heads) * p.cache.D;
-        check_rows("k", k, p.batch.rows, ldk, width);
-        check_rows("v", v, p.batch.rows, ldv, width);
+        check_rows("k", k, p.cache.dtype, p.batch.rows, ldk, width);
+        check_rows("v", v, p.cache.dtype, p.batch.rows, ldv, width);
         if (q_heads) {
-            check_rows("q", q, p.batch.rows, ldq, static_cast<long long>(q_heads) * p.cache.D);
-            check_rows("q_out", q_out, p.batch.rows, ldq, static_cast<long long>(q_heads) * p.cache.D);
+            check_rows("q", q, p.cache.dtype, p.batch.rows, ldq, static_cast<long long>(q_heads) * p.cache.D);
+            check_rows("q_out", q_out, p.cache.dtype, p.batch.rows, ldq, static_cast<long long>(q_heads) * p.cache.D);
         }
         p.dtype = p.cache.dtype;
         p.D = p.cache.D;
@@ -1871,8 +1890,8 @@ int sana_op_paged_attention_device(sana_cuda_ctx* ctx, const sana_paged_batch* b
     return guard(ctx, [&] {
         sana::PagedAttention p = paged_attention_of(batch, cache, q_heads, window, sinks);
         const long long width = static_cast<long long>(q_heads) * p.cache.D;
-        check_rows("q", q, p.batch.rows, ldq, width);
-        check_rows("out", out, p.batch.rows, ldo, width);
+        check_rows("q", q, p.cache.dtype, p.batch.rows, ldq, width);
+        check_rows("out", out, p.cache.dtype, p.batch.rows, ldo, width);
         SANA_REQUIRE(std::isfinite(scale), "scale must be finite");
         SANA_REQUIRE(softcap >= 0.f && std::isfinite(softcap), "softcap must be finite and not negative");
         SANA_REQUIRE(softcap == 0.f || std::abs(scale) <= 1e30f * softcap, "softcap is too small for the scale");
