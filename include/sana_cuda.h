@@ -477,9 +477,8 @@ int sana_cuda_prompt_pairs_device(sana_cuda_ctx *ctx, int pairs, const float *ne
  * shared, and single tokens for prompt rewriting. No reference counterpart (llama.cpp's).
  *
  * All take device pointers of the handle's device (whatever device is current), each aligned to its
- * elements, queue their
- * work on the handle's stream, allocate nothing, never wait for the device and may be captured
- * into a CUDA graph. Argument errors that the host can see are SANA_ERR_INVALID and launch
+ * elements, queue their work on the handle's stream, allocate nothing, never wait for the device
+ * and may be captured into a CUDA graph. Argument errors that the host can see are SANA_ERR_INVALID and launch
  * nothing. What only the device sees (a page number outside the pool, a sequence longer than
  * the table, more new tokens than `max_new` or than `rows`, an offset beyond the rows) is
  * checked there: the kernels access nothing out of range, leave out the keys or rows
@@ -497,7 +496,8 @@ enum { SANA_DTYPE_F32 = 0, SANA_DTYPE_BF16 = 1, SANA_DTYPE_E4M3 = 2 };
  * ldo, F32, BF16, or E4M3 with scale: fp32 [rows, ceil(C / group)] (contiguous), one scale per
  * `group` channels of a row, the last group possibly shorter; group 0 is the whole row:
  *   scale = max(max|y| / 448, 2^-100),  out = y / scale rounded to nearest even.
- * A NaN among a group's y makes its scale and values NaN. out may be x where the types agree.
+ * A NaN among a group's y makes its scale and values NaN. out may be x where types and row
+ * strides agree, and must overlap no other operand.
  * 1 <= C <= 16384. */
 int sana_op_add_rms_norm_device(sana_cuda_ctx *ctx, const void *x, int x_dtype, long long ldx, const void *residual,
                                 int residual_dtype, long long ldr, void *sum, const float *weight,

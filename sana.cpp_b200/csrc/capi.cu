@@ -1753,6 +1753,9 @@ int sana_op_add_rms_norm_device(sana_cuda_ctx* ctx, const void* x, int x_dtype, 
         check_aligned("sum", sum, residual ? dtype_bytes(residual_dtype) : 1);
         check_aligned("weight", weight, sizeof(float));
         check_aligned("scale", scale, sizeof(float));
+        // rows are read and written by blocks of their own: in place only where every row stays in its place
+        SANA_REQUIRE(out != x || rows <= 1 || (out_dtype == x_dtype && ldo == ldx),
+                     "out may be x only with x's type and row stride");
         sana::AddRmsNorm p;
         p.x = x;
         p.residual = residual;

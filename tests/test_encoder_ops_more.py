@@ -45,3 +45,12 @@ def test_append_refuses_misaligned_rows(handle, change, word):
     a = {**dict(q=PTR, ldq=512, heads=8, qo=PTR, k=PTR, ldk=128, v=PTR, ldv=128), **change}
     assert lib.sana_op_rotary_append_device(h, ctypes.byref(r), ctypes.byref(b), ctypes.byref(c), *a.values()) == INVALID
     assert word in message(lib, h)
+
+
+@pytest.mark.parametrize("change", [dict(ldx=72), dict(ldo=72), dict(ot=1), dict(ot=2, scale=PTR)])
+def test_norm_in_place_needs_the_same_rows(handle, change):
+    """Another row stride or element size would write rows that other blocks still read."""
+    lib, h, created = handle
+    assert lib.sana_op_add_rms_norm_device(h, *{**NORM, **change}.values()) == INVALID and "out may be x" in message(lib, h)
+    if not created:  # a single row may: the argument check passes, and the missing device is reported
+        assert lib.sana_op_add_rms_norm_device(h, *{**NORM, **change, "rows": 1}.values()) == 4
