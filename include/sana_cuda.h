@@ -495,7 +495,7 @@ enum { SANA_DTYPE_F32 = 0, SANA_DTYPE_BF16 = 1, SANA_DTYPE_E4M3 = 2 };
  * weight [C] fp32 or NULL (ones; weight_offset is then ignored). out [rows, C], row stride
  * ldo, F32, BF16, or E4M3 with scale: fp32 [rows, ceil(C / group)] (contiguous), one scale per
  * `group` channels of a row, the last group possibly shorter; group 0 is the whole row:
- *   scale = max(max|y| / 448, 2^-100),  out = y / scale rounded to nearest even.
+ *   scale = max(max|y| / 448, 2^-100),  out = y / scale (a quotient in fp32) rounded to nearest even.
  * A NaN among a group's y makes its scale and values NaN. out may be x where types and row
  * strides agree, and must overlap no other operand.
  * 1 <= C <= 16384. */

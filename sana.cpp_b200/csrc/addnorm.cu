@@ -159,19 +159,27 @@ __global__ void __launch_bounds__(1024) add_rms_norm_kernel(const TX* x, const T
             if (c >= a.C) continue;
             const int g = c / a.group;
             const float s = max_nan(__uint_as_float(gmax[g]) / kE4M3Max, kScaleFloor);
-            const float inv_s = 1.0f / s;
+            // y / s in fp32 from the group's reciprocal and one residual (Markstein 1990): quotients that
+            // fp32 holds come out exact, so that those midway between two e4m3 values go to the even one, which
+            // the product alone can miss. Where s is infinite the residual is left at y, and finite y give 0.
+            // 38400 x 2304, device time: 148.2 us, 146.9 with the product alone, 155.8 with divisions.
+            const float inv_s = 1.0f / s, minus_s = s < INFINITY ? -s : 0.f;
+            auto quotient = [&](float y) {
+                const float q = y * inv_s;
+                return fmaf(fmaf(q, minus_s, y), inv_s, q);
+            };
             if (c == g * a.group) a.scale[row * a.groups + g] = s;
             TO* o = out + row * a.ldo + c;
             if constexpr (VEC == 1) {
-                *reinterpret_cast<__nv_fp8_storage_t*>(o) = __nv_cvt_float_to_fp8(h[i][0] * inv_s, __NV_SATFINITE, __NV_E4M3);
+                *reinterpret_cast<__nv_fp8_storage_t*>(o) = __nv_cvt_float_to_fp8(quotient(h[i][0]), __NV_SATFINITE, __NV_E4M3);
             } else {
                 uint32_t w[2];
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(h[i][4 * j] * inv_s, h[i][4 * j + 1] * inv_s),
+                    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(quotient(h[i][4 * j]), quotient(h[i][4 * j + 1])),
                                                                  __NV_SATFINITE, __NV_E4M3);
                     const uint32_t hi = __nv_cvt_float2_to_fp8x2(
-                        make_float2(h[i][4 * j + 2] * inv_s, h[i][4 * j + 3] * inv_s), __NV_SATFINITE, __NV_E4M3);
+                        make_float2(quotient(h[i][4 * j + 2]), quotient(h[i][4 * j + 3])), __NV_SATFINITE, __NV_E4M3);
                     w[j] = lo | (hi << 16);
                 }
                 *reinterpret_cast<uint2*>(o) = make_uint2(w[0], w[1]);
