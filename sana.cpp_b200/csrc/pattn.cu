@@ -763,7 +763,7 @@ Args plan(const PagedAttention& p, Kind kind, int num_sms) {
         a.align = std::max(1, copy_box(p.cache, a.BM));  // a group brings as many keys as a block has rows
         resident = p.cache.D > 128 ? 1 : 2;
     }
-    a.row_tiles = ceil_div(packed, a.BM);
+    a.row_tiles = std::max(1, ceil_div(packed, a.BM));  // (max_new 0: the checks still run)
     const long long span = p.window > 0 ? std::min<long long>(p.batch.max_kv, static_cast<long long>(p.window) + p.batch.max_new +
                                                                                  p.sinks)
                                         : p.batch.max_kv;
@@ -907,7 +907,7 @@ size_t paged_attention_workspace(const PagedAttention& p, int num_sms) {
 
 void paged_attention(PagedAttention p, int num_sms, cudaStream_t st) {
     p.page_div = page_divisor(p.cache.page_size);
-    if (p.batch.S == 0 || p.batch.rows == 0 || p.batch.max_new == 0) return;
+    if (p.batch.S == 0 || p.batch.rows == 0) return;
     const bool mma = cache_fits_mma(p.cache) && (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 &&
                      (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.ldq % 8 == 0 && p.ldo % 8 == 0;
     // the tcgen05 kernel maps a tile's largest score alone, which takes a map that rises: scale > 0; and it has the cheap

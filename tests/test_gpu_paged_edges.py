@@ -157,3 +157,38 @@ def test_nothing_cached(g, dtype, max_new):
     with pytest.raises(ValueError, match="kv_len"):
         g.synchronize()
     assert (out == 3.0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("max_kv", [0, 64])
+def test_no_new_tokens_allowed(g, dtype, max_kv):
+    """max_new 0: sequences without new tokens are left alone, others are recorded and left out, by both operators."""
+    b = Paged([2, 0], [6, 2], 2, 64, 16, dtype, seed=0, fill=7.0)
+    q, k = randn(2, 4, 64, seed=1, dtype=dtype), randn(2, 2, 64, seed=2, dtype=dtype)
+    out = torch.full_like(q, 3.0)
+    for starts in ([0, 0, 0], [0, 2, 2]):
+        row_start = torch.tensor(starts, dtype=torch.int32, device="cuda")
+        for call in (lambda: g.paged_attention_device(q, b.k, b.v, row_start, b.kv_len, b.table, 0, max_kv, out=out),
+                     lambda: g.rotary_append_device(None, k, k, None, b.k, b.v, row_start, b.kv_len, b.table, 0, max_kv=max_kv)):
+            call()
+            if starts[1] or max_kv == 0:
+                with pytest.raises(ValueError, match="row_start" if starts[1] else "kv_len"):
+                    g.synchronize()
+            g.synchronize()
+    assert (out == 3.0).all() and (b.k == 7.0).all() and (b.v == 7.0).all()
+
+
+# --- a chunk and single tokens in one batch -------------------------------------------------------
+
+@pytest.mark.parametrize("dtype, D", [(BF16, 64), (BF16, 128), (BF16, 256), (F32, 64)])
+@pytest.mark.parametrize("new, past", [([300, 1], [10, 3000]), ([1, 1, 40, 1], [2500, 900, 0, 17]), ([1, 130, 1], [4000, 70, 1300])])
+@pytest.mark.parametrize("window, sinks", [(0, 0), (700, 5)])
+@pytest.mark.parametrize("page", [16, 24])
+def test_chunks_and_single_tokens_in_one_batch(g, dtype, D, new, past, window, sinks, page):
+    """One launch for all, whose tiles and splits are the longest ones': each row as it would be alone."""
+    b = Paged(new, past, 2, D, page, dtype, seed=D).fill(3)
+    q = randn(b.rows, 4, D, seed=9, dtype=dtype, scale=2.0)
+    got = g.paged_attention_device(q, b.k, b.v, *b.args(), b.max_kv, window=window, sinks=sinks)
+    g.synchronize()
+    want, tol = attention_want(b, q, D ** -0.5, window, sinks, 0.0)
+    close(got, want, tol + want.abs() * 2 * U[dtype])
