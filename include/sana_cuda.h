@@ -491,7 +491,7 @@ enum { SANA_DTYPE_F32 = 0, SANA_DTYPE_BF16 = 1, SANA_DTYPE_E4M3 = 2 };
  *   y = h / sqrt(mean(h^2) + eps) * (weight + weight_offset)       (mean and root in fp32)
  * x F32 or BF16, row stride ldx elements. residual F32 or BF16 [rows, C], row stride ldr, or
  * NULL (h = x, residual_dtype ignored). sum receives h in the residual's type with row stride
- * ldr; it may be residual itself (in place), must not overlap it otherwise, and may be NULL.
+ * ldr; it may be residual itself (in place), must overlap no operand otherwise, and may be NULL.
  * weight [C] fp32 or NULL (ones; weight_offset is then ignored). out [rows, C], row stride
  * ldo, F32, BF16, or E4M3 with scale: fp32 [rows, ceil(C / group)] (contiguous), one scale per
  * `group` channels of a row, the last group possibly shorter; group 0 is the whole row:
@@ -520,7 +520,7 @@ int sana_rotary_frequencies(int rotated, double base, int scaling, double stretc
 /* How heads are turned: the first `rotated` channels of each head (even, <= head_dim; the
  * rest stays), as pairs (i, i + rotated/2), or (2i, 2i+1) with interleaved != 0:
  *   y_a = m (x_a cos t - x_b sin t), y_b = m (x_b cos t + x_a sin t),  t = position * freq[i]
- * with the product and its reduction in 64 bits. freq: device, rotated/2 doubles; magnitude
+ * with the product and its reduction in 64 bits, sine and cosine in fp32. freq: device, rotated/2 doubles; magnitude
  * m scales the turned channels (1 for none). */
 typedef struct sana_rotary {
     const double *freq;
@@ -556,8 +556,9 @@ typedef struct sana_paged_cache {
  * device; entries behind a sequence's last page are not read, and neither are entries that no
  * new token sees. max_new and max_kv are upper bounds of the new and of the cached tokens of
  * any sequence (they size the launch; a sequence beyond them is recorded and left out). Rows in
- * front of the first sequence and behind the last are left as they were. A sequence may have no
- * new token. */
+ * front of the first sequence and behind the last are left as they were, so that a part of a
+ * batch is the same arrays from its first sequence on. A sequence may have no new token. Without
+ * rows nothing is launched. */
 typedef struct sana_paged_batch {
     int sequences, rows, max_new, max_kv;
     const int *row_start;
@@ -581,14 +582,19 @@ int sana_op_rotary_append_device(sana_cuda_ctx *ctx, const sana_rotary *rotary, 
  *   out = softmax_j(s_j) v_j,  s_j = scale q.k_j, or softcap * tanh(scale q.k_j / softcap)
  * with softcap > 0. Query head h reads cache head h / (q_heads / kv_heads). q and out
  * [rows, q_heads, head_dim] of the cache's dtype, row strides ldq, ldo (out must not overlap
- * q); scores, softmax statistics and sums are fp32. What a token does not see does not reach
- * its output, be it NaN or infinite; a token that sees nothing gets zeros. head_dim <= 256.
- * BF16 with head_dim a multiple of 8 and 16-byte aligned pointers and strides runs on the
- * tensor cores (pages whose size divides 128, or is a multiple of it, and is at least 8, are the
- * fast ones there), the rest on the CUDA cores. workspace: device, 16-byte aligned,
- * sana_op_paged_attention_workspace() bytes of the same batch, cache, heads, window and sinks
- * (0 bytes, which invalid arguments give too: may be NULL); its contents need no preparation and nothing is kept in it, but two
- * calls that may overlap (two streams, two graphs in flight) need one each. */
+ * q). Scores, softmax statistics and sums are fp32; on the tensor cores the probabilities are
+ * rounded to bf16 before they meet the values, and in chunks with head_dim <= 64 the divisor is
+ * the sum of the unrounded ones. What a token does not see does not reach its output, be it NaN
+ * or infinite; a token that sees nothing gets zeros. head_dim <= 256. BF16 with head_dim a
+ * multiple of 8 and 16-byte aligned pointers and strides runs on the tensor cores (pages whose
+ * size divides 128, or is a multiple of it, and is at least 8, are the fast ones there: chunks
+ * over others take 1.6 to 2.7 times as long), the rest on the CUDA cores. One plan serves the whole
+ * batch, by max_new and max_kv: single tokens far behind should not share a call with a long
+ * chunk, but take one of their own over their part of the batch. workspace: device, 16-byte
+ * aligned, sana_op_paged_attention_workspace() bytes of the same batch, cache, heads, window and
+ * sinks (0 bytes, which invalid arguments give too: may be NULL); its contents need no preparation
+ * and nothing is kept in it, but two calls that may overlap (two streams, two graphs in flight)
+ * need one each. */
 int sana_op_paged_attention_device(sana_cuda_ctx *ctx, const sana_paged_batch *batch, const sana_paged_cache *cache,
                                    const void *q, long long ldq, int q_heads, float scale, int window, int sinks,
                                    float softcap, void *out, long long ldo, void *workspace, size_t workspace_bytes);

@@ -7,7 +7,7 @@
 // written once; the sum of squares is fp32, each thread's elements first, then a fixed tree over
 // lanes and warps (the same bits every run). h is rounded before it is squared so that the norm is
 // that of the stream a later reader sees; y is rounded once, at its store. Bound by HBM for many rows
-// (38400 x 2304, bf16 + fp32 stream to e4m3 with a scale per 128: 162 to 169 us, 5.8 to 6.0 TB/s), by the launch for few.
+// (38400 x 2304, bf16 + fp32 stream to e4m3 with a scale per 128: 163 to 172 us a call, 5.7 to 6.0 TB/s), by the launch for few.
 #include <cuda_fp8.h>
 
 #include "encoder.h"

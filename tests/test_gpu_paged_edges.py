@@ -193,3 +193,16 @@ def test_chunks_and_single_tokens_in_one_batch(g, dtype, D, new, past, window, s
     g.synchronize()
     want, tol = attention_want(b, q, D ** -0.5, window, sinks, 0.0)
     close(got, want, tol + want.abs() * 2 * U[dtype])
+
+
+def test_a_batch_in_two_calls(g):
+    """Chunks and single tokens of one batch in a call each, over their parts of the same arrays: together all rows."""
+    b = Paged([200, 30, 1, 1, 1], [10, 40, 3000, 500, 0], 2, 128, 16, BF16, seed=2, trailing=2).fill(3)
+    q = randn(b.rows, 8, 128, seed=9, dtype=BF16, scale=2.0)
+    out = torch.full_like(q, 5.0)
+    for lo, hi, max_new, max_kv in ((0, 2, 200, 210), (2, 5, 1, 3001)):
+        g.paged_attention_device(q, b.k, b.v, b.row_start[lo:hi + 1], b.kv_len[lo:hi], b.table[lo:hi], max_new, max_kv, out=out)
+    g.synchronize()
+    want, tol = attention_want(b, q, 128 ** -0.5, 0, 0, 0.0)
+    close(out[:-2], want[:-2], (tol + want.abs() * 2 * U[BF16])[:-2])
+    assert (out[-2:] == 5.0).all()
