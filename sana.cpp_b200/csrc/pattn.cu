@@ -669,7 +669,7 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
     int active = 0;
     if (s < p.batch.S) {
         const Sequence sq = sequence(p, s, false);
-        if (sq.ok && row >= sq.row0) {
+        if (sq.ok && row >= sq.row0 && row - sq.row0 < sq.n_new) {
             const int rr = (row - sq.row0) * a.G + h % a.G, tile = rr / a.BM;
             const KeyTiles kt = key_tiles(sq.past, sq.n_new, a.G, tile * a.BM, (tile + 1) * a.BM, p.window, p.sinks, a.BN, a.align);
             active = (kt.n + a.split_tiles - 1) / a.split_tiles;

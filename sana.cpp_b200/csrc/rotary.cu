@@ -59,7 +59,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) rotary_kernel(const __
         const int s = sequence_of(p.batch.row_start, S, row);
         if (s >= S) return;  // behind the last sequence
         const Sequence sq = batch_sequence(p.batch, s, false, p.bad);
-        if (!sq.ok || row < sq.row0) return;  // left out, or in front of the first sequence
+        // left out, in front of the first sequence, or of none that holds it (row_start not ascending)
+        if (!sq.ok || row < sq.row0 || row - sq.row0 >= sq.n_new) return;
         pos = sq.past + static_cast<int>(row - sq.row0);
         const int slot = pos / p.cache.page_size;
         const int page = slot < p.batch.table_width ? p.batch.table[s * p.batch.table_stride + slot] : -1;

@@ -206,3 +206,26 @@ def test_a_batch_in_two_calls(g):
     want, tol = attention_want(b, q, 128 ** -0.5, 0, 0, 0.0)
     close(out[:-2], want[:-2], (tol + want.abs() * 2 * U[BF16])[:-2])
     assert (out[-2:] == 5.0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_row_start_that_descends(g, dtype):
+    """Recorded by both operators. The append writes no row at a place that is not its sequence's: a row is looked up by
+    the ends, and the last sequence (rows 4 and 5) is not the one that holds rows 7 and 8."""
+    b = Paged([2, 7, 0, 2], [6, 2, 3, 50], 2, 64, 16, dtype, seed=1, fill=7.0)
+    starts = torch.tensor([0, 2, 9, 4, 6], dtype=torch.int32, device="cuda")
+    q, k = randn(10, 4, 64, seed=1, dtype=dtype), randn(10, 2, 64, seed=2, dtype=dtype)
+    out = torch.full_like(q, 3.0)
+    g.rotary_append_device(None, k, k, None, b.k, b.v, starts, b.kv_len, b.table, 7, max_kv=64)
+    with pytest.raises(ValueError, match="row_start"):
+        g.synchronize()
+    assert torch.equal(b.v[b.places(0, 6, 8)], k[:2])
+    page, slot = b.places(3, 0, 64)  # the last sequence's page: its own two tokens at most
+    kept = (b.v[page, slot] == 7.0).flatten(1).all(1)
+    assert kept[:50].all() and kept[52:].all()
+    b.v.fill_(0.0)
+    b.k.fill_(0.0)
+    g.paged_attention_device(q, b.k, b.v, starts, b.kv_len, b.table, 7, 64, out=out)
+    with pytest.raises(ValueError, match="row_start"):
+        g.synchronize()
+    assert (out[9:] == 3.0).all()
