@@ -476,14 +476,14 @@ int sana_cuda_prompt_pairs_device(sana_cuda_ctx *ctx, int pairs, const float *ne
  * one batch, keys and values in a paged cache whose instruction prefix is computed once and
  * shared, and single tokens for prompt rewriting. No reference counterpart (llama.cpp's).
  *
- * All take device pointers of the handle's device (whatever device is current), each aligned to its
- * elements, queue their work on the handle's stream, allocate nothing, never wait for the device
- * and may be captured into a CUDA graph. Argument errors that the host can see are SANA_ERR_INVALID and launch
- * nothing. What only the device sees (a page number outside the pool, a sequence longer than
- * the table, more new tokens than `max_new` or than `rows`, an offset beyond the rows) is
- * checked there: the kernels access nothing out of range, leave out the keys or rows
- * concerned, and record it; the next sana_cuda_synchronize (or host-buffer call) of the handle
- * returns SANA_ERR_INVALID once and clears the record. */
+ * All take device pointers of the handle's device (whatever device is current), each aligned to
+ * its elements, queue their work on the handle's stream, allocate nothing, never wait for the
+ * device and may be captured into a CUDA graph. Argument errors that the host can see are
+ * SANA_ERR_INVALID and launch nothing. What only the device sees (a page number outside the
+ * pool, a sequence longer than the table, more new tokens than `max_new` or than `rows`, an
+ * offset beyond the rows) is checked there: the kernels access nothing out of range, leave out
+ * the keys or rows concerned, and record it; the next sana_cuda_synchronize (or host-buffer call)
+ * of the handle returns SANA_ERR_INVALID once and clears the record. */
 enum { SANA_DTYPE_F32 = 0, SANA_DTYPE_BF16 = 1, SANA_DTYPE_E4M3 = 2 };
 
 /* Residual addition and root-mean-square norm of rows x [rows, C] in one pass:
@@ -520,8 +520,8 @@ int sana_rotary_frequencies(int rotated, double base, int scaling, double stretc
 /* How heads are turned: the first `rotated` channels of each head (even, <= head_dim; the
  * rest stays), as pairs (i, i + rotated/2), or (2i, 2i+1) with interleaved != 0:
  *   y_a = m (x_a cos t - x_b sin t), y_b = m (x_b cos t + x_a sin t),  t = position * freq[i]
- * with the product and its reduction in 64 bits, sine and cosine in fp32. freq: device, rotated/2 doubles; magnitude
- * m scales the turned channels (1 for none). */
+ * with the product and its reduction in 64 bits, sine and cosine in fp32. freq: device,
+ * rotated/2 doubles; magnitude m scales the turned channels (1 for none). */
 typedef struct sana_rotary {
     const double *freq;
     int rotated;

@@ -237,12 +237,13 @@ __device__ __forceinline__ float wide_cap_log2(float x, float to_z, float scale_
     return fabsf(z) < 0.25f ? x * scale_log2 * series : soft_cap_log2(z, kTwoLog2e, cap_log2);
 }
 
-// DP: padded head size. WIDE: soft caps beyond kCheapCap, a kernel of its own (as a branch, or for every cap, it cost single
-// tokens at head size 256 3 %: 428 us for 64 behind 100 to 16000 tokens, 414 without). Groups of WM warps (16 rows each) share out each step's 64 keys, 4 / WM
-// groups: a single token's few rows keep all four warps busy on different keys. Every group runs
-// on its own: it brings its keys and values into its own ring of ST tiles, waits for them alone
-// (no block barrier in the loop), and every warp has its own softmax; the groups' results are
-// joined once at the end. P is rounded to bf16 for the second product.
+// DP: padded head size. WIDE: soft caps beyond kCheapCap, a kernel of its own (as a branch, or for every cap, it cost
+// single tokens at head size 256 3 %: 428 us for 64 behind 100 to 16000 tokens, 414 without). Groups of WM warps (16
+// rows each) share out each step's 64 keys, 4 / WM groups: a single token's few rows keep all four
+// warps busy on different keys. Every group runs on its own: it brings its keys and values into its
+// own ring of ST tiles, waits for them alone (no block barrier in the loop), and every warp has its
+// own softmax; the groups' results are joined once at the end. P is rounded to bf16 for the second
+// product.
 //
 // Keys and values sit in slabs of 64 channels, rows of 128 bytes whose 16-byte chunks are swapped
 // by the row number (c ^ (r & 7)), so that ldmatrix meets no bank twice. TMA: a page's keys come by
